@@ -64,6 +64,46 @@ class FlashParams(ctypes.Structure):
     ]
 
 
+class VarlenParams(ctypes.Structure):
+    _fields_ = [
+        ("q", SageTensor), ("k", SageTensor), ("v", SageTensor), ("out", SageTensor),
+        ("log_normalizer", ctypes.c_void_p), ("cu_seqlens_q", ctypes.c_void_p), ("cu_seqlens_k", ctypes.c_void_p),
+        ("seqs", c_i64), ("total_q", c_i64), ("total_k", c_i64), ("heads_q", c_i64), ("heads_kv", c_i64), ("head_dim", c_i64),
+        ("dtype", c_i32), ("causal", c_i32),
+        ("sm_scale", ctypes.c_float),
+    ]
+
+
+class PagedParams(ctypes.Structure):
+    _fields_ = [
+        ("q", SageTensor), ("out", SageTensor), ("k_cache", SageTensor), ("v_cache", SageTensor),
+        ("log_normalizer", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p),
+        ("table_stride", c_i64), ("seqs", c_i64), ("new_tokens", c_i64), ("heads_q", c_i64), ("heads_kv", c_i64),
+        ("head_dim", c_i64), ("pages", c_i64), ("page_size", c_i64), ("table_width", c_i64),
+        ("dtype", c_i32),
+        ("sm_scale", ctypes.c_float),
+    ]
+
+
+class AppendParams(ctypes.Structure):
+    _fields_ = [
+        ("k", SageTensor), ("v", SageTensor), ("k_cache", SageTensor), ("v_cache", SageTensor),
+        ("slots", ctypes.c_void_p),
+        ("tokens", c_i64), ("heads_kv", c_i64), ("head_dim", c_i64), ("pages", c_i64), ("page_size", c_i64),
+        ("dtype", c_i32), ("slots_int64", c_i32),
+    ]
+
+
+class CopyParams(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p),
+        ("k_stride_layer", c_i64), ("k_stride_page", c_i64), ("v_stride_layer", c_i64), ("v_stride_page", c_i64),
+        ("src", ctypes.c_void_p), ("dst", ctypes.c_void_p),
+        ("count", c_i64), ("layers", c_i64), ("pages", c_i64), ("page_bytes", c_i64),
+        ("src_int64", c_i32), ("dst_int64", c_i32),
+    ]
+
+
 EXPORTS = (
     "sage_per_block_int8",
     "sage_per_block_int8_smooth_k",
@@ -83,6 +123,11 @@ EXPORTS = (
     "sage_k_mean",
     "sage_k_mean_workspace_bytes",
     "sage_k_mean_noalloc",
+    "sage_flash_varlen_fwd",
+    "sage_paged_attn_workspace_bytes",
+    "sage_paged_attn",
+    "sage_cache_append",
+    "sage_cache_copy_pages",
     "sage_hip_last_error",
     "sage_hip_abi_version",
 )
@@ -148,6 +193,16 @@ def load():
     lib.sage_k_mean_noalloc.argtypes = [ctypes.POINTER(SageTensor), c_i32, ctypes.c_void_p, c_i32, c_i64, c_i64, c_i64,
                                         c_i64, ctypes.c_void_p]
     lib.sage_k_mean_noalloc.restype = ctypes.c_int
+    lib.sage_flash_varlen_fwd.argtypes = [ctypes.POINTER(VarlenParams), ctypes.c_void_p]
+    lib.sage_flash_varlen_fwd.restype = ctypes.c_int
+    lib.sage_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedParams)]
+    lib.sage_paged_attn_workspace_bytes.restype = c_i64
+    lib.sage_paged_attn.argtypes = [ctypes.POINTER(PagedParams), ctypes.c_void_p, c_i64, ctypes.c_void_p]
+    lib.sage_paged_attn.restype = ctypes.c_int
+    lib.sage_cache_append.argtypes = [ctypes.POINTER(AppendParams), ctypes.c_void_p]
+    lib.sage_cache_append.restype = ctypes.c_int
+    lib.sage_cache_copy_pages.argtypes = [ctypes.POINTER(CopyParams), ctypes.c_void_p]
+    lib.sage_cache_copy_pages.restype = ctypes.c_int
     if lib.sage_hip_abi_version() != ABI_VERSION:
         raise ImportError(f"{LIB_PATH}: ABI version {lib.sage_hip_abi_version()} != {ABI_VERSION}; rebuild it")
     _lib = lib

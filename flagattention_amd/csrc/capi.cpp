@@ -278,3 +278,102 @@ static int check_flash_params(const sage_flash_params* p, bool forward) {
         return fail(SAGE_E_INVALID, "sage_flash_attn_fwd: out rows must be 16-byte aligned");
     return SAGE_OK;
 }
+
+// ---- packed sequences and paged caches
+
+static bool misaligned_row(const sage_tensor& t, int esz) {
+    return ((uintptr_t)t.ptr % 16) != 0 || (t.stride_b * esz) % 16 != 0 || (t.stride_h * esz) % 16 != 0 || (t.stride_n * esz) % 16 != 0;
+}
+
+static int check_heads(const char* who, int64_t heads_q, int64_t heads_kv, int64_t head_dim, int32_t dtype, float sm_scale) {
+    if (head_dim != 64 && head_dim != 128)
+        return fail(SAGE_E_UNSUPPORTED, "%s: head_dim %lld not supported (64 or 128)", who, (long long)head_dim);
+    if (heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0)
+        return fail(SAGE_E_INVALID, "%s: heads_q %lld is not a positive multiple of heads_kv %lld", who, (long long)heads_q, (long long)heads_kv);
+    if (heads_q > (1 << 16)) return fail(SAGE_E_UNSUPPORTED, "%s: more than 65536 heads", who);
+    if (dtype != SAGE_F16 && dtype != SAGE_BF16) return fail(SAGE_E_UNSUPPORTED, "%s: q, k, v must be fp16 or bf16", who);
+    if (!(sm_scale > 0.0f) || !(sm_scale < 3.0e38f)) return fail(SAGE_E_INVALID, "%s: sm_scale must be positive and finite", who);
+    return SAGE_OK;
+}
+
+extern "C" int sage_flash_varlen_fwd(const sage_varlen_params* p, void* stream) {
+    const char* who = "sage_flash_varlen_fwd";
+    if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
+    if (int rc = check_heads(who, p->heads_q, p->heads_kv, p->head_dim, p->dtype, p->sm_scale)) return rc;
+    if (p->seqs < 0 || p->total_q < 0 || p->total_k < 0) return fail(SAGE_E_INVALID, "%s: negative size", who);
+    if (p->seqs == 0 || p->total_q == 0) return SAGE_OK;  // (no row to write)
+    if (!p->q.ptr || !p->out.ptr || !p->cu_seqlens_q || !p->cu_seqlens_k || (p->total_k > 0 && (!p->k.ptr || !p->v.ptr)))
+        return fail(SAGE_E_INVALID, "%s: null pointer", who);
+    const int64_t lim = 1LL << 30;
+    if (p->seqs >= lim || p->total_k >= lim || p->total_q >= lim || p->total_q * (p->heads_q / p->heads_kv) >= lim)
+        return fail(SAGE_E_UNSUPPORTED, "%s: seqs, total_k and total_q x heads_q / heads_kv must stay below 2^30", who);
+    if (misaligned_row(p->q, 2) || misaligned_row(p->k, 2) || misaligned_row(p->v, 2) || misaligned_row(p->out, 2))
+        return fail(SAGE_E_INVALID, "%s: rows of q, k, v and out must be 16-byte aligned", who);
+    if (p->k.stride_n < 0 || p->v.stride_n < 0 || p->k.stride_n >= (1LL << 24) || p->v.stride_n >= (1LL << 24))
+        return fail(SAGE_E_UNSUPPORTED, "%s: token stride of k or v out of range for 32-bit tile offsets", who);
+    return launch_flash_varlen(*p, (hipStream_t)stream);
+}
+
+// nothing: the call is valid and has no row to compute
+static int check_paged(const char* who, const sage_paged_params* p, bool& nothing) {
+    nothing = false;
+    if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
+    if (int rc = check_heads(who, p->heads_q, p->heads_kv, p->head_dim, p->dtype, p->sm_scale)) return rc;
+    if (p->seqs < 0 || p->new_tokens < 0 || p->pages < 0 || p->table_width < 0) return fail(SAGE_E_INVALID, "%s: negative size", who);
+    if (p->page_size <= 0) return fail(SAGE_E_INVALID, "%s: page_size must be positive", who);
+    nothing = p->seqs == 0 || p->new_tokens == 0;
+    if (nothing) return SAGE_OK;
+    if (p->pages == 0 || p->table_width == 0) return fail(SAGE_E_INVALID, "%s: a cache without pages or a table without entries", who);
+    if (!p->q.ptr || !p->out.ptr || !p->k_cache.ptr || !p->v_cache.ptr || !p->block_table || !p->seq_lens)
+        return fail(SAGE_E_INVALID, "%s: null pointer", who);
+    const int64_t lim = 1LL << 30;
+    if (p->seqs >= lim || p->new_tokens >= lim || p->new_tokens * (p->heads_q / p->heads_kv) >= lim || p->pages >= lim || p->page_size >= lim ||
+        p->table_width >= lim)
+        return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30", who);
+    if (misaligned_row(p->q, 2) || misaligned_row(p->out, 2) || misaligned_row(p->k_cache, 2) || misaligned_row(p->v_cache, 2))
+        return fail(SAGE_E_INVALID, "%s: rows of q, out and the caches must be 16-byte aligned", who);
+    return SAGE_OK;
+}
+
+extern "C" int64_t sage_paged_attn_workspace_bytes(const sage_paged_params* p) {
+    bool nothing;
+    if (check_paged("sage_paged_attn_workspace_bytes", p, nothing)) return -1;
+    return nothing ? 0 : paged_workspace_bytes(*p);
+}
+
+extern "C" int sage_paged_attn(const sage_paged_params* p, void* workspace, int64_t workspace_bytes, void* stream) {
+    bool nothing;
+    if (int rc = check_paged("sage_paged_attn", p, nothing)) return rc;
+    if (int rc = check_workspace("sage_paged_attn", workspace, workspace_bytes)) return rc;
+    return nothing ? SAGE_OK : launch_paged_attn(*p, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int sage_cache_append(const sage_append_params* p, void* stream) {
+    const char* who = "sage_cache_append";
+    if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
+    if (!float_dtype_ok(p->dtype)) return fail(SAGE_E_INVALID, "%s: bad dtype %d", who, p->dtype);
+    if (p->tokens < 0 || p->heads_kv < 0 || p->head_dim < 0 || p->pages < 0) return fail(SAGE_E_INVALID, "%s: negative size", who);
+    if (p->page_size <= 0) return fail(SAGE_E_INVALID, "%s: page_size must be positive", who);
+    const int e = dtype_bytes(p->dtype);
+    const int64_t lim = 1LL << 30;
+    if (p->tokens >= lim || p->pages >= lim || p->page_size >= lim || p->heads_kv > (1 << 16) || p->head_dim > (1 << 12))
+        return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30, heads_kv at most 65536, head_dim at most 4096", who);
+    if (p->tokens == 0 || p->heads_kv == 0 || p->head_dim == 0 || p->pages == 0) return SAGE_OK;
+    if (!p->k.ptr || !p->v.ptr || !p->k_cache.ptr || !p->v_cache.ptr || !p->slots) return fail(SAGE_E_INVALID, "%s: null pointer", who);
+    if (p->head_dim * e % 16 != 0 || misaligned_row(p->k, e) || misaligned_row(p->v, e) || misaligned_row(p->k_cache, e) || misaligned_row(p->v_cache, e))
+        return fail(SAGE_E_INVALID, "%s: rows of k, v and the caches must be 16-byte aligned and a multiple of 16 bytes long", who);
+    return launch_cache_append(*p, (hipStream_t)stream);
+}
+
+extern "C" int sage_cache_copy_pages(const sage_copy_params* p, void* stream) {
+    const char* who = "sage_cache_copy_pages";
+    if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
+    if (p->count < 0 || p->layers < 0 || p->pages < 0 || p->page_bytes < 0) return fail(SAGE_E_INVALID, "%s: negative size", who);
+    if (p->count >= (1LL << 30) || p->pages >= (1LL << 30) || p->page_bytes >= (1LL << 30) || p->layers > 32767)
+        return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30, layers at most 32767", who);
+    if (p->count == 0 || p->layers == 0 || p->pages == 0 || p->page_bytes == 0) return SAGE_OK;
+    if (!p->k_cache || !p->v_cache || !p->src || !p->dst) return fail(SAGE_E_INVALID, "%s: null pointer", who);
+    if (p->page_bytes % 16 != 0 || ((uintptr_t)p->k_cache | (uintptr_t)p->v_cache | p->k_stride_layer | p->k_stride_page | p->v_stride_layer | p->v_stride_page) % 16 != 0)
+        return fail(SAGE_E_INVALID, "%s: pages must be 16-byte aligned and a multiple of 16 bytes long", who);
+    return launch_cache_copy(*p, (hipStream_t)stream);
+}

@@ -267,6 +267,101 @@ int64_t sage_flash_total_attention_workspace_bytes(const sage_flash_params* p);
 int sage_flash_total_attention_ws(const sage_flash_params* p, const float* log_normalizer, float* total_attention,
                                   void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * The dense forward over packed sequences of different lengths (no padding): sequence s has the queries
+ * cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 of q and the keys cu_seqlens_k[s] .. cu_seqlens_k[s + 1] - 1 of k and v,
+ * and attends to itself only.  Causal: key j of a sequence is visible to its query i iff j <= i + (Lk - Lq).
+ *
+ *   q, out       [total_q, Hq, D], k, v [total_k, Hkv, D] through stride_n (token) and stride_h; stride_b is not used
+ *   cu_seqlens_* seqs + 1 offsets on the device, not decreasing, from 0 to at most total_q / total_k.  They are read by the
+ *                kernel: a captured graph follows their present values.  Offsets out of order or out of range are clamped
+ *                (no access outside the tensors).  Rows of out and log_normalizer that belong to no sequence are not written.
+ *   log_normalizer  optional [Hq, total_q] fp32 contiguous, natural log; NULL = none
+ *   dtype        SAGE_F16 / SAGE_BF16 of q, k, v and out
+ * A query that sees no key yields a zero row and a log normalizer of -inf; so does one whose scores are all -inf.  An infinity or
+ * NaN in a key or value that a query does not see has no effect on it.  head_dim 64 or 128.
+ */
+typedef struct sage_varlen_params {
+    sage_tensor q, k, v, out;
+    float* log_normalizer;
+    const int32_t* cu_seqlens_q;
+    const int32_t* cu_seqlens_k;
+    int64_t seqs, total_q, total_k, heads_q, heads_kv, head_dim;
+    int32_t dtype, causal;
+    float sm_scale;
+} sage_varlen_params;
+
+int sage_flash_varlen_fwd(const sage_varlen_params* p, void* stream);
+
+/*
+ * Dense attention of the newest tokens of every sequence over a cache of keys and values in pages: token t of sequence s,
+ * t < seq_lens[s], lies in page block_table[s * table_stride + t / page_size] at place t % page_size; the last new_tokens of them
+ * are the queries' own, whose keys and values are in the cache already.  Query m sees the tokens up to
+ * seq_lens[s] - new_tokens + m.
+ *
+ *   q, out       [seqs, new_tokens, Hq, D] through stride_b (sequence), stride_n (new token) and stride_h
+ *   k_cache, v_cache  [pages, ..] through stride_b (page), stride_h and stride_n (place in a page)
+ *   block_table  [seqs, table_width] int32 on the device, rows table_stride entries apart; entries past a sequence's last page are not
+ *                read.  The tokens of an entry that is no page of the cache (negative, or pages and more) take no part.
+ *   seq_lens     [seqs] int32 on the device, clamped to 0 .. table_width * page_size
+ *   log_normalizer  optional [seqs, Hq, new_tokens] fp32 contiguous, natural log; NULL = none
+ * The table and the lengths are read by the kernels: a captured graph follows their present values.  Zero rows, infinities and
+ * NaN as for sage_flash_varlen_fwd.  head_dim 64 or 128; any page_size.
+ *
+ * workspace: rules of sage_attn_fwd_ws.  With one, the keys of all sequences are shared out evenly over the compute units,
+ * whatever the lengths are, and a second kernel joins the parts; without one (or where table_width * page_size is
+ * small) a workgroup takes each sequence and K/V head.
+ */
+typedef struct sage_paged_params {
+    sage_tensor q, out, k_cache, v_cache;
+    float* log_normalizer;
+    const int32_t* block_table;
+    const int32_t* seq_lens;
+    int64_t table_stride, seqs, new_tokens, heads_q, heads_kv, head_dim, pages, page_size, table_width;
+    int32_t dtype;
+    float sm_scale;
+} sage_paged_params;
+
+int64_t sage_paged_attn_workspace_bytes(const sage_paged_params* p);
+int sage_paged_attn(const sage_paged_params* p, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Writes rows of new tokens into the pages of a cache: row t of k and v goes to slot slots[t] = page * page_size + place.
+ * Slots that the cache does not have (negative, or pages * page_size and more) are not written: padding.  Slots that
+ * occur twice get one row or the other, or pieces of both.
+ *
+ *   k, v         [tokens, Hkv, D] through stride_n (token) and stride_h;  k_cache, v_cache as for sage_paged_attn
+ *   slots        [tokens] on the device, int32 or (slots_int64) int64
+ *   dtype        of all four (SAGE_F16 / SAGE_BF16 / SAGE_F32); rows of a multiple of 16 bytes
+ */
+typedef struct sage_append_params {
+    sage_tensor k, v, k_cache, v_cache;
+    const void* slots;
+    int64_t tokens, heads_kv, head_dim, pages, page_size;
+    int32_t dtype, slots_int64;
+} sage_append_params;
+
+int sage_cache_append(const sage_append_params* p, void* stream);
+
+/*
+ * Copies pages within a cache of one or more layers: page src[i] to page dst[i], K and V, in every layer.  A page is page_bytes
+ * contiguous bytes (a multiple of 16), pages *_stride_page and layers *_stride_layer bytes apart.  Pairs with a page that the
+ * cache does not have (negative, or pages and more) copy nothing.  No page may be written that another pair reads or writes.
+ *
+ *   src, dst     [count] on the device, each int32 or (src_int64 / dst_int64) int64
+ */
+typedef struct sage_copy_params {
+    void* k_cache;
+    void* v_cache;
+    int64_t k_stride_layer, k_stride_page, v_stride_layer, v_stride_page;
+    const void* src;
+    const void* dst;
+    int64_t count, layers, pages, page_bytes;
+    int32_t src_int64, dst_int64;
+} sage_copy_params;
+
+int sage_cache_copy_pages(const sage_copy_params* p, void* stream);
+
 /* Message describing the last non-zero status returned on this thread ("" if none). */
 const char* sage_hip_last_error(void);
 
