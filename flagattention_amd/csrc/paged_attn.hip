@@ -65,9 +65,7 @@ __device__ __forceinline__ int seq_chunks(const PagedArgs& a, int s) { return ma
 __device__ __forceinline__ int line_total(const PagedArgs& a) {
     int sum = 0;
     for (int s = threadIdx.x & 63; s < a.seqs; s += 64) sum += seq_chunks(a, s);
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-    return __builtin_amdgcn_readfirstlane(sum) * a.Hkv * a.row_tiles;
+    return wave_sum(sum) * a.Hkv * a.row_tiles;
 }
 
 template <int D> __device__ __forceinline__ int paged_v_swizzle(int row) { return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
@@ -245,12 +243,12 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
             }
             // P is rounded to 16 bits for the matrix instructions (at most 1, so half a step of 1 off); its sum is taken before that
             vec16 pf[2];
-            float p[16], psum = 0.0f;
+            float psum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                p[i] = __builtin_amdgcn_exp2f(x[i] - m_use);
-                psum += p[i];
-                pf[i >> 3][i & 7] = (VT)p[i];
+                const float p = __builtin_amdgcn_exp2f(x[i] - m_use);
+                psum += p;
+                pf[i >> 3][i & 7] = (VT)p;
             }
             l_i += psum;
             // ---- O^T += V^T.P^T
@@ -284,7 +282,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++)
                         o[dt] = PVT::mfma(__builtin_bit_cast(vec16, finite_only<VT>(v_fragment(c, dt))), pf[c], o[dt]);
-                add_nonfinite<D, VT>(vlds, [](int row) { return paged_v_swizzle<D>(row); }, p, my_last - key0 + 1, o);
+                add_nonfinite<D, VT>(vlds, [](int row) { return paged_v_swizzle<D>(row); }, pf[0], pf[1], my_last - key0 + 1, o);
             }
             seen = seen_next;
         }

@@ -12,15 +12,24 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
 
-// Inclusive sum over the lanes of a wave.
-__device__ __forceinline__ int wave_scan(int x) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int y = __shfl_up(x, d);
-        if ((int)(threadIdx.x & 63) >= d) x += y;
-    }
+// Inclusive scan over the lanes of a wave (0: what joins nothing), by lane moves inside the vector unit.
+template <typename Join>
+__device__ __forceinline__ int wave_scan(int x, Join&& join) {
+    auto step = [&](auto ctrl, auto rows) {
+        x = join(x, __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    };
+    step(IC<0x111>{}, IC<0xf>{});  // from 1, 2, 4, 8 lanes below, within rows of 16
+    step(IC<0x112>{}, IC<0xf>{});
+    step(IC<0x114>{}, IC<0xf>{});
+    step(IC<0x118>{}, IC<0xf>{});
+    step(IC<0x142>{}, IC<0xa>{});  // the last lane of a row into the next one: rows 1 and 3
+    step(IC<0x143>{}, IC<0xc>{});  // lane 31 into rows 2 and 3
     return x;
 }
+__device__ __forceinline__ int wave_scan(int x) { return wave_scan(x, [](int a, int b) { return a + b; }); }
+// Over all lanes, the same in each of them: the sum, the largest of numbers that are not negative.
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+__device__ __forceinline__ int wave_max(int x) { return __builtin_amdgcn_readlane(wave_scan(x, [](int a, int b) { return max(a, b); }), 63); }
 
 // Which of n consecutive runs, run i count(i) >= 0 entries long, holds entry `at`, and where that run begins; false: all of
 // them end before `at`.  Every wave finds it for itself: lane after lane takes an equal stretch of the runs, a scan says
@@ -75,18 +84,24 @@ __device__ __forceinline__ v4i finite_only(v4i x) {
     return x;
 }
 
-// What the infinities and NaN of a V tile in LDS add to the outputs of a lane's row: for every key j < last_seen_end of the tile and
-// every channel that the lane holds.  p: the lane's P of the tile's keys 8 (i / 4) + 4 half + i % 4 (0 for keys the row does
-// not see, which add nothing).  V row j, chunk c lies at row j * 2 D + 16 (c ^ swizzle(j)).  Slow, and hardly ever called.
+// What the infinities and NaN of a V tile in LDS add to the outputs of a lane's row: for every key j < see_end of the tile and
+// every channel that the lane holds.  p0, p1: the lane's P of the tile's keys 8 (i / 4) + 4 half + i % 4, i < 8 and the others.
+// V row j, chunk c lies at row j * 2 D + 16 (c ^ swizzle(j)).  Slow, and hardly ever called.
 template <int D, typename VT, typename Swizzle>
-__device__ __forceinline__ void add_nonfinite(const unsigned char* vtile, Swizzle&& swizzle, const float (&p)[16], int see_end, v16f (&acc)[D / 32]) {
+__device__ __forceinline__ void add_nonfinite(const unsigned char* vtile, Swizzle&& swizzle, typename PV<VT>::vec p0, typename PV<VT>::vec p1,
+                                              int see_end, v16f (&acc)[D / 32]) {
     const int half = (threadIdx.x >> 5) & 1;
+    const v4i w0 = __builtin_bit_cast(v4i, p0), w1 = __builtin_bit_cast(v4i, p1);
 #pragma unroll 1
     for (int j = 0; j < 32; j++) {
-        const int owner = (j >> 2) & 1, reg = 4 * (j >> 3) + (j & 3);  // P of key j: register reg of the lane of that half
-        float mine = 0.0f;
+        const int owner = (j >> 2) & 1, reg = 4 * (j >> 3) + (j & 3);  // P of key j: number reg of the lane of that half
+        unsigned pair = 0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) mine = i == reg ? p[i] : mine;
+        for (int i = 0; i < 8; i++) {
+            const int w = i < 4 ? w0[i & 3] : w1[i & 3];
+            pair = i == reg >> 1 ? (unsigned)w : pair;
+        }
+        const float mine = (float)__builtin_bit_cast(VT, (unsigned short)(reg & 1 ? pair >> 16 : pair));
         const float other = __shfl_xor(mine, 32);
         const float pj = owner == half ? mine : other;
         const bool sees = j < see_end;
