@@ -123,6 +123,7 @@ EXPORTS = (
     "sage_k_mean",
     "sage_k_mean_workspace_bytes",
     "sage_k_mean_noalloc",
+    "sage_flash_varlen_workspace_bytes",
     "sage_flash_varlen_fwd",
     "sage_paged_attn_workspace_bytes",
     "sage_paged_attn",
@@ -193,7 +194,9 @@ def load():
     lib.sage_k_mean_noalloc.argtypes = [ctypes.POINTER(SageTensor), c_i32, ctypes.c_void_p, c_i32, c_i64, c_i64, c_i64,
                                         c_i64, ctypes.c_void_p]
     lib.sage_k_mean_noalloc.restype = ctypes.c_int
-    lib.sage_flash_varlen_fwd.argtypes = [ctypes.POINTER(VarlenParams), ctypes.c_void_p]
+    lib.sage_flash_varlen_workspace_bytes.argtypes = [ctypes.POINTER(VarlenParams)]
+    lib.sage_flash_varlen_workspace_bytes.restype = c_i64
+    lib.sage_flash_varlen_fwd.argtypes = [ctypes.POINTER(VarlenParams), ctypes.c_void_p, c_i64, ctypes.c_void_p]
     lib.sage_flash_varlen_fwd.restype = ctypes.c_int
     lib.sage_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedParams)]
     lib.sage_paged_attn_workspace_bytes.restype = c_i64

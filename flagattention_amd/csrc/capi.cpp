@@ -296,12 +296,14 @@ static int check_heads(const char* who, int64_t heads_q, int64_t heads_kv, int64
     return SAGE_OK;
 }
 
-extern "C" int sage_flash_varlen_fwd(const sage_varlen_params* p, void* stream) {
-    const char* who = "sage_flash_varlen_fwd";
+// nothing: the call is valid and has no row to compute
+static int check_varlen(const char* who, const sage_varlen_params* p, bool& nothing) {
+    nothing = false;
     if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
     if (int rc = check_heads(who, p->heads_q, p->heads_kv, p->head_dim, p->dtype, p->sm_scale)) return rc;
     if (p->seqs < 0 || p->total_q < 0 || p->total_k < 0) return fail(SAGE_E_INVALID, "%s: negative size", who);
-    if (p->seqs == 0 || p->total_q == 0) return SAGE_OK;  // (no row to write)
+    nothing = p->seqs == 0 || p->total_q == 0;
+    if (nothing) return SAGE_OK;
     if (!p->q.ptr || !p->out.ptr || !p->cu_seqlens_q || !p->cu_seqlens_k || (p->total_k > 0 && (!p->k.ptr || !p->v.ptr)))
         return fail(SAGE_E_INVALID, "%s: null pointer", who);
     const int64_t lim = 1LL << 30;
@@ -311,10 +313,22 @@ extern "C" int sage_flash_varlen_fwd(const sage_varlen_params* p, void* stream) 
         return fail(SAGE_E_INVALID, "%s: rows of q, k, v and out must be 16-byte aligned", who);
     if (p->k.stride_n < 0 || p->v.stride_n < 0 || p->k.stride_n >= (1LL << 24) || p->v.stride_n >= (1LL << 24))
         return fail(SAGE_E_UNSUPPORTED, "%s: token stride of k or v out of range for 32-bit tile offsets", who);
-    return launch_flash_varlen(*p, (hipStream_t)stream);
+    return SAGE_OK;
 }
 
-// nothing: the call is valid and has no row to compute
+extern "C" int64_t sage_flash_varlen_workspace_bytes(const sage_varlen_params* p) {
+    bool nothing;
+    if (check_varlen("sage_flash_varlen_workspace_bytes", p, nothing)) return -1;
+    return nothing ? 0 : varlen_workspace_bytes(*p);
+}
+
+extern "C" int sage_flash_varlen_fwd(const sage_varlen_params* p, void* workspace, int64_t workspace_bytes, void* stream) {
+    bool nothing;
+    if (int rc = check_varlen("sage_flash_varlen_fwd", p, nothing)) return rc;
+    if (int rc = check_workspace("sage_flash_varlen_fwd", workspace, workspace_bytes)) return rc;
+    return nothing ? SAGE_OK : launch_flash_varlen(*p, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
 static int check_paged(const char* who, const sage_paged_params* p, bool& nothing) {
     nothing = false;
     if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);

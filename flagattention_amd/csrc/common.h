@@ -37,7 +37,8 @@ int launch_flash_total_attention(const sage_flash_params& p, const float* log_no
                                  int64_t workspace_bytes, hipStream_t stream);
 int64_t total_workspace_bytes(const sage_flash_params& p);
 int launch_flash_dropout(const sage_flash_params& p, float dropout_p, uint64_t seed, uint64_t offset, hipStream_t stream);
-int launch_flash_varlen(const sage_varlen_params& p, hipStream_t stream);
+int64_t varlen_workspace_bytes(const sage_varlen_params& p);
+int launch_flash_varlen(const sage_varlen_params& p, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 int64_t paged_workspace_bytes(const sage_paged_params& p);
 int launch_paged_attn(const sage_paged_params& p, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 int launch_cache_append(const sage_append_params& p, hipStream_t stream);

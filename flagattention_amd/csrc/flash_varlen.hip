@@ -21,7 +21,10 @@
 // Measured (bf16, D128, causal): those documents 593 us = 1100 TFLOP/s, one sequence of 16384 tokens with H16/2 952 us = 1155 TFLOP/s (a
 // library product of 8192^3 reaches 1356 here); 48 prompts of 1 to 700 tokens 48 us.  Tiles of 32 keys, each multiplied, weighed and
 // added in turn: 811, 1272 and 54 us.  Eight waves per workgroup: 2 % more for long sequences, 28 % less for short ones.
+#include <math.h>
+
 #include "serve_common.h"
+#include "step_lines.h"
 
 namespace sage {
 namespace {
@@ -39,12 +42,15 @@ struct VarlenArgs {
     int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h, os_t, os_h;
     int32_t seqs, total_q, total_k, Hkv, groups, causal;
     float qk_scale;  // sm_scale * log2(e)
+    // Cut launch: workgroups that share all steps evenly, tokens of a block (a power of two; log2), partial results.
+    int32_t shares, tokens_shift;
+    float* part_o;    // [2 * shares][4 waves][D / 32][4][64 lanes][4]: normalized outputs in the order of the accumulator registers
+    float* part_lse;  // [2 * shares][128], base 2
 };
 
 constexpr int kVarWaves = 4;
 constexpr int kVarThreads = 64 * kVarWaves;
 constexpr int kVarRows = 32 * kVarWaves;
-constexpr int kVarKeys = 64;  // keys per tile
 constexpr float kLag = 8.0f;
 
 // Sequence s of a packed axis.  (Offsets out of order or past the end give no rows that do not exist.)
@@ -104,11 +110,53 @@ __device__ __forceinline__ bool find_block(const VarlenArgs& a, int at, int& q0,
 
 template <int D> __device__ __forceinline__ int var_v_swizzle(int row) { return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
 
+__device__ __forceinline__ int sequence_steps(const VarlenArgs& a, int s) {
+    int begin, m, n;
+    sequence(a.cu_q, s, a.total_q, begin, m);
+    sequence(a.cu_k, s, a.total_k, begin, n);
+    return Steps(m, n, a.tokens_shift, a.causal).total() * a.Hkv;
+}
+
+__device__ __forceinline__ int all_steps(const VarlenArgs& a) {
+    int sum = 0;
+    for (int s = threadIdx.x & 63; s < a.seqs; s += 64) sum += sequence_steps(a, s);
+    return wave_sum(sum);
+}
+
+// The block that holds step `pos` of the line.
+struct BlockAt {
+    int q0, M, k0, N;  // its sequence
+    int hk, block;
+    int begin, tiles;  // its first step on the line; its tiles are the steps from begin + kStart on
+    bool found;
+    __device__ BlockAt(const VarlenArgs& a, int pos) {
+        int seq, first;
+        found = find_run(a.seqs, pos, [&](int s) { return sequence_steps(a, s); }, seq, first);
+        if (!found) return;
+        sequence(a.cu_q, seq, a.total_q, q0, M);
+        sequence(a.cu_k, seq, a.total_k, k0, N);
+        const Steps line(M, N, a.tokens_shift, a.causal);
+        const int per_head = line.total();
+        hk = (pos - first) / per_head;
+        first += hk * per_head;
+        int low = 0, high = line.nb;
+        while (high - low > 1) {
+            const int mid = (low + high) / 2;
+            if (first + line.before(mid) <= pos) low = mid;
+            else high = mid;
+        }
+        block = low;
+        begin = first + line.before(low);
+        tiles = line.tiles(low);
+    }
+};
+
 // One row by one wave, from its keys alone: query token qt, head h, the first n keys from k0 on.  A lane is a key for the scores,
-// and D / 64 channels for the output.  For rows whose tiles hold infinities or NaN in V: a thousand times slower than a tile's share
+// and D / 64 channels for the output.  part_o: where the wave's partial results begin and the row's log-sum-exp goes, for row r of
+// the wave, or null.  For rows whose tiles hold infinities or NaN in V: a thousand times slower than a tile's share
 // of the kernel below, and hardly ever called.
 template <int D, typename VT>
-__device__ void careful_row(const VarlenArgs& a, int qt, int h, int hk, int k0, int n) {
+__device__ void careful_row(const VarlenArgs& a, int qt, int h, int hk, int k0, int n, float* part_o, float* part_lse, int r) {
     constexpr int CH = D / 64;
     typedef VT vt8 __attribute__((ext_vector_type(8)));
     const int lane = threadIdx.x & 63;
@@ -146,13 +194,24 @@ __device__ void careful_row(const VarlenArgs& a, int qt, int h, int hk, int k0, 
         }
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    if (part_o) {
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const int c = lane + 64 * i;
+            part_o[(c / 8) * 256 + (32 * (c / 4 % 2) + r) * 4 + c % 4] = o[i] * inv;
+        }
+        if (lane == 0) part_lse[r] = __builtin_log2f(l) + (m == -INFINITY ? 0.0f : m);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < CH; i++) static_cast<VT*>(a.out)[(int64_t)qt * a.os_t + (int64_t)h * a.os_h + lane + 64 * i] = (VT)(o[i] * inv);
     if (a.lse && lane == 0) a.lse[(int64_t)h * a.total_q + qt] = (__builtin_log2f(l) + (m == -INFINITY ? 0.0f : m)) * 0.693147180559945309f;
 }
 
-template <int D, typename VT>
-__global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs a) {
+// CUT: a workgroup takes an equal share of the launch's steps instead of a block: the end of one, whole ones, the beginning of another.
+template <int D, typename VT, bool CUT>
+__global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs args) {
+    const VarlenArgs& a0 = args;
     using PVT = PV<VT>;
     using vec16 = typename PVT::vec;
     constexpr int KS = D / 16;      // matrix instructions of one 32 x 32 score tile
@@ -167,10 +226,48 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
 
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x % a.Hkv;
-    int q0, M, k0, N, block;
-    if (!find_block(a, blockIdx.x / a.Hkv, q0, M, k0, N, block)) return;
-    const int rows = M * a.groups, row0 = block * kVarRows;
+    int pos = 0, pos_end = 1, share = 0;  // (CUT) this workgroup's steps
+    if constexpr (CUT) {
+        // (neighbours on the line, which read the same keys, on one XCD: workgroups go to the eight of them in turn)
+        share = blockIdx.x % 8 * (a0.shares / 8) + blockIdx.x / 8;
+        const EqualShares line(all_steps(a0), a0.shares);
+        pos = line.begin(share);
+        pos_end = line.begin(share + 1);
+    }
+    const int pos_begin = pos;
+  while (pos < pos_end) {
+    // (CUT: the arguments are read again for each piece, behind an opaque pointer: kept across the pieces they cost scalar registers
+    // that the step loop then reloads)
+    typedef __attribute__((address_space(4))) const void* const_ptr;
+    const_ptr again_args = (const_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    if constexpr (CUT) asm volatile("" : "+s"(again_args));
+    const VarlenArgs& a = CUT ? *(const VarlenArgs*)again_args : args;
+    int hk = blockIdx.x % a.Hkv, q0, M, k0, N, block;
+    int block_rows = kVarRows, first_tile = 0, cut_tiles = 0;
+    bool whole = true;
+    const int slot = 2 * share + (pos != pos_begin);  // (CUT) of the piece's results, if it is not the whole block
+    if constexpr (CUT) {
+        const BlockAt at(a, pos);
+        if (!at.found) return;
+        q0 = at.q0; M = at.M; k0 = at.k0; N = at.N; hk = at.hk; block = at.block;
+        block_rows = a.groups << a.tokens_shift;
+        first_tile = max(pos - at.begin - kStart, 0);
+        const bool later = pos != pos_begin;
+        pos = min(at.begin + kStart + at.tiles, pos_end);
+        cut_tiles = pos - at.begin - kStart - first_tile;
+        if (cut_tiles <= 0) break;  // (no tile of this block: it is the next share's)
+        whole = cut_tiles == at.tiles;
+        if (later) __syncthreads();  // (the piece before has been read)
+    } else {
+        pos = pos_end;
+        if (!find_block(a, blockIdx.x / a.Hkv, q0, M, k0, N, block)) return;
+    }
+    // rows of this block; the problem of a piece begins at its first key
+    const int row0 = block * block_rows, rows = CUT ? min(row0 + block_rows, M * a.groups) : M * a.groups;
+    if constexpr (CUT) {
+        k0 += first_tile * kVarKeys;
+        N -= first_tile * kVarKeys;
+    }
     const int shift = N - M;
     const int row = row0 + 32 * wave + l32;
     const bool row_ok = row < rows;
@@ -189,14 +286,16 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     // keys that any row of the workgroup / of this wave can see, and those that every row of the wave sees
     int n_end = N, wave_end = N, all_see = N;
     if (a.causal) {
-        n_end = max(min(N, (min(row0 + kVarRows, rows) - 1) / a.groups + 1 + shift), 0);
+        n_end = max(min(N, (min(row0 + block_rows, rows) - 1) / a.groups + 1 + shift), 0);
         wave_end = max(min(N, (min(row0 + 32 * wave + 32, rows) - 1) / a.groups + 1 + shift), 0);
         all_see = max(min(N, min(row0 + 32 * wave, rows - 1) / a.groups + 1 + shift), 0);
     }
     const int my_lim = a.causal ? min(my_m + shift, N - 1) : N - 1;  // last key this lane's row sees
-    const int ntiles = (n_end + kVarKeys - 1) / kVarKeys;
-    const int my_tiles = row0 + 32 * wave < rows ? (wave_end + kVarKeys - 1) / kVarKeys : 0;  // that this wave multiplies with
-    const int clear_tiles = all_see / kVarKeys;                                               // the first ones hide no key
+    int ntiles = (n_end + kVarKeys - 1) / kVarKeys;
+    if (CUT) ntiles = min(ntiles, cut_tiles);
+    // tiles that this wave multiplies with, and how many of them, the first ones, hide no key
+    const int my_tiles = row0 + 32 * wave < rows ? min((wave_end + kVarKeys - 1) / kVarKeys, ntiles) : 0;
+    const int clear_tiles = min(all_see / kVarKeys, my_tiles);
 
     // Tile t of K and V -> one of the two buffers, straight into LDS (written in assembly, as in attn_fast_kernel.h: the compiler
     // would wait for every outstanding load before each LDS read; m0 holds the LDS address and nothing else here uses it).
@@ -403,40 +502,160 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // nothing of this workgroup is on its way into LDS when it ends
 
+    // accumulator i of tile dt: channel 32 dt + 8 (i / 4) + 4 half + i % 4
+    float* part_o = whole ? nullptr : a.part_o + ((int64_t)slot * kVarWaves + wave) * (32 * D);
+    float* part_lse = whole ? nullptr : a.part_lse + (int64_t)slot * kVarRows + 32 * wave;
     if (__builtin_expect(again, 0)) {
-        for (int r = row0 + 32 * wave; r < min(row0 + 32 * wave + 32, rows); r++) {
-            const int m = r / a.groups;
-            careful_row<D, VT>(a, q0 + m, hk * a.groups + r % a.groups, hk, k0, a.causal ? min(m + shift, N - 1) + 1 : N);
+        for (int r = 0; r < 32 && row0 + 32 * wave + r < rows; r++) {
+            const int m = (row0 + 32 * wave + r) / a.groups, n = a.causal ? min(m + shift, N - 1) + 1 : N;
+            careful_row<D, VT>(a, q0 + m, hk * a.groups + (row0 + 32 * wave + r) % a.groups, hk, k0, CUT ? min(n, kVarKeys * ntiles) : n, part_o, part_lse, r);
         }
-        return;
+        continue;
     }
     const float l_tot = l_i + __shfl_xor(l_i, 32);
     // l = 0: a row that saw no key: zero row.  (NaN stays.)
     const float inv = l_tot != 0.0f ? 1.0f / l_tot : 0.0f;
-    if (!row_ok) return;
-    // accumulator i of tile dt: channel 32 dt + 8 (i / 4) + 4 half + i % 4
-    VT* op = static_cast<VT*>(a.out) + (int64_t)(q0 + my_m) * a.os_t + (int64_t)my_h * a.os_h + 4 * half;
+    const float lse2 = __builtin_log2f(l_tot) + (m_i == -INFINITY ? 0.0f : m_i);
+    if (CUT && !whole) {
+        if (row_ok) {
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++)
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    *reinterpret_cast<v4f*>(part_o + ((4 * dt + g) * 64 + lane) * 4) =
+                        v4f{acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv, acc[dt][4 * g + 3] * inv};
+            if (half == 0) part_lse[l32] = lse2;
+        }
+    } else if (row_ok) {
+        VT* op = static_cast<VT*>(a.out) + (int64_t)(q0 + my_m) * a.os_t + (int64_t)my_h * a.os_h + 4 * half;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                store_rounded(op + 32 * dt + 8 * g, v4f{acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv, acc[dt][4 * g + 3] * inv});
+        if (a.lse && half == 0) a.lse[(int64_t)my_h * a.total_q + q0 + my_m] = lse2 * 0.693147180559945309f;
+    }
+  }
+}
+
+// The blocks of a cut launch that lie in more than one share: lse = log2 sum_s 2^lse_s, out = sum_s 2^(lse_s - lse) o_s.  A workgroup per
+// cut between two shares and wave of a block; the first cut inside a block takes care of it.  A wave adds 32 channels of 32 rows
+// in the order of the registers that left them.
+template <int D, typename VT>
+__global__ __launch_bounds__(2 * D) void varlen_combine_kernel(VarlenArgs a) {
+    const EqualShares line(all_steps(a), a.shares);
+    const int cut = blockIdx.x + 1, pos = line.begin(cut), wave = blockIdx.y;
+    if (line.begin(cut + 1) <= pos) return;  // (the shares from here on are empty)
+    const BlockAt at(a, pos);
+    if (!at.found) return;
+    const int first = line.owner(at.begin + kStart);
+    if (pos <= at.begin + kStart || first + 1 != cut) return;
+    const int last = line.owner(at.begin + kStart + at.tiles - 1);
+    const int block_rows = a.groups << a.tokens_shift;
+    const int row0 = at.block * block_rows + 32 * wave, rows = min((at.block + 1) * block_rows, at.M * a.groups);
+    if (row0 >= rows) return;
+    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5, dt = threadIdx.x >> 6;
+    auto slot = [&](int w) { return (int64_t)(2 * w + (w == first && at.begin > line.begin(w))); };
+    v4f acc[4];
+#pragma unroll
+    for (int g = 0; g < 4; g++) acc[g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, den = 0.0f;
+    constexpr int kBatch = 4;  // parts on their way together
+    for (int w0 = first; w0 <= last; w0 += kBatch) {
+        float x[kBatch];
+        v4f o[kBatch][4];
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {  // (past the end: the last part once more)
+            const int64_t s = slot(min(w0 + u, last));
+            x[u] = a.part_lse[s * kVarRows + 32 * wave + l32];
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                o[u][g] = *reinterpret_cast<const v4f*>(a.part_o + ((s * kVarWaves + wave) * (D / 8) + 4 * dt + g) * 256 + lane * 4);
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) top = x[u] > top || x[u] != x[u] ? x[u] : top;  // (NaN stays)
+        const float use = top == -INFINITY ? 0.0f : top;  // (no key seen so far: weights of 0)
+        const float alpha = __builtin_amdgcn_exp2f(m - use);
+        den *= alpha;
 #pragma unroll
         for (int g = 0; g < 4; g++)
-            store_rounded(op + 32 * dt + 8 * g, v4f{acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv, acc[dt][4 * g + 3] * inv});
-    if (a.lse && half == 0) {
-        a.lse[(int64_t)my_h * a.total_q + q0 + my_m] = (__builtin_log2f(l_tot) + (m_i == -INFINITY ? 0.0f : m_i)) * 0.693147180559945309f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[g][i] *= alpha;
+        m = top;
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {
+            if (w0 + u > last) break;
+            const float w = __builtin_amdgcn_exp2f(x[u] - use);
+            den += w;
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[g][i] = __builtin_fmaf(w, o[u][g][i], acc[g][i]);
+        }
     }
+    const int row = row0 + l32;
+    if (row >= rows) return;
+    const float inv = den != 0.0f ? 1.0f / den : 0.0f;
+    const int my_m = row / a.groups, my_h = at.hk * a.groups + row % a.groups;
+    VT* op = static_cast<VT*>(a.out) + (int64_t)(at.q0 + my_m) * a.os_t + (int64_t)my_h * a.os_h + 32 * dt + 4 * half;
+#pragma unroll
+    for (int g = 0; g < 4; g++) store_rounded(op + 8 * g, v4f{acc[g][0] * inv, acc[g][1] * inv, acc[g][2] * inv, acc[g][3] * inv});
+    if (a.lse && dt == 0 && half == 0)
+        a.lse[(int64_t)my_h * a.total_q + at.q0 + my_m] = (__builtin_log2f(den) + (m == -INFINITY ? 0.0f : m)) * 0.693147180559945309f;
+}
+
+constexpr int kVarShares = 512;  // two workgroups on each compute unit
+
+// Does a cut launch pay?  By its time against that of whole blocks, in steps of the kernel, for sequences of the mean lengths (the
+// real ones are the device's): whole blocks take the longest one, or an even share where there are more than fit the chip; a cut
+// launch takes an even share with the blocks' starts, one more start and about 15 steps for the partial results and the second
+// launch.  Measured, whole and cut: H32/8 D128, 512 queries against 16512 keys 286 and 156 us, 3 x 100 to 400 against up to 8000
+// 146 and 79, 8 x 64 to 256 against up to 4000 86 and 77; 2000 causal 49 and 63, 2048 against 32000 951 and 1021; H16 D64, 6 x 129
+// to 512 against up to 7000 85 and 58, 2 x 3000 causal 51 and 68.
+bool cut_pays(const sage_varlen_params& p) {
+    const double blocks = (double)p.total_q * (p.heads_q / p.heads_kv) / kVarRows + 0.5 * p.seqs, load = blocks * p.heads_kv / kVarShares;
+    const double longest = (double)p.total_k / p.seqs / kVarKeys;
+    const double mean = p.causal ? longest - 0.5 * fmin((double)p.total_q / p.seqs / kVarKeys, longest) : longest;
+    const double whole = kStart + (load > 1.0 ? load * mean : longest), cut = load * (kStart + mean) + kStart + 15.0;
+    return 1.1 * cut < whole;
+}
+
+struct VarlenPlan { int64_t blocks; int shares, tokens_shift; };
+
+// Whole blocks, or (with_workspace) a cut launch.  The lengths are the device's: what the host knows are the totals.
+VarlenPlan plan_varlen(const sage_varlen_params& p, bool with_workspace) {
+    const int64_t groups = p.heads_q / p.heads_kv;
+    VarlenPlan plan{p.total_q * groups / kVarRows + p.seqs, 0, 0};  // at most: a ragged last block for every sequence
+    if (!with_workspace || groups > kVarRows) return plan;
+    while (2 * groups << plan.tokens_shift <= kVarRows) plan.tokens_shift++;
+    const int64_t blocks = (p.total_q >> plan.tokens_shift) + p.seqs, tiles = p.total_k / kVarKeys + 1;
+    if (blocks * p.heads_kv > 0x7fffffffLL / (tiles + kStart)) return plan;
+    if (cut_pays(p)) plan.shares = kVarShares;
+    return plan;
 }
 
 template <int D, typename VT>
-int launch_d(const VarlenArgs& a, hipStream_t stream) {
-    const int64_t blocks = ((int64_t)a.total_q * a.groups) / kVarRows + a.seqs;  // at most: a ragged last block for every sequence
+int launch_d(const VarlenArgs& a, int64_t blocks, hipStream_t stream) {
+    if (a.shares) {
+        hipLaunchKernelGGL((flash_varlen_kernel<D, VT, true>), dim3((unsigned)a.shares), dim3(kVarThreads), 0, stream, a);
+        if (int rc = check_launch("flash_varlen_kernel")) return rc;
+        hipLaunchKernelGGL((varlen_combine_kernel<D, VT>), dim3((unsigned)a.shares - 1, kVarWaves), dim3(2 * D), 0, stream, a);
+        return check_launch("varlen_combine_kernel");
+    }
     if (blocks * a.Hkv > 0x7fffffffLL) return fail(SAGE_E_UNSUPPORTED, "sage_flash_varlen_fwd: too many workgroups for one launch");
-    hipLaunchKernelGGL((flash_varlen_kernel<D, VT>), dim3((unsigned)(blocks * a.Hkv)), dim3(kVarThreads), 0, stream, a);
+    hipLaunchKernelGGL((flash_varlen_kernel<D, VT, false>), dim3((unsigned)(blocks * a.Hkv)), dim3(kVarThreads), 0, stream, a);
     return check_launch("flash_varlen_kernel");
 }
 
 }  // namespace
 
-int launch_flash_varlen(const sage_varlen_params& p, hipStream_t stream) {
+int64_t varlen_workspace_bytes(const sage_varlen_params& p) {
+    return 2LL * plan_varlen(p, true).shares * kVarRows * (p.head_dim + 1) * (int64_t)sizeof(float);
+}
+
+int launch_flash_varlen(const sage_varlen_params& p, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+    const VarlenPlan plan = plan_varlen(p, workspace != nullptr && workspace_bytes >= varlen_workspace_bytes(p));
     VarlenArgs a{};
     a.q = p.q.ptr; a.k = p.k.ptr; a.v = p.v.ptr; a.out = p.out.ptr; a.lse = p.log_normalizer;
     a.cu_q = p.cu_seqlens_q; a.cu_k = p.cu_seqlens_k;
@@ -445,8 +664,11 @@ int launch_flash_varlen(const sage_varlen_params& p, hipStream_t stream) {
     a.seqs = (int)p.seqs; a.total_q = (int)p.total_q; a.total_k = (int)p.total_k;
     a.Hkv = (int)p.heads_kv; a.groups = (int)(p.heads_q / p.heads_kv); a.causal = p.causal ? 1 : 0;
     a.qk_scale = p.sm_scale * 1.44269504089f;
-    if (p.head_dim == 128) return p.dtype == SAGE_BF16 ? launch_d<128, __bf16>(a, stream) : launch_d<128, _Float16>(a, stream);
-    return p.dtype == SAGE_BF16 ? launch_d<64, __bf16>(a, stream) : launch_d<64, _Float16>(a, stream);
+    a.shares = plan.shares; a.tokens_shift = plan.tokens_shift;
+    a.part_o = (float*)workspace;
+    a.part_lse = a.part_o + 2LL * plan.shares * kVarRows * p.head_dim;
+    if (p.head_dim == 128) return p.dtype == SAGE_BF16 ? launch_d<128, __bf16>(a, plan.blocks, stream) : launch_d<128, _Float16>(a, plan.blocks, stream);
+    return p.dtype == SAGE_BF16 ? launch_d<64, __bf16>(a, plan.blocks, stream) : launch_d<64, _Float16>(a, plan.blocks, stream);
 }
 
 }  // namespace sage

@@ -47,17 +47,6 @@ struct PagedArgs {
     float* part_lse;               // [2 * shares][tile_rows], base 2
 };
 
-// The line of chunks, and its equal shares.
-struct Line {
-    int base, rest;  // share w has base chunks, one more for w < rest
-    __device__ Line(int total, int shares) : base(total / shares), rest(total % shares) {}
-    __device__ int begin(int w) const { return w * base + min(w, rest); }
-    __device__ int owner(int pos) const {
-        const int longer = rest * (base + 1);
-        return pos < longer ? pos / (base + 1) : rest + (pos - longer) / base;
-    }
-};
-
 __device__ __forceinline__ int seq_len(const PagedArgs& a, int s) { return min(max(a.lens[s], 0), a.capacity); }
 __device__ __forceinline__ int seq_chunks(const PagedArgs& a, int s) { return max((seq_len(a, s) + kChunk - 1) / kChunk, 1); }
 
@@ -98,7 +87,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
         pos = blockIdx.x % per_seq * c;
         end = pos + c;
     } else {
-        const Line line(line_total(a), a.shares);
+        const EqualShares line(line_total(a), a.shares);
         pos = line.begin(blockIdx.x);
         end = line.begin(blockIdx.x + 1);
         if (pos >= end) return;
@@ -344,7 +333,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedArgs 
     constexpr int kBatch = 8;  // loads on their way together
     __shared__ float sm_m[kPagedThreads], sm_den[kPagedThreads];
     __shared__ v4f sm_acc[kPagedThreads];
-    const Line line(line_total(a), a.shares);
+    const EqualShares line(line_total(a), a.shares);
     const int cut = blockIdx.x + 1, pos = line.begin(cut);
     const int per_seq = a.Hkv * a.row_tiles;
     int seq, seq_begin;

@@ -3,6 +3,7 @@
 #include <type_traits>
 
 #include "attn_common.h"
+#include "step_lines.h"
 
 namespace sage {
 namespace attn {

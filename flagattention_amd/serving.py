@@ -158,7 +158,13 @@ def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fals
         p.seqs, p.total_q, p.total_k = cu_seqlens_q.numel() - 1, T, Tk
         p.heads_q, p.heads_kv, p.head_dim = H, Hk, max(D, 64)
         p.dtype, p.causal, p.sm_scale = DTYPE_CODE[q.dtype], 1 if causal else 0, sm_scale
-        _lib.check(_lib.load().sage_flash_varlen_fwd(p, current_stream_ptr(q.device)), "sage_flash_varlen_fwd")
+        lib = _lib.load()
+        ws_bytes = lib.sage_flash_varlen_workspace_bytes(p)
+        if ws_bytes < 0:
+            _lib.check(-1, "sage_flash_varlen_workspace_bytes")
+        ws = split_workspace(q.device, ws_bytes) if ws_bytes else None
+        _lib.check(lib.sage_flash_varlen_fwd(p, ws.data_ptr() if ws is not None else None, ws_bytes, current_stream_ptr(q.device)),
+                   "sage_flash_varlen_fwd")
         if D < 64:
             o = o[..., :D].contiguous() if out is None else out.copy_(o[..., :D])
     return (o, L) if return_log_normalizer else o

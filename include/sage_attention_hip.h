@@ -280,6 +280,10 @@ int sage_flash_total_attention_ws(const sage_flash_params* p, const float* log_n
  *   dtype        SAGE_F16 / SAGE_BF16 of q, k, v and out
  * A query that sees no key yields a zero row and a log normalizer of -inf; so does one whose scores are all -inf.  An infinity or
  * NaN in a key or value that a query does not see has no effect on it.  head_dim 64 or 128.
+ *
+ * workspace: rules of sage_attn_fwd_ws.  With one, calls of few blocks of 128 rows (a row: a query and one of its heads) are cut into
+ * equal shares of all their 64-key steps, whose partial results a second kernel joins; their results agree with those of the uncut
+ * call to the rounding of P.
  */
 typedef struct sage_varlen_params {
     sage_tensor q, k, v, out;
@@ -291,7 +295,8 @@ typedef struct sage_varlen_params {
     float sm_scale;
 } sage_varlen_params;
 
-int sage_flash_varlen_fwd(const sage_varlen_params* p, void* stream);
+int64_t sage_flash_varlen_workspace_bytes(const sage_varlen_params* p);
+int sage_flash_varlen_fwd(const sage_varlen_params* p, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Dense attention of the newest tokens of every sequence over a cache of keys and values in pages: token t of sequence s,

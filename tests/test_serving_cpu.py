@@ -126,6 +126,15 @@ def test_struct_layouts_match_header(tmp_path):
             assert int(seen[f"{cname}.{n}"]) == getattr(cls, n).offset, (cname, n)
 
 
+def test_lines_of_steps(tmp_path):
+    if shutil.which("g++") is None:
+        pytest.skip("needs g++")
+    exe = str(tmp_path / "check")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-o", exe, os.path.join(ROOT, "tests", "csrc", "step_lines_check.cpp")], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=100)
+    assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout
+
+
 def _varlen_params():
     from flagattention_amd import _lib
 
@@ -160,8 +169,8 @@ def test_varlen_validation(field, value, status, message):
 
     lib, p = _lib.load(), _varlen_params()
     setattr(p, field, value)
-    assert lib.sage_flash_varlen_fwd(p, None) == status and message in lib.sage_hip_last_error()
-    assert lib.sage_flash_varlen_fwd(None, None) == -1
+    assert lib.sage_flash_varlen_fwd(p, None, 0, None) == status and message in lib.sage_hip_last_error()
+    assert lib.sage_flash_varlen_fwd(None, None, 0, None) == -1
 
 
 def test_varlen_validation_of_rows():
@@ -172,11 +181,11 @@ def test_varlen_validation_of_rows():
                                       ("v", "stride_n", 1 << 24, -2), ("v", "ptr", None, -1)):
         p = _varlen_params()
         setattr(getattr(p, name), part, value)
-        assert lib.sage_flash_varlen_fwd(p, None) == status, (name, part)
+        assert lib.sage_flash_varlen_fwd(p, None, 0, None) == status, (name, part)
     for empty in ("seqs", "total_q"):  # nothing to compute, nothing launched
         p = _varlen_params()
         setattr(p, empty, 0)
-        assert lib.sage_flash_varlen_fwd(p, None) == 0
+        assert lib.sage_flash_varlen_fwd(p, None, 0, None) == 0
 
 
 @pytest.mark.parametrize("field,value,status,message", [
@@ -205,6 +214,23 @@ def test_paged_workspace():
     assert lib.sage_paged_attn(p, None, 16, None) == -1 and lib.sage_paged_attn(p, 4100, n, None) == -1
     p.seqs = 0
     assert lib.sage_paged_attn(p, None, 0, None) == 0 and lib.sage_paged_attn_workspace_bytes(p) == 0
+
+
+def test_varlen_workspace():
+    """Few blocks against many keys are cut into equal shares: two partial results of 128 rows for each of 512 workgroups."""
+    from flagattention_amd import _lib
+
+    lib, p = _lib.load(), _varlen_params()
+    assert lib.sage_flash_varlen_workspace_bytes(p) == 0
+    p.total_q, p.total_k, p.seqs = 512, 17000, 1
+    assert lib.sage_flash_varlen_workspace_bytes(p) == 2 * 512 * 128 * (128 + 1) * 4
+    assert lib.sage_flash_varlen_fwd(p, None, 16, None) == -1 and lib.sage_flash_varlen_fwd(p, 4100, 1 << 30, None) == -1
+    p.total_q = 17000
+    assert lib.sage_flash_varlen_workspace_bytes(p) == 0
+    p.heads_q, p.heads_kv, p.total_q = 256, 1, 512  # (a query's rows do not fit a block)
+    assert lib.sage_flash_varlen_workspace_bytes(p) == 0
+    p.head_dim = 96
+    assert lib.sage_flash_varlen_workspace_bytes(p) == -1
 
 
 def test_cache_movement_validation():

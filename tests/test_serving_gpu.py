@@ -169,6 +169,42 @@ def test_varlen_long_sequence(gpu_device):
     _check_varlen(q, k, v, cu, cu, True)
 
 
+@pytest.fixture
+def workspaces(monkeypatch):
+    """The sizes of the workspaces that calls take."""
+    from flagattention_amd import serving
+
+    taken, make = [], serving.split_workspace
+    monkeypatch.setattr(serving, "split_workspace", lambda device, n: taken.append(n) or make(device, n))
+    return taken
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "fp16"), (128, "bf16")])
+@pytest.mark.parametrize("heads", [(4, 4), (8, 2), (7, 1), (3, 1), (40, 2)])
+@pytest.mark.parametrize("m,n", [((100,), (9000,)), ((40, 0, 129, 1), (5000, 7, 3003, 6000)), ((64, 70), (63, 12000)), ((3, 5, 200), (0, 8000, 150))])
+def test_varlen_cut_into_shares(m, n, heads, d, dtype, workspaces, gpu_device):
+    """Few queries against many keys: blocks that several workgroups share, shares that hold several blocks, blocks that see
+    nothing, sequences without keys or queries."""
+    h, hk = heads
+    q = _randn((sum(m), h, d), DTYPES[dtype], gpu_device, 0)
+    k, v = (_randn((sum(n), hk, d), DTYPES[dtype], gpu_device, i) for i in (1, 2))
+    for causal in (False, True):
+        _check_varlen(q, k, v, _cu(m, gpu_device), _cu(n, gpu_device), causal)
+    assert len(workspaces) == 4 and min(workspaces) > 0
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_varlen_cut_with_nonfinite_values(value, workspaces, gpu_device):
+    m, n = (70, 33), (4000, 5000)
+    q = _randn((sum(m), 8, 128), torch.bfloat16, gpu_device, 0)
+    k, v = (_randn((sum(n), 2, 128), torch.bfloat16, gpu_device, i) for i in (1, 2))
+    v[3999, 0, 5] = value
+    v[3970, 1, 100] = -value
+    v[4000 + 4980, 1, 0] = value
+    _check_varlen(q, k, v, _cu(m, gpu_device), _cu(n, gpu_device), True)
+    assert workspaces
+
+
 def test_varlen_agrees_with_the_rectangular_forward(gpu_device):
     """Sequences of one length are a batch: the same answers as flash_attention, to the rounding of P and of the output."""
     import flag_attn
