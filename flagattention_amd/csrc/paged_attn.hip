@@ -6,9 +6,9 @@
 //
 // Bound by the bytes of K and V: the rows of all query heads that share a K/V head (row r = query r / group, head r % group) are
 // multiplied from the same tiles, up to 32 rows at a time, so that the cache is read once.  A workgroup is four waves, and a wave
-// walks over 32-key tiles of its own without a barrier: S^T = K.Q^T and O^T += V^T.P^T on the 32x32 matrix instructions, K rows
-// straight into the operand, V through the wave's slice of LDS, from where it is read transposed.  The entries of the block table
-// are fetched a tile ahead of the rows they lead to.
+// walks over 32-key tiles of its own without a barrier: S^T = K.Q^T and O^T += V^T.P^T on the 16x16 matrix instructions, K rows
+// straight into the operand, V through the wave's slice of LDS, from where it is read transposed.  The registers of a tile are
+// requested anew as soon as their contents are used up, and the entries of the block table a tile ahead of the rows they lead to.
 //
 // The work is one line: sequence after sequence, K/V head after head, in chunks of 128 keys.  Every workgroup takes an equal
 // share of it, whatever the lengths are, which only the device knows: the end of one item (rows of a K/V head of a sequence),
@@ -25,8 +25,10 @@ constexpr int kPagedWaves = 4;
 constexpr int kPagedThreads = 64 * kPagedWaves;
 constexpr int kTileKeys = 32;
 constexpr int kChunk = kTileKeys * kPagedWaves;  // keys of a unit of the line: a tile for every wave
+#ifndef PAGED_WAVES
+#define PAGED_WAVES 2
+#endif
 constexpr int kPagedShares = 512;                // two workgroups on each compute unit
-constexpr int kRowsPerTile = 32;
 
 struct PagedArgs {
     const unsigned char* q;
@@ -40,7 +42,8 @@ struct PagedArgs {
     int64_t os_s, os_h, os_m, table_stride;                        // elements
     int32_t seqs, M, Hq, Hkv, groups, pages, page_size, page_shift;  // page_shift: log2 of page_size, -1: it has none
     int32_t capacity;                                                // keys that a row of the table can lead to
-    int32_t row_tiles, tile_rows;  // tiles of up to 32 rows of an item's queries; rows of one
+    int32_t row_waves;             // waves that share an item's rows, sixteen each: 1, 2 or 4
+    int32_t row_tiles, tile_rows;  // items that the rows of a K/V head make; rows of one
     int32_t shares;                // equal shares of the line; 0: a workgroup per item
     float qk_scale;                // sm_scale * log2(e)
     float* part_o;                 // [2 * shares][tile_rows][D]
@@ -57,26 +60,33 @@ __device__ __forceinline__ int line_total(const PagedArgs& a) {
     return wave_sum(sum) * a.Hkv * a.row_tiles;
 }
 
-template <int D> __device__ __forceinline__ int paged_v_swizzle(int row) { return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
+// V tiles in LDS: 16-byte chunk c of row r lies at chunk c ^ paged_v_swizzle(r), so that the sixteen rows which a transposed read
+// touches, 32 bytes each, spread over all banks.
+template <int D> __device__ __forceinline__ int paged_v_swizzle(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
 
-// SEVERAL: more than one new token per sequence, whose rows see different keys.
-template <int D, typename VT, bool SEVERAL>
-__global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs a) {
+// SEVERAL: more than one new token per sequence, whose rows see different keys.  PAGE16: the page size
+// is a multiple of 16, so that 16 keys of a tile share a page, whose address is then computed in scalar registers.
+template <int D, typename VT, bool SEVERAL, bool PAGE16>
+__global__ __launch_bounds__(kPagedThreads, PAGED_WAVES) void paged_attn_kernel(PagedArgs a) {
     using PVT = PV<VT>;
     using vec16 = typename PVT::vec;
-    constexpr int KSTEPS = D / 16;        // matrix instructions of a 32 x 32 score tile: 32 bytes of a row each
-    constexpr int DT = D / 32;
+    constexpr int KSTEPS = D / 32;        // matrix instructions of a 16 x 16 score tile: 64 bytes of a row each
+    constexpr int CT = D / 16;            // 16-channel tiles
     constexpr int V_RS = 2 * D;           // bytes per V row in LDS
     constexpr int VCPR = V_RS / 16;       // 16-byte chunks per V row
     constexpr int VLOADS = kTileKeys * VCPR / 64;
+    constexpr int VSTEP = 64 / VCPR;      // rows of a V load
     constexpr int V_TILE = kTileKeys * V_RS;
-    constexpr int SL_RS = 32 + 4;         // floats per row of the buffer in which the waves' results meet, 32 channels at a time
-    constexpr int SLICE = kPagedWaves * 32 * SL_RS * 4;
+    constexpr int SL_RS = D + 4;          // floats per row of the buffer in which the waves' results meet, sixteen rows at a time
+    constexpr int SLICE = kPagedWaves * 16 * SL_RS * 4;
     __shared__ __attribute__((aligned(16))) unsigned char smem[kPagedWaves * V_TILE > SLICE ? kPagedWaves * V_TILE : SLICE];
-    __shared__ float row_m[kPagedWaves][32], row_l[kPagedWaves][32];
+    __shared__ float row_m[kPagedWaves][16], row_l[kPagedWaves][16];
 
-    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Waves share the rows of an item, sixteen each, and then its key tiles.
+    const int row_waves = a.row_waves, key_waves = kPagedWaves / row_waves, row_wave = wave % row_waves;
+    const int kstep = kTileKeys * key_waves;
     const int per_seq = a.Hkv * a.row_tiles;  // items of a sequence
     const int rows = a.groups * a.M;
     int seq, pos, end, seq_begin;  // share of the line; where the sequence begins on it
@@ -95,21 +105,19 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
     }
     const int share_begin = pos;
 
-    const int vr0 = lane / VCPR, vchunk = lane % VCPR;  // V load e of a lane: row vr0 + e * 64 / VCPR, this chunk
+    const int vr0 = lane / VCPR, vchunk = lane % VCPR;  // V load e of a lane: row vr0 + VSTEP e, this chunk
     unsigned char* vlds = smem + wave * V_TILE;
-    int vtr[DT];  // LDS offsets of the transposed fragment reads (see attn_fast_kernel.h)
-    {
-        const int s4 = (lane >> 2) & 3, a4 = lane & 3, g1 = (lane >> 4) & 1;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-            vtr[dt] = (4 * half + s4) * V_RS + 16 * ((4 * dt + 2 * g1 + (a4 >> 1)) ^ paged_v_swizzle<D>(s4)) + 8 * (a4 & 1);
-    }
+    // ds_read_b64_tr_b16: in each group of 16 lanes, lane 4 s + c supplies channels 4 c .. of key row s, and lane i receives channel i
+    // of the four rows.  Group g reads keys 4 g .. and 16 + 4 g .. of the tile, where the lane's P come from.
+    const int vkey = 4 * quad + ((lane >> 2) & 3);
+    const int vtr = vkey * V_RS + 16 * (((lane & 3) >> 1) ^ paged_v_swizzle<D>(vkey)) + 8 * (lane & 1);
+    static_assert(D == 64 || D == 128, "swizzle periods");
 
     while (pos < end) {
         // ---- the piece: chunks `first` .. of an item
         const int len = seq_len(a, seq), chunks = seq_chunks(a, seq);
         const int item = (pos - seq_begin) / chunks, first = pos - seq_begin - item * chunks;
-        const int hk = item / a.row_tiles, row0 = item % a.row_tiles * kRowsPerTile;
+        const int hk = item / a.row_tiles, row0 = item % a.row_tiles * (16 * row_waves);
         const int n = min(chunks - first, end - pos);
         const bool whole = n == chunks;
         const int slot = 2 * (int)blockIdx.x + (pos != share_begin);
@@ -122,102 +130,131 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
         }
 
         // this lane's row; rows past the last one multiply a copy of it
-        const int r = min(row0 + l32, rows - 1);
-        const int mi = r / a.groups, h = hk * a.groups + r % a.groups;
+        const int wrow0 = row0 + 16 * row_wave, r = min(wrow0 + l16, rows - 1);
+        const int mi = SEVERAL ? r / a.groups : 0, h = hk * a.groups + (SEVERAL ? r % a.groups : r);
         v4i qf[KSTEPS];
         {
-            const unsigned char* qp = a.q + (int64_t)oseq * a.qs_s + (int64_t)h * a.qs_h + (int64_t)mi * a.qs_m + 16 * half;
+            const unsigned char* qp = a.q + (int64_t)oseq * a.qs_s + (int64_t)h * a.qs_h + (int64_t)mi * a.qs_m + 16 * quad;
 #pragma unroll
-            for (int t = 0; t < KSTEPS; t++) qf[t] = *reinterpret_cast<const v4i*>(qp + 32 * t);
+            for (int t = 0; t < KSTEPS; t++) qf[t] = *reinterpret_cast<const v4i*>(qp + 64 * t);
         }
-        const int my_last = len - a.M + mi;            // last key the row sees
-        const int all_see = len - a.M + row0 / a.groups;  // ... the tile's first row
+        const int my_last = len - a.M + mi;                                      // last key the row sees
+        const int all_see = len - a.M + min(wrow0, rows - 1) / a.groups;  // ... the wave's first row
 
         const unsigned char* kg = a.k + (int64_t)hk * a.ks_h;
         const unsigned char* vg = a.v + (int64_t)hk * a.vs_h;
-        const int32_t* table = a.table + (int64_t)oseq * a.table_stride;
-        // Key key0 + l32: its page, or -1 (no such key, or an entry that is no page), and its place in the page.
-        auto load_entry = [&](int key0) {
-            const int t = key0 + l32;
-            const int idx = a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size;
-            return t < kend ? table[idx] : -1;
-        };
-        auto place = [&](int key0) {
-            const int t = key0 + l32;
-            return a.page_shift >= 0 ? t & (a.page_size - 1) : t % a.page_size;
-        };
-        v4i kf[KSTEPS], vr[VLOADS];
-        // Rows of keys that do not exist read page 0: finite or not, they are taken out below.
-        auto load_k = [&](int page, int at) {
-            const unsigned char* p = kg + (int64_t)page * a.ks_p + (int64_t)at * a.ks_n + 16 * half;
+        typedef __attribute__((address_space(4))) const int32_t* const_i32_ptr;  // (scalar loads)
+        const const_i32_ptr table = (const_i32_ptr)(uintptr_t)(a.table + (int64_t)oseq * a.table_stride);
+        auto page_of = [&](int t) { return a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size; };
+        auto place_of = [&](int t) { return a.page_shift >= 0 ? t & (a.page_size - 1) : t % a.page_size; };
+
+        v4i kf[2][KSTEPS], vr[VLOADS];
+        // The tile's table entries: two in scalar registers, or one per lane, for key key0 + lane % 32.
+        int entry[2] = {-1, -1};
+        auto load_entries = [&](int key0) {
+            if constexpr (PAGE16) {
 #pragma unroll
-            for (int t = 0; t < KSTEPS; t++) kf[t] = *reinterpret_cast<const v4i*>(p + 32 * t);
-        };
-        auto load_v = [&](int page, int at) {
-            const int64_t mine = (int64_t)page * a.vs_p + (int64_t)at * a.vs_n;
-#pragma unroll
-            for (int e = 0; e < VLOADS; e++) {
-                const int from = vr0 + e * (64 / VCPR);  // the lane that knows the row
-                const unsigned lo = __shfl((int)(unsigned)mine, from);
-                const int hi = __shfl((int)(mine >> 32), from);
-                vr[e] = *reinterpret_cast<const v4i*>(vg + (((int64_t)hi << 32) | lo) + 16 * vchunk);
+                for (int u = 0; u < 2; u++) entry[u] = table[page_of(min(key0 + 16 * u, kend - 1))];
+            } else {
+                entry[0] = a.table[(int64_t)oseq * a.table_stride + page_of(min(key0 + (lane & 31), kend - 1))];
             }
+        };
+        // K and V of the tile whose entries are here, and which of its keys exist (bit j: key j).  Rows of keys that do not
+        // exist read a page that does: finite or not, they are taken out below.
+        auto load_tile = [&](int key0) {
+            unsigned seen = kend - key0 >= kTileKeys ? ~0u : kend > key0 ? (1u << (kend - key0)) - 1 : 0u;
+            if constexpr (PAGE16) {
+                const unsigned char *kp[2], *vp[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const bool ok = (unsigned)entry[u] < (unsigned)a.pages;
+                    if (!ok) seen &= u ? 0xffffu : 0xffff0000u;
+                    const int page = ok ? entry[u] : 0, at = place_of(key0 + 16 * u);
+                    kp[u] = kg + (int64_t)page * a.ks_p + (int64_t)at * a.ks_n;
+                    vp[u] = vg + (int64_t)page * a.vs_p + (int64_t)at * a.vs_n;
+                }
+                const unsigned koff = (unsigned)l16 * (unsigned)a.ks_n + 16 * quad, voff = (unsigned)vr0 * (unsigned)a.vs_n + 16 * vchunk;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int t = 0; t < KSTEPS; t++) kf[u][t] = *reinterpret_cast<const v4i*>(kp[u] + koff + 64 * t);
+#pragma unroll
+                for (int e = 0; e < VLOADS; e++) {
+                    const int r = VSTEP * e;  // (a load's rows lie in one half of the tile)
+                    vr[e] = *reinterpret_cast<const v4i*>(vp[r / 16] + (unsigned)(r % 16) * (unsigned)a.vs_n + voff);
+                }
+            } else {
+                const bool ok = (unsigned)entry[0] < (unsigned)a.pages;
+                seen &= (unsigned)__builtin_amdgcn_ballot_w64(ok);
+                const int64_t page = ok ? entry[0] : 0, at = ok ? place_of(min(key0 + (lane & 31), kend - 1)) : 0;
+                const int64_t ko = page * a.ks_p + at * a.ks_n, vo = page * a.vs_p + at * a.vs_n;
+                auto from = [&](int64_t x, int who) {  // the lane that knows the row
+                    return ((int64_t)__shfl((int)(x >> 32), who) << 32) | (unsigned)__shfl((int)(unsigned)x, who);
+                };
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const unsigned char* p = kg + from(ko, 16 * u + l16) + 16 * quad;
+#pragma unroll
+                    for (int t = 0; t < KSTEPS; t++) kf[u][t] = *reinterpret_cast<const v4i*>(p + 64 * t);
+                }
+#pragma unroll
+                for (int e = 0; e < VLOADS; e++) vr[e] = *reinterpret_cast<const v4i*>(vg + from(vo, vr0 + VSTEP * e) + 16 * vchunk);
+            }
+            return seen;
         };
 
         float m_i = -INFINITY, l_i = 0.0f;
-        v16f o[DT];
+        v4f o[CT];
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[dt][i] = 0.0f;
+        for (int ct = 0; ct < CT; ct++) o[ct] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-        int key0 = kbeg + kTileKeys * wave;
-        unsigned seen = 0, seen_next = 0;  // bit j: key j of the tile (of the next one) exists
-        int entry = -1;                    // of the next tile
+        int key0 = kbeg + kTileKeys * (wave / row_waves);
+        unsigned seen = 0;
         if (key0 < kend) {
-            const int e = load_entry(key0);
-            entry = load_entry(key0 + kChunk);
-            const bool ok = (unsigned)e < (unsigned)a.pages;
-            seen = (unsigned)__builtin_amdgcn_ballot_w64(ok);
-            const int page = ok ? e : 0, at = ok ? place(key0) : 0;
-            load_k(page, at);
-            load_v(page, at);
+            load_entries(key0);
+            seen = load_tile(key0);
+            load_entries(key0 + kstep);  // (past the end: the last entry once more)
         }
-        for (; key0 < kend; key0 += kChunk) {
-            const bool ok = (unsigned)entry < (unsigned)a.pages;  // (behind the last tile: no key, page 0 once more)
-            seen_next = (unsigned)__builtin_amdgcn_ballot_w64(ok);
-            const int page = ok ? entry : 0, at = ok ? place(key0 + kChunk) : 0;
-            entry = load_entry(key0 + 2 * kChunk);
-            // ---- S^T = K.Q^T; the K registers are requested anew right behind it
-            v16f s;
+        for (; key0 < kend; key0 += kstep) {
+            // ---- S^T = K.Q^T: register i of score tile u is key key0 + 16 u + 4 quad + i of the lane's row
+            v4f s[2];
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = 0.0f;
+            for (int u = 0; u < 2; u++) {
+                s[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int t = 0; t < KSTEPS; t++) s = PVT::mfma(__builtin_bit_cast(vec16, kf[t]), __builtin_bit_cast(vec16, qf[t]), s);
-            load_k(page, at);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int t = 0; t < KSTEPS; t++)
+                    s[u] = PVT::mfma16(__builtin_bit_cast(vec16, kf[u][t]), __builtin_bit_cast(vec16, qf[t]), s[u]);
+            }
             // ---- V tile -> LDS (the wave's own slice: a wave's LDS instructions run in order, no barrier); rows of keys that do
             //      not exist as zeros
 #pragma unroll
             for (int e = 0; e < VLOADS; e++) {
-                const int row = vr0 + e * (64 / VCPR);
+                const int row = vr0 + VSTEP * e;
                 if (seen != ~0u && !((seen >> row) & 1)) vr[e] = v4i{0, 0, 0, 0};
                 *reinterpret_cast<v4i*>(vlds + row * V_RS + 16 * (vchunk ^ paged_v_swizzle<D>(row))) = vr[e];
             }
-            load_v(page, at);
             __builtin_amdgcn_sched_barrier(0);
-            // ---- online softmax: register i of this lane is key key0 + 8 (i / 4) + 4 half + i % 4 of its row
+            // ---- the registers of K and V are requested anew
+            const unsigned tile_seen = seen;
+            seen = load_tile(key0 + kstep);
+            load_entries(key0 + 2 * kstep);
+            __builtin_amdgcn_sched_barrier(0);
+            // ---- online softmax
             const bool some_see = SEVERAL && key0 + kTileKeys - 1 > all_see;  // keys that some rows see and others do not
-            const bool hides = seen != ~0u || some_see;
-            float x[16];
             float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int j = 8 * (i >> 2) + 4 * half + (i & 3);
-                x[i] = s[i] * a.qk_scale;
-                if (hides) x[i] = ((seen >> j) & 1) && (!SEVERAL || key0 + j <= my_last) ? x[i] : -INFINITY;
-                mx = fmaxf(mx, x[i]);
-            }
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float x = s[u][i] * a.qk_scale;
+                    if (tile_seen != ~0u || some_see) {
+                        const int j = 16 * u + 4 * quad + i;
+                        x = ((tile_seen >> j) & 1) && (!SEVERAL || key0 + j <= my_last) ? x : -INFINITY;
+                    }
+                    s[u][i] = x;
+                    mx = fmaxf(mx, x);
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float m_new = fmaxf(m_i, mx);
             const float m_use = m_new == -INFINITY ? 0.0f : m_new;  // (no key seen yet: every P below is exp2(-inf) = 0)
@@ -225,101 +262,95 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
                 const float alpha = __builtin_amdgcn_exp2f(m_i - m_use);  // 0 for a row without a reference point
                 l_i *= alpha;
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++)
+                for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[dt][i] *= alpha;
+                    for (int i = 0; i < 4; i++) o[ct][i] *= alpha;
                 m_i = m_new;
             }
-            // P is rounded to 16 bits for the matrix instructions (at most 1, so half a step of 1 off); its sum is taken before that
-            vec16 pf[2];
+            // P is rounded to 16 bits for the matrix instructions (at most 1, half a step of itself off); its sum is taken before that
+            vec16 pf;
             float psum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float p = __builtin_amdgcn_exp2f(x[i] - m_use);
-                psum += p;
-                pf[i >> 3][i & 7] = (VT)p;
-            }
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float p = __builtin_amdgcn_exp2f(s[u][i] - m_use);
+                    psum += p;
+                    pf[4 * u + i] = (VT)p;
+                }
             l_i += psum;
             // ---- O^T += V^T.P^T
-            auto v_fragment = [&](int c, int dt) {
-                const unsigned char* p0 = vlds + vtr[dt] + 16 * c * V_RS;
+            auto v_fragment = [&](int ct) {  // channels 16 ct ..
+                const unsigned char* p0 = vlds + (vtr ^ (32 * ct));
                 const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p0);
-                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p0 + 8 * V_RS));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p0 + 16 * V_RS));
                 return __builtin_bit_cast(v4i, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             };
-            // An infinity or NaN in V under a hidden key must not reach the rows that do not see it (0 times it is NaN): where a tile
-            // that hides keys holds one, the matrix instructions get zeros in its place, and it is added to the rows that see its key.
+            // An infinity or NaN in V must not reach the rows that do not see its key (0 times it is NaN): where a tile that some rows
+            // see further into than others holds one, the matrix instructions get zeros in its place, and it is added to the rows
+            // that see its key.
             unsigned odd = 0;
             if (SEVERAL && some_see) {
 #pragma unroll
-                for (int c = 0; c < 2; c++)
+                for (int ct = 0; ct < CT; ct++) {
+                    const v4i f = v_fragment(ct);
 #pragma unroll
-                    for (int dt = 0; dt < DT; dt++) {
-                        const v4i f = v_fragment(c, dt);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) odd |= nonfinite_halves<VT>((unsigned)f[i]);
-                    }
+                    for (int i = 0; i < 4; i++) odd |= nonfinite_halves<VT>((unsigned)f[i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                asm volatile("" ::: "memory");  // (the fragments are read again below: kept they cost 32 registers)
             }
             if (!SEVERAL || __builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) == 0, 1)) {
 #pragma unroll
-                for (int c = 0; c < 2; c++)
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) o[dt] = PVT::mfma(__builtin_bit_cast(vec16, v_fragment(c, dt)), pf[c], o[dt]);
+                for (int ct = 0; ct < CT; ct++) o[ct] = PVT::mfma16(__builtin_bit_cast(vec16, v_fragment(ct)), pf, o[ct]);
             } else {
 #pragma unroll
-                for (int c = 0; c < 2; c++)
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++)
-                        o[dt] = PVT::mfma(__builtin_bit_cast(vec16, finite_only<VT>(v_fragment(c, dt))), pf[c], o[dt]);
-                add_nonfinite<D, VT>(vlds, [](int row) { return paged_v_swizzle<D>(row); }, pf[0], pf[1], my_last - key0 + 1, o);
+                for (int ct = 0; ct < CT; ct++) {
+                    o[ct] = PVT::mfma16(__builtin_bit_cast(vec16, finite_only<VT>(v_fragment(ct))), pf, o[ct]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                add_nonfinite<D, VT>(vlds, [](int row) { return paged_v_swizzle<D>(row); }, pf, my_last - key0 + 1, o);
             }
-            seen = seen_next;
         }
 
         // ---- the waves of the workgroup -> one normalized result and its log-sum-exp
-        const float l_tot = l_i + __shfl_xor(l_i, 32);
-        if (half == 0) {
-            row_m[wave][l32] = m_i;
-            row_l[wave][l32] = l_tot;
+        l_i += __shfl_xor(l_i, 16);
+        l_i += __shfl_xor(l_i, 32);
+        if (quad == 0) {
+            row_m[wave][l16] = m_i;
+            row_l[wave][l16] = l_i;
         }
         __syncthreads();
         float m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kPagedWaves; w++) m = fmaxf(m, row_m[w][l32]);
+        for (int w = row_wave; w < kPagedWaves; w += row_waves) m = fmaxf(m, row_m[w][l16]);
         const float m_use = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int w = 0; w < kPagedWaves; w++) l += row_l[w][l32] * __builtin_amdgcn_exp2f(row_m[w][l32] - m_use);
+        for (int w = row_wave; w < kPagedWaves; w += row_waves) l += row_l[w][l16] * __builtin_amdgcn_exp2f(row_m[w][l16] - m_use);
         // l = 0: a row that saw no key; its output is 0, its log-sum-exp -inf.  (NaN stays.)
         const float f = l != 0.0f ? __builtin_amdgcn_exp2f(m_i - m_use) / l : 0.0f;
-        if (wave == 0 && half == 0 && row0 + l32 < rows) {
+        if (wave == row_wave && quad == 0 && wrow0 + l16 < rows) {
             const float lse2 = __builtin_log2f(l) + m_use;
-            if (!whole) a.part_lse[(int64_t)slot * a.tile_rows + l32] = lse2;
+            if (!whole) a.part_lse[(int64_t)slot * a.tile_rows + 16 * row_wave + l16] = lse2;
             else if (a.lse) a.lse[((int64_t)oseq * a.Hq + h) * a.M + mi] = lse2 * 0.693147180559945309f;
         }
-        float* slice = reinterpret_cast<float*>(smem);
+        float* slice = reinterpret_cast<float*>(smem);  // (the V tiles have been read, since the barrier above)
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
-            __syncthreads();  // the V tiles / the previous channels have been read
+        for (int ct = 0; ct < CT; ct++)
+            *reinterpret_cast<v4f*>(slice + (wave * 16 + l16) * SL_RS + 16 * ct + 4 * quad) = v4f{o[ct][0] * f, o[ct][1] * f, o[ct][2] * f, o[ct][3] * f};
+        __syncthreads();
+        const int tile_end = min(16 * row_waves, rows - row0);  // rows that exist
+        for (int piece = tid; piece < tile_end * (D / 4); piece += kPagedThreads) {
+            const int orow = piece / (D / 4), c = 4 * (piece % (D / 4));
+            v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int w = orow / 16; w < kPagedWaves; w += row_waves) {
+                const v4f x = *reinterpret_cast<const v4f*>(slice + (w * 16 + orow % 16) * SL_RS + c);
 #pragma unroll
-            for (int g = 0; g < 4; g++)
-                *reinterpret_cast<v4f*>(slice + (wave * 32 + l32) * SL_RS + 8 * g + 4 * half) =
-                    v4f{o[dt][4 * g] * f, o[dt][4 * g + 1] * f, o[dt][4 * g + 2] * f, o[dt][4 * g + 3] * f};
-            __syncthreads();
-            const int orow = tid / 8, c = 4 * (tid % 8);  // 32 rows of eight groups of four channels
-            if (row0 + orow < rows) {
-                v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int w = 0; w < kPagedWaves; w++) {
-                    const v4f x = *reinterpret_cast<const v4f*>(slice + (w * 32 + orow) * SL_RS + c);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sum[i] += x[i];
-                }
-                const int om = (row0 + orow) / a.groups, oh = hk * a.groups + (row0 + orow) % a.groups;
-                if (whole)
-                    store_rounded(static_cast<VT*>(a.out) + (int64_t)oseq * a.os_s + (int64_t)oh * a.os_h + (int64_t)om * a.os_m + 32 * dt + c, sum);
-                else
-                    *reinterpret_cast<v4f*>(a.part_o + ((int64_t)slot * a.tile_rows + orow) * D + 32 * dt + c) = sum;
+                for (int i = 0; i < 4; i++) sum[i] += x[i];
             }
+            const int om = SEVERAL ? (row0 + orow) / a.groups : 0, oh = hk * a.groups + (SEVERAL ? (row0 + orow) % a.groups : row0 + orow);
+            if (whole)
+                store_rounded(static_cast<VT*>(a.out) + (int64_t)oseq * a.os_s + (int64_t)oh * a.os_h + (int64_t)om * a.os_m + c, sum);
+            else
+                *reinterpret_cast<v4f*>(a.part_o + ((int64_t)slot * a.tile_rows + orow) * D + c) = sum;
         }
         __syncthreads();  // (the next piece's V tiles go where the results lie)
     }
@@ -344,7 +375,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedArgs 
     const int first = line.owner(begin);
     if (begin == pos || first + 1 != cut) return;
     const int last = line.owner(begin + chunks - 1);
-    const int hk = item / a.row_tiles, row0 = item % a.row_tiles * kRowsPerTile, rows = a.groups * a.M;
+    const int hk = item / a.row_tiles, row0 = item % a.row_tiles * (16 * a.row_waves), rows = a.groups * a.M;
     const int c = 4 * (threadIdx.x % TPR), sg = (threadIdx.x / TPR) % SG;
     const int trow = blockIdx.y * ROWS + threadIdx.x / (TPR * SG);  // row of the tile
     if (row0 + (int)blockIdx.y * ROWS >= rows) return;
@@ -411,14 +442,15 @@ __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedArgs 
 }
 
 struct PagedPlan {
-    int64_t row_tiles, tile_rows, capacity, items, shares;
+    int64_t row_waves, row_tiles, tile_rows, capacity, items, shares;
 };
 
 PagedPlan plan_paged(const sage_paged_params& p) {
     PagedPlan plan;
     const int64_t rows = p.heads_q / p.heads_kv * p.new_tokens;
-    plan.row_tiles = (rows + kRowsPerTile - 1) / kRowsPerTile;
-    plan.tile_rows = rows < kRowsPerTile ? rows : kRowsPerTile;
+    plan.row_waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    plan.row_tiles = (rows + 16 * plan.row_waves - 1) / (16 * plan.row_waves);
+    plan.tile_rows = rows < 16 * plan.row_waves ? rows : 16 * plan.row_waves;
     const int64_t most = 0x7fffffffLL - 4 * kChunk;
     plan.capacity = p.table_width > most / p.page_size ? most : p.table_width * p.page_size;
     plan.items = p.seqs * p.heads_kv * plan.row_tiles;
@@ -439,8 +471,12 @@ int64_t paged_workspace_bytes(const sage_paged_params& p) {
 
 template <int D, typename VT>
 static int launch_paged(const PagedArgs& a, int64_t wgs, hipStream_t stream) {
-    if (a.M > 1) hipLaunchKernelGGL((paged_attn_kernel<D, VT, true>), dim3((unsigned)wgs), dim3(kPagedThreads), 0, stream, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<D, VT, false>), dim3((unsigned)wgs), dim3(kPagedThreads), 0, stream, a);
+    const dim3 grid((unsigned)wgs), block(kPagedThreads);
+    const bool page16 = a.page_size % 16 == 0;
+    if (a.M > 1 && page16) hipLaunchKernelGGL((paged_attn_kernel<D, VT, true, true>), grid, block, 0, stream, a);
+    else if (a.M > 1) hipLaunchKernelGGL((paged_attn_kernel<D, VT, true, false>), grid, block, 0, stream, a);
+    else if (page16) hipLaunchKernelGGL((paged_attn_kernel<D, VT, false, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<D, VT, false, false>), grid, block, 0, stream, a);
     if (int rc = check_launch("paged_attn_kernel")) return rc;
     if (a.shares < 2) return SAGE_OK;
     constexpr int rows = kPagedThreads / D;
@@ -463,7 +499,7 @@ int launch_paged_attn(const sage_paged_params& p, void* workspace, int64_t works
     a.groups = (int)(p.heads_q / p.heads_kv);
     a.pages = (int)p.pages; a.page_size = (int)p.page_size;
     a.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)p.page_size) : -1;
-    a.capacity = (int)plan.capacity; a.row_tiles = (int)plan.row_tiles; a.tile_rows = (int)plan.tile_rows;
+    a.capacity = (int)plan.capacity; a.row_tiles = (int)plan.row_tiles; a.row_waves = (int)plan.row_waves; a.tile_rows = (int)plan.tile_rows;
     a.shares = (int)plan.shares;
     a.qk_scale = p.sm_scale * 1.44269504089f;
     a.part_o = (float*)workspace;

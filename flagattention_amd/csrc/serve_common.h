@@ -85,43 +85,39 @@ __device__ __forceinline__ v4i finite_only(v4i x) {
     return x;
 }
 
-// What the infinities and NaN of a V tile in LDS add to the outputs of a lane's row: for every key j < see_end of the tile and
-// every channel that the lane holds.  p0, p1: the lane's P of the tile's keys 8 (i / 4) + 4 half + i % 4, i < 8 and the others.
-// V row j, chunk c lies at row j * 2 D + 16 (c ^ swizzle(j)).  Slow, and hardly ever called.
+// What the infinities and NaN of a 32-key V tile in LDS add to the outputs of a lane's row (16x16 layout: accumulator i of tile ct is
+// channel 16 ct + 4 quad + i): for every key j < see_end of the tile and every channel that the lane holds.  p: the lane's P of the
+// keys 16 (e / 4) + 4 quad + e % 4.  V row j, chunk c lies at row j * 2 D + 16 (c ^ swizzle(j)).  Slow, and hardly ever called.
 template <int D, typename VT, typename Swizzle>
-__device__ __forceinline__ void add_nonfinite(const unsigned char* vtile, Swizzle&& swizzle, typename PV<VT>::vec p0, typename PV<VT>::vec p1,
-                                              int see_end, v16f (&acc)[D / 32]) {
-    const int half = (threadIdx.x >> 5) & 1;
-    const v4i w0 = __builtin_bit_cast(v4i, p0), w1 = __builtin_bit_cast(v4i, p1);
+__device__ __forceinline__ void add_nonfinite(const unsigned char* vtile, Swizzle&& swizzle, typename PV<VT>::vec p, int see_end, v4f (&acc)[D / 16]) {
+    const int lane = threadIdx.x & 63, quad = lane >> 4;
+    const v4i words = __builtin_bit_cast(v4i, p);
 #pragma unroll 1
     for (int j = 0; j < 32; j++) {
-        const int owner = (j >> 2) & 1, reg = 4 * (j >> 3) + (j & 3);  // P of key j: number reg of the lane of that half
+        const int owner = (j >> 2) & 3, e = 4 * (j >> 4) + (j & 3);  // P of key j: number e of the lane of that quad
         unsigned pair = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int w = i < 4 ? w0[i & 3] : w1[i & 3];
-            pair = i == reg >> 1 ? (unsigned)w : pair;
+        for (int i = 0; i < 4; i++) {
+            const int w = words[i];
+            pair = i == e >> 1 ? (unsigned)w : pair;
         }
-        const float mine = (float)__builtin_bit_cast(VT, (unsigned short)(reg & 1 ? pair >> 16 : pair));
-        const float other = __shfl_xor(mine, 32);
-        const float pj = owner == half ? mine : other;
+        const float mine = (float)__builtin_bit_cast(VT, (unsigned short)(e & 1 ? pair >> 16 : pair));
+        const float pj = __shfl(mine, 16 * owner + (lane & 15));
         const bool sees = j < see_end;
 #pragma unroll
-        for (int dt = 0; dt < D / 32; dt++)
+        for (int ct = 0; ct < D / 16; ct++) {
+            typedef unsigned v2u __attribute__((ext_vector_type(2)));
+            const v2u w = *reinterpret_cast<const v2u*>(vtile + j * (2 * D) + 16 * ((2 * ct + (quad >> 1)) ^ swizzle(j)) + 8 * (quad & 1));
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                typedef unsigned v2u __attribute__((ext_vector_type(2)));
-                const v2u w = *reinterpret_cast<const v2u*>(vtile + j * (2 * D) + 16 * ((4 * dt + g) ^ swizzle(j)) + 8 * half);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const unsigned word = w[i >> 1];
-                    const unsigned z = nonfinite_halves<VT>(word);
-                    const float v = (float)__builtin_bit_cast(VT, (unsigned short)(word >> (16 * (i & 1))));
-                    const bool odd = (z >> (15 + 16 * (i & 1))) & 1;
-                    acc[dt][4 * g + i] = sees && odd ? __builtin_fmaf(pj, v, acc[dt][4 * g + i]) : acc[dt][4 * g + i];
-                }
-                __builtin_amdgcn_sched_barrier(0);  // (a few registers at a time)
+            for (int i = 0; i < 4; i++) {
+                const unsigned word = w[i >> 1];
+                const unsigned z = nonfinite_halves<VT>(word);
+                const float v = (float)__builtin_bit_cast(VT, (unsigned short)(word >> (16 * (i & 1))));
+                const bool odd = (z >> (15 + 16 * (i & 1))) & 1;
+                acc[ct][i] = sees && odd ? __builtin_fmaf(pj, v, acc[ct][i]) : acc[ct][i];
             }
+            __builtin_amdgcn_sched_barrier(0);  // (a few registers at a time)
+        }
     }
 }
 
