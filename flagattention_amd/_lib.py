@@ -222,7 +222,8 @@ class _PythonHost:
     def quant(*call):
         return None
 
-    attn = flash = put_quant = put_attn = put_flash = quant
+    attn = flash = varlen = paged = append = copy = quant
+    put_quant = put_attn = put_flash = put_varlen = put_paged = put_append = put_copy = quant
 
 
 def host():

@@ -1,7 +1,7 @@
 // Native host side of the calls whose shape has been seen before: a CPython extension (module flagattention_amd._host) that
 // finds the filled parameter struct of a call by the metadata of its tensors, allocates the outputs and calls the library.
 //
-// The Python functions (sage_attention/quant.py, sage_attention/attention.py, flash.py) check the arguments of a call, fill the
+// The Python functions (sage_attention/quant.py, sage_attention/attention.py, flash.py, serving.py) check the arguments of a call, fill the
 // parameter struct and register it here under the call's key: every size, stride, dtype and flag that the checks and the
 // struct depend on.  A later call with the same key has passed the same checks, so only pointers are written (their
 // alignment, the one property of a call that the key does not hold, is looked at every time).  Anything else - a tensor
@@ -144,7 +144,7 @@ PyObject* put(const Key& key, PyObject* params, PyObject* ws, bool fused) {
     Py_ssize_t size;
     if (PyBytes_AsStringAndSize(params, &data, &size) < 0) return nullptr;
     plan.params.assign(data, (size_t)size);
-    plan.workspace = PyLong_AsLongLong(ws);
+    if (ws) plan.workspace = PyLong_AsLongLong(ws);
     if (PyErr_Occurred()) return nullptr;
     plan.fused = fused;
     make_room();
@@ -371,6 +371,187 @@ PyObject* put_flash(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params
     });
 }
 
+// A scale given as None or as a float: part of the key.
+bool add_scale(Key& key, PyObject* o) {
+    if (o == Py_None) key.add((int64_t)0);
+    else if (PyFloat_CheckExact(o)) {
+        key.add((int64_t)1);
+        key.add(PyFloat_AS_DOUBLE(o));
+    } else return false;
+    return true;
+}
+
+// Tensors a[from] .. a[to - 1], without gradients, into the key.
+bool add_tensors(Key& key, PyObject* const* a, int from, int to, const at::Tensor** t) {
+    for (int i = from; i < to; i++) {
+        if (!plain(a[i])) return false;
+        t[i] = &THPVariable_Unpack(a[i]);
+        if (t[i]->requires_grad()) return false;
+        key.add(*t[i]);
+    }
+    key.add((int64_t)t[from]->device().index());
+    return true;
+}
+
+// The first `rows` tensors are ready (aligned rows), and all of them on the current device, which is dev.
+bool all_ready(const at::Tensor* const* t, int rows, int all, const at::Device& dev) {
+    if (!dev.is_cuda() || c10::hip::current_device() != dev.index()) return false;
+    for (int i = 0; i < rows; i++)
+        if (!ready(*t[i], dev)) return false;
+    for (int i = rows; i < all; i++)
+        if (t[i]->device() != dev) return false;
+    return true;
+}
+
+// ---- packed sequences: (q, k, v, cu_seqlens_q, cu_seqlens_k, causal, sm_scale, want_log_normalizer)
+struct VarlenCall {
+    const at::Tensor* t[5];
+    bool causal, want_l;
+    Key key;
+    bool parse(PyObject* const* a, Py_ssize_t n) {
+        if (n < 8 || !is_bool(a[5], causal) || !is_bool(a[7], want_l)) return false;
+        key.add((int64_t)4);
+        if (!add_tensors(key, a, 0, 5, t) || !add_scale(key, a[6])) return false;
+        key.add((int64_t)causal);
+        return true;
+    }
+};
+
+PyObject* varlen(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        VarlenCall c;
+        if (!c.parse(a, n)) return none();
+        Plan* plan = find(c.key);
+        if (!plan) return none();
+        const at::Device dev = c.t[0]->device();
+        if (!all_ready(c.t, 3, 5, dev)) return none();
+        auto& p = *reinterpret_cast<sage_varlen_params*>(&plan->params[0]);
+        const at::Tensor o = at::empty(c.t[0]->sizes(), options(dev, c.t[0]->scalar_type()));
+        at::Tensor l;
+        if (c.want_l) l = at::empty({p.heads_q, p.total_q}, options(dev, at::kFloat));
+        p.q.ptr = c.t[0]->data_ptr(); p.k.ptr = c.t[1]->data_ptr(); p.v.ptr = c.t[2]->data_ptr(); p.out.ptr = o.data_ptr();
+        p.log_normalizer = c.want_l ? (float*)l.data_ptr() : nullptr;
+        p.cu_seqlens_q = (const int32_t*)c.t[3]->data_ptr(); p.cu_seqlens_k = (const int32_t*)c.t[4]->data_ptr();
+        void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+        at::Tensor ws;
+        if (plan->workspace > 0) ws = workspace(dev, plan->workspace);
+        if (int rc = sage_flash_varlen_fwd(&p, plan->workspace > 0 ? ws.data_ptr() : nullptr, plan->workspace, stream)) return PyLong_FromLong(rc);
+        return pack({&o, c.want_l ? &l : nullptr});
+    });
+}
+
+PyObject* put_varlen(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params, workspace bytes)
+    return guarded([&]() -> PyObject* {
+        VarlenCall c;
+        if (n != 10 || !c.parse(a, n)) return none();
+        return put(c.key, a[8], a[9], false);
+    });
+}
+
+// ---- paged attention: (q, k_cache, v_cache, block_table, seq_lens, sm_scale, layout, want_log_normalizer)
+struct PagedCall {
+    const at::Tensor* t[5];
+    bool hnd, want_l;
+    Key key;
+    bool parse(PyObject* const* a, Py_ssize_t n) {
+        if (n < 8 || !is_hnd(a[6], hnd) || !is_bool(a[7], want_l)) return false;
+        key.add((int64_t)5);
+        if (!add_tensors(key, a, 0, 5, t) || !add_scale(key, a[5])) return false;
+        key.add((int64_t)hnd);
+        return true;
+    }
+};
+
+PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        PagedCall c;
+        if (!c.parse(a, n)) return none();
+        Plan* plan = find(c.key);
+        if (!plan) return none();
+        const at::Device dev = c.t[0]->device();
+        if (!all_ready(c.t, 3, 5, dev)) return none();
+        auto& p = *reinterpret_cast<sage_paged_params*>(&plan->params[0]);
+        const at::Tensor o = at::empty(c.t[0]->sizes(), options(dev, c.t[0]->scalar_type()));
+        at::Tensor l;
+        if (c.want_l) l = c.t[0]->dim() == 3 ? at::empty({p.seqs, p.heads_q}, options(dev, at::kFloat))
+                                             : at::empty({p.seqs, p.heads_q, p.new_tokens}, options(dev, at::kFloat));
+        p.q.ptr = c.t[0]->data_ptr(); p.out.ptr = o.data_ptr(); p.k_cache.ptr = c.t[1]->data_ptr(); p.v_cache.ptr = c.t[2]->data_ptr();
+        p.log_normalizer = c.want_l ? (float*)l.data_ptr() : nullptr;
+        p.block_table = (const int32_t*)c.t[3]->data_ptr(); p.seq_lens = (const int32_t*)c.t[4]->data_ptr();
+        void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+        at::Tensor ws;
+        if (plan->workspace > 0) ws = workspace(dev, plan->workspace);
+        if (int rc = sage_paged_attn(&p, plan->workspace > 0 ? ws.data_ptr() : nullptr, plan->workspace, stream)) return PyLong_FromLong(rc);
+        return pack({&o, c.want_l ? &l : nullptr});
+    });
+}
+
+PyObject* put_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params, workspace bytes)
+    return guarded([&]() -> PyObject* {
+        PagedCall c;
+        if (n != 10 || !c.parse(a, n)) return none();
+        return put(c.key, a[8], a[9], false);
+    });
+}
+
+// ---- the cache's movements, which return a status where the plan is known: (k, v, k_cache, v_cache, slots, layout) and
+//      (k_cache, v_cache, src, dst)
+struct MoveCall {
+    const at::Tensor* t[5];
+    int tensors;
+    Key key;
+    bool parse(PyObject* const* a, Py_ssize_t n, int tensors_) {
+        tensors = tensors_;
+        bool hnd = false;
+        if (n < tensors + (tensors == 5) || (tensors == 5 && !is_hnd(a[5], hnd))) return false;
+        key.add((int64_t)(1 + tensors + 2 * hnd) << 8);
+        return add_tensors(key, a, 0, tensors, t);
+    }
+};
+
+PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        MoveCall c;
+        if (!c.parse(a, n, 5)) return none();
+        Plan* plan = find(c.key);
+        const at::Device dev = c.t[0]->device();
+        if (!plan || !all_ready(c.t, 4, 5, dev)) return none();
+        auto& p = *reinterpret_cast<sage_append_params*>(&plan->params[0]);
+        p.k.ptr = c.t[0]->data_ptr(); p.v.ptr = c.t[1]->data_ptr(); p.k_cache.ptr = c.t[2]->data_ptr(); p.v_cache.ptr = c.t[3]->data_ptr();
+        p.slots = c.t[4]->data_ptr();
+        return PyLong_FromLong(sage_cache_append(&p, c10::hip::getCurrentHIPStream(dev.index()).stream()));
+    });
+}
+
+PyObject* put_append(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params)
+    return guarded([&]() -> PyObject* {
+        MoveCall c;
+        if (n != 7 || !c.parse(a, n, 5)) return none();
+        return put(c.key, a[6], nullptr, false);
+    });
+}
+
+PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        MoveCall c;
+        if (!c.parse(a, n, 4)) return none();
+        Plan* plan = find(c.key);
+        const at::Device dev = c.t[0]->device();
+        if (!plan || !all_ready(c.t, 2, 4, dev)) return none();
+        auto& p = *reinterpret_cast<sage_copy_params*>(&plan->params[0]);
+        p.k_cache = c.t[0]->data_ptr(); p.v_cache = c.t[1]->data_ptr(); p.src = c.t[2]->data_ptr(); p.dst = c.t[3]->data_ptr();
+        return PyLong_FromLong(sage_cache_copy_pages(&p, c10::hip::getCurrentHIPStream(dev.index()).stream()));
+    });
+}
+
+PyObject* put_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params)
+    return guarded([&]() -> PyObject* {
+        MoveCall c;
+        if (n != 5 || !c.parse(a, n, 4)) return none();
+        return put(c.key, a[4], nullptr, false);
+    });
+}
+
 PyMethodDef methods[] = {
     {"quant", (PyCFunction)(void (*)(void))quant, METH_FASTCALL, "outputs of a quantizer call whose plan is known, None, or a status"},
     {"put_quant", (PyCFunction)(void (*)(void))put_quant, METH_FASTCALL, "registers the plan of a quantizer call"},
@@ -378,6 +559,14 @@ PyMethodDef methods[] = {
     {"put_attn", (PyCFunction)(void (*)(void))put_attn, METH_FASTCALL, "registers the plan of a SageAttention call"},
     {"flash", (PyCFunction)(void (*)(void))flash, METH_FASTCALL, "outputs of a dense forward call whose plan is known, None, or a status"},
     {"put_flash", (PyCFunction)(void (*)(void))put_flash, METH_FASTCALL, "registers the plan of a dense forward call"},
+    {"varlen", (PyCFunction)(void (*)(void))varlen, METH_FASTCALL, "outputs of a call over packed sequences whose plan is known, None, or a status"},
+    {"put_varlen", (PyCFunction)(void (*)(void))put_varlen, METH_FASTCALL, "registers the plan of a call over packed sequences"},
+    {"paged", (PyCFunction)(void (*)(void))paged, METH_FASTCALL, "outputs of a paged attention call whose plan is known, None, or a status"},
+    {"put_paged", (PyCFunction)(void (*)(void))put_paged, METH_FASTCALL, "registers the plan of a paged attention call"},
+    {"append", (PyCFunction)(void (*)(void))append, METH_FASTCALL, "status of a cache write whose plan is known, or None"},
+    {"put_append", (PyCFunction)(void (*)(void))put_append, METH_FASTCALL, "registers the plan of a cache write"},
+    {"copy", (PyCFunction)(void (*)(void))copy, METH_FASTCALL, "status of a page copy whose plan is known, or None"},
+    {"put_copy", (PyCFunction)(void (*)(void))put_copy, METH_FASTCALL, "registers the plan of a page copy"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "native host side of calls whose shape has been seen before", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -21,14 +21,12 @@ namespace {
 
 using namespace attn;
 
-constexpr int kPagedWaves = 4;
+constexpr int kPagedWaves = 4;   // (eight, for one workgroup on a compute unit: 10 to 20 % slower)
 constexpr int kPagedThreads = 64 * kPagedWaves;
 constexpr int kTileKeys = 32;
-constexpr int kChunk = kTileKeys * kPagedWaves;  // keys of a unit of the line: a tile for every wave
-#ifndef PAGED_WAVES
-#define PAGED_WAVES 2
-#endif
+constexpr int kChunk = kTileKeys * kPagedWaves;  // keys of a unit of the line
 constexpr int kPagedShares = 512;                // two workgroups on each compute unit
+constexpr int kCombineThreads = 256;
 
 struct PagedArgs {
     const unsigned char* q;
@@ -67,7 +65,7 @@ template <int D> __device__ __forceinline__ int paged_v_swizzle(int row) { retur
 // SEVERAL: more than one new token per sequence, whose rows see different keys.  PAGE16: the page size
 // is a multiple of 16, so that 16 keys of a tile share a page, whose address is then computed in scalar registers.
 template <int D, typename VT, bool SEVERAL, bool PAGE16>
-__global__ __launch_bounds__(kPagedThreads, PAGED_WAVES) void paged_attn_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs a) {
     using PVT = PV<VT>;
     using vec16 = typename PVT::vec;
     constexpr int KSTEPS = D / 32;        // matrix instructions of a 16 x 16 score tile: 64 bytes of a row each
@@ -151,7 +149,7 @@ __global__ __launch_bounds__(kPagedThreads, PAGED_WAVES) void paged_attn_kernel(
         v4i kf[2][KSTEPS], vr[VLOADS];
         // The tile's table entries: two in scalar registers, or one per lane, for key key0 + lane % 32.
         int entry[2] = {-1, -1};
-        auto load_entries = [&](int key0) {
+        auto load_entries = [&](int key0) {  // (past the end: the last one once more)
             if constexpr (PAGE16) {
 #pragma unroll
                 for (int u = 0; u < 2; u++) entry[u] = table[page_of(min(key0 + 16 * u, kend - 1))];
@@ -213,7 +211,7 @@ __global__ __launch_bounds__(kPagedThreads, PAGED_WAVES) void paged_attn_kernel(
         if (key0 < kend) {
             load_entries(key0);
             seen = load_tile(key0);
-            load_entries(key0 + kstep);  // (past the end: the last entry once more)
+            load_entries(key0 + kstep);
         }
         for (; key0 < kend; key0 += kstep) {
             // ---- S^T = K.Q^T: register i of score tile u is key key0 + 16 u + 4 quad + i of the lane's row
@@ -356,25 +354,40 @@ __global__ __launch_bounds__(kPagedThreads, PAGED_WAVES) void paged_attn_kernel(
     }
 }
 
-// The parts of the items that were cut: lse = log2 sum_s 2^lse_s, out = sum_s 2^(lse_s - lse) o_s.  A workgroup per cut between two
-// shares; the first cut inside an item takes care of it.  SG groups of D / 4 threads share the parts of a row.
-template <int D, typename VT>
-__global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedArgs a) {
-    constexpr int TPR = D / 4, SG = 4, ROWS = kPagedThreads / (TPR * SG);
+// The parts of the items that were cut: lse = log2 sum_s 2^lse_s, out = sum_s 2^(lse_s - lse) o_s.  A workgroup per item (BY_ITEM) and
+// few of its rows, or, where the items outnumber the cuts, per cut between two shares: the first cut inside an item takes care of it
+// (per item: 32 sequences x 8 K/V heads 58.2 -> 57.6 us for the whole call, 1000 x 8 450 -> 470).  SG groups of D / 4 threads share
+// the parts of a row.
+template <int D, typename VT, bool BY_ITEM>
+__global__ __launch_bounds__(kCombineThreads) void paged_combine_kernel(PagedArgs a) {
+    constexpr int TPR = D / 4, SG = 4, ROWS = kCombineThreads / (TPR * SG);
     constexpr int kBatch = 8;  // loads on their way together
-    __shared__ float sm_m[kPagedThreads], sm_den[kPagedThreads];
-    __shared__ v4f sm_acc[kPagedThreads];
-    const EqualShares line(line_total(a), a.shares);
-    const int cut = blockIdx.x + 1, pos = line.begin(cut);
+    __shared__ float sm_m[kCombineThreads], sm_den[kCombineThreads];
+    __shared__ v4f sm_acc[kCombineThreads];
     const int per_seq = a.Hkv * a.row_tiles;
-    int seq, seq_begin;
-    if (line.begin(cut + 1) <= pos) return;  // (the shares from here on are empty)
-    if (!find_run(a.seqs, pos, [&](int s) { return seq_chunks(a, s) * per_seq; }, seq, seq_begin)) return;
-    const int chunks = seq_chunks(a, seq), item = (pos - seq_begin) / chunks;
-    const int begin = seq_begin + item * chunks;
-    const int first = line.owner(begin);
-    if (begin == pos || first + 1 != cut) return;
-    const int last = line.owner(begin + chunks - 1);
+    int seq, item, begin;  // begin: of the item on the line
+    int all = 0, before = 0;  // chunks of the sequences; of those before this workgroup's
+    for (int i = threadIdx.x & 63; i < a.seqs; i += 64) {
+        const int n = seq_chunks(a, i);
+        all += n;
+        before += i < (int)blockIdx.x / per_seq ? n : 0;
+    }
+    const EqualShares line(wave_sum(all) * per_seq, a.shares);
+    if (BY_ITEM) {
+        seq = blockIdx.x / per_seq;
+        item = blockIdx.x % per_seq;
+        begin = wave_sum(before) * per_seq + item * seq_chunks(a, seq);
+    } else {
+        const int pos = line.begin(blockIdx.x + 1);
+        if (pos >= line.begin(blockIdx.x + 2)) return;  // (the shares from here on are empty)
+        if (!find_run(a.seqs, pos, [&](int s) { return seq_chunks(a, s) * per_seq; }, seq, begin)) return;
+        item = (pos - begin) / seq_chunks(a, seq);
+        begin += item * seq_chunks(a, seq);
+        if (begin == pos || line.owner(begin) != (int)blockIdx.x) return;
+    }
+    const int chunks = seq_chunks(a, seq);
+    const int first = line.owner(begin), last = line.owner(begin + chunks - 1);
+    if (first == last) return;  // (whole)
     const int hk = item / a.row_tiles, row0 = item % a.row_tiles * (16 * a.row_waves), rows = a.groups * a.M;
     const int c = 4 * (threadIdx.x % TPR), sg = (threadIdx.x / TPR) % SG;
     const int trow = blockIdx.y * ROWS + threadIdx.x / (TPR * SG);  // row of the tile
@@ -470,7 +483,9 @@ int64_t paged_workspace_bytes(const sage_paged_params& p) {
 }
 
 template <int D, typename VT>
-static int launch_paged(const PagedArgs& a, int64_t wgs, hipStream_t stream) {
+static int launch_paged(const PagedArgs& a, const PagedPlan& plan, hipStream_t stream) {
+    const int64_t wgs = plan.shares ? plan.shares : plan.items;
+    if (wgs > 0x7fffffffLL || plan.items > 0x7fffffffLL) return fail(SAGE_E_UNSUPPORTED, "sage_paged_attn: too many workgroups for one launch");
     const dim3 grid((unsigned)wgs), block(kPagedThreads);
     const bool page16 = a.page_size % 16 == 0;
     if (a.M > 1 && page16) hipLaunchKernelGGL((paged_attn_kernel<D, VT, true, true>), grid, block, 0, stream, a);
@@ -479,9 +494,12 @@ static int launch_paged(const PagedArgs& a, int64_t wgs, hipStream_t stream) {
     else hipLaunchKernelGGL((paged_attn_kernel<D, VT, false, false>), grid, block, 0, stream, a);
     if (int rc = check_launch("paged_attn_kernel")) return rc;
     if (a.shares < 2) return SAGE_OK;
-    constexpr int rows = kPagedThreads / D;
-    hipLaunchKernelGGL((paged_combine_kernel<D, VT>), dim3((unsigned)(a.shares - 1), (unsigned)((a.tile_rows + rows - 1) / rows)),
-                       dim3(kPagedThreads), 0, stream, a);
+    constexpr int rows = kCombineThreads / D;
+    const unsigned row_groups = (unsigned)((a.tile_rows + rows - 1) / rows);
+    if (plan.items < a.shares)
+        hipLaunchKernelGGL((paged_combine_kernel<D, VT, true>), dim3((unsigned)plan.items, row_groups), dim3(kCombineThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((paged_combine_kernel<D, VT, false>), dim3((unsigned)a.shares - 1, row_groups), dim3(kCombineThreads), 0, stream, a);
     return check_launch("paged_combine_kernel");
 }
 
@@ -504,10 +522,8 @@ int launch_paged_attn(const sage_paged_params& p, void* workspace, int64_t works
     a.qk_scale = p.sm_scale * 1.44269504089f;
     a.part_o = (float*)workspace;
     a.part_lse = a.part_o + 2 * plan.shares * plan.tile_rows * p.head_dim;
-    if (plan.shares == 0 && plan.items > 0x7fffffffLL) return fail(SAGE_E_UNSUPPORTED, "sage_paged_attn: too many workgroups for one launch");
-    const int64_t wgs = plan.shares ? plan.shares : plan.items;
-    if (p.head_dim == 128) return p.dtype == SAGE_BF16 ? launch_paged<128, __bf16>(a, wgs, stream) : launch_paged<128, _Float16>(a, wgs, stream);
-    return p.dtype == SAGE_BF16 ? launch_paged<64, __bf16>(a, wgs, stream) : launch_paged<64, _Float16>(a, wgs, stream);
+    if (p.head_dim == 128) return p.dtype == SAGE_BF16 ? launch_paged<128, __bf16>(a, plan, stream) : launch_paged<128, _Float16>(a, plan, stream);
+    return p.dtype == SAGE_BF16 ? launch_paged<64, __bf16>(a, plan, stream) : launch_paged<64, _Float16>(a, plan, stream);
 }
 
 }  // namespace sage

@@ -22,6 +22,10 @@ from .sage_attention._common import DTYPE_CODE, current_stream_ptr, device_guard
 __all__ = ["flash_attention_varlen", "paged_attention", "append_to_cache", "copy_pages"]
 
 
+def _host():
+    return _lib._host_module or _lib.host()
+
+
 def _no_grad(what, *tensors):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise NotImplementedError(f"{what}: forward only (no backward pass is built); call it under torch.no_grad() or on "
@@ -119,6 +123,13 @@ def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fals
     """
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q
+    call = (q, k, v, cu_seqlens_q, cu_seqlens_k, causal, sm_scale, return_log_normalizer)
+    if out is None:
+        res = _host().varlen(*call)  # a call shape seen before: (o, log normalizer), or a status
+        if res is not None:
+            if type(res) is int:
+                _lib.check(res, "sage_flash_varlen_fwd")
+            return res if return_log_normalizer else res[0]
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k, v must be (tokens, heads, head_dim) tensors")
     T, H, D = q.shape
@@ -162,6 +173,8 @@ def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fals
         ws_bytes = lib.sage_flash_varlen_workspace_bytes(p)
         if ws_bytes < 0:
             _lib.check(-1, "sage_flash_varlen_workspace_bytes")
+        if out is None and all(x is y for x, y in zip((q, k, v, cu_seqlens_q, cu_seqlens_k), call)):  # (nothing was copied)
+            _host().put_varlen(*call, bytes(p), ws_bytes)
         ws = split_workspace(q.device, ws_bytes) if ws_bytes else None
         _lib.check(lib.sage_flash_varlen_fwd(p, ws.data_ptr() if ws is not None else None, ws_bytes, current_stream_ptr(q.device)),
                    "sage_flash_varlen_fwd")
@@ -184,6 +197,13 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
     Returns ``o`` in the shape of ``q``, or ``(o, log_normalizer)`` with the natural log-sum-exp ``[S, H]`` (``[S, H, M]``) in fp32.
     ``out``: where to write instead of a new tensor.
     """
+    call = (q, k_cache, v_cache, block_table, seq_lens, sm_scale, tensor_layout, return_log_normalizer)
+    if out is None:
+        res = _host().paged(*call)  # a call shape seen before: (o, log normalizer), or a status
+        if res is not None:
+            if type(res) is int:
+                _lib.check(res, "sage_paged_attn")
+            return res if return_log_normalizer else res[0]
     hnd = _layout(tensor_layout)
     if q.dim() not in (3, 4):
         raise ValueError("q must be (sequences, heads, head_dim) or (sequences, new tokens, heads, head_dim)")
@@ -227,6 +247,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
         ws_bytes = lib.sage_paged_attn_workspace_bytes(p)
         if ws_bytes < 0:
             _lib.check(-1, "sage_paged_attn_workspace_bytes")
+        if out is None and q is call[0] and block_table is call[3] and seq_lens is call[4]:  # (nothing was copied)
+            _host().put_paged(*call, bytes(p), ws_bytes)
         ws = split_workspace(q.device, ws_bytes) if ws_bytes else None
         _lib.check(lib.sage_paged_attn(p, ws.data_ptr() if ws is not None else None, ws_bytes, current_stream_ptr(q.device)),
                    "sage_paged_attn")
@@ -241,6 +263,10 @@ def append_to_cache(k, v, k_cache, v_cache, slots, tensor_layout="HND"):
     ``slots[t] // page_size``.  Tokens whose slot the cache does not have are left out: -1 for the rows a batch is padded with.
     The other slots of a call have to differ.
     """
+    call = (k, v, k_cache, v_cache, slots, tensor_layout)
+    status = _host().append(*call)  # a call shape seen before
+    if status is not None:
+        return _lib.check(status, "sage_cache_append")
     hnd = _layout(tensor_layout)
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError("k and v must be (tokens, heads, head_dim) tensors of the same shape")
@@ -262,6 +288,8 @@ def append_to_cache(k, v, k_cache, v_cache, slots, tensor_layout="HND"):
         p.slots, p.slots_int64 = slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0
         p.tokens, p.heads_kv, p.head_dim, p.pages, p.page_size = k.shape[0], Hk, D, pages, page_size
         p.dtype = DTYPE_CODE[k.dtype]
+        if k is call[0] and v is call[1] and slots is call[4]:  # (nothing was copied)
+            _host().put_append(*call, bytes(p))
         _lib.check(_lib.load().sage_cache_append(p, current_stream_ptr(k.device)), "sage_cache_append")
 
 
@@ -285,6 +313,10 @@ def copy_pages(k_cache, v_cache, src, dst):
     cache does not have are left out.  Pages that are written must differ from each other and from every page that is read: that is
     so where sequences split (the last page of each goes to a new one) and where pages in use move to unused ones.
     """
+    call = (k_cache, v_cache, src, dst)
+    status = _host().copy(*call)  # a call shape seen before
+    if status is not None:
+        return _lib.check(status, "sage_cache_copy_pages")
     if k_cache.dim() not in (4, 5) or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError("k_cache and v_cache must be (pages, ...) or (layers, pages, ...) tensors of the same shape and dtype")
     src, dst = _index_list(src, "src"), _index_list(dst, "dst")
@@ -311,5 +343,7 @@ def copy_pages(k_cache, v_cache, src, dst):
         setattr(p, f"{name}_stride_page", t.stride(1 if layered else 0) * e)
     p.src, p.src_int64 = src.data_ptr(), 1 if src.dtype == torch.int64 else 0
     p.dst, p.dst_int64 = dst.data_ptr(), 1 if dst.dtype == torch.int64 else 0
+    if src is call[2] and dst is call[3]:  # (nothing was copied)
+        _host().put_copy(*call, bytes(p))
     with device_guard(k_cache.device):
         _lib.check(_lib.load().sage_cache_copy_pages(p, current_stream_ptr(k_cache.device)), "sage_cache_copy_pages")

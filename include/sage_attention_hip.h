@@ -306,8 +306,8 @@ int sage_flash_varlen_fwd(const sage_varlen_params* p, void* workspace, int64_t 
  *
  *   q, out       [seqs, new_tokens, Hq, D] through stride_b (sequence), stride_n (new token) and stride_h
  *   k_cache, v_cache  [pages, ..] through stride_b (page), stride_h and stride_n (place in a page)
- *   block_table  [seqs, table_width] int32 on the device, rows table_stride entries apart; entries past a sequence's last page are not
- *                read.  The tokens of an entry that is no page of the cache (negative, or pages and more) take no part.
+ *   block_table  [seqs, table_width] int32 on the device, rows table_stride entries apart; entries past a sequence's last page have no
+ *                effect.  The tokens of an entry that is no page of the cache (negative, or pages and more) take no part.
  *   seq_lens     [seqs] int32 on the device, clamped to 0 .. table_width * page_size
  *   log_normalizer  optional [seqs, Hq, new_tokens] fp32 contiguous, natural log; NULL = none
  * The table and the lengths are read by the kernels: a captured graph follows their present values.  Zero rows, infinities and

@@ -169,40 +169,43 @@ def test_varlen_long_sequence(gpu_device):
     _check_varlen(q, k, v, cu, cu, True)
 
 
-@pytest.fixture
-def workspaces(monkeypatch):
-    """The sizes of the workspaces that calls take."""
-    from flagattention_amd import serving
+def _is_cut(q, k, seqs, causal):
+    """Whether a call of these sizes is cut into equal shares."""
+    from flagattention_amd import _lib
 
-    taken, make = [], serving.split_workspace
-    monkeypatch.setattr(serving, "split_workspace", lambda device, n: taken.append(n) or make(device, n))
-    return taken
+    p = _lib.VarlenParams()
+    for t, x in ((p.q, q), (p.k, k), (p.v, k), (p.out, q)):
+        t.ptr, t.stride_h, t.stride_n = x.data_ptr(), x.stride(1), x.stride(0)
+    p.cu_seqlens_q = p.cu_seqlens_k = 4096
+    p.seqs, p.total_q, p.total_k, p.heads_q, p.heads_kv, p.head_dim = seqs, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2]
+    p.dtype, p.causal, p.sm_scale = _lib.SAGE_BF16, int(causal), 0.1
+    return _lib.load().sage_flash_varlen_workspace_bytes(p) > 0
 
 
 @pytest.mark.parametrize("d,dtype", [(64, "fp16"), (128, "bf16")])
 @pytest.mark.parametrize("heads", [(4, 4), (8, 2), (7, 1), (3, 1), (40, 2)])
 @pytest.mark.parametrize("m,n", [((100,), (9000,)), ((40, 0, 129, 1), (5000, 7, 3003, 6000)), ((64, 70), (63, 12000)), ((3, 5, 200), (0, 8000, 150))])
-def test_varlen_cut_into_shares(m, n, heads, d, dtype, workspaces, gpu_device):
+def test_varlen_cut_into_shares(m, n, heads, d, dtype, gpu_device):
     """Few queries against many keys: blocks that several workgroups share, shares that hold several blocks, blocks that see
     nothing, sequences without keys or queries."""
     h, hk = heads
     q = _randn((sum(m), h, d), DTYPES[dtype], gpu_device, 0)
     k, v = (_randn((sum(n), hk, d), DTYPES[dtype], gpu_device, i) for i in (1, 2))
     for causal in (False, True):
+        assert _is_cut(q, k, len(m), causal)
         _check_varlen(q, k, v, _cu(m, gpu_device), _cu(n, gpu_device), causal)
-    assert len(workspaces) == 4 and min(workspaces) > 0
 
 
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
-def test_varlen_cut_with_nonfinite_values(value, workspaces, gpu_device):
+def test_varlen_cut_with_nonfinite_values(value, gpu_device):
     m, n = (70, 33), (4000, 5000)
     q = _randn((sum(m), 8, 128), torch.bfloat16, gpu_device, 0)
     k, v = (_randn((sum(n), 2, 128), torch.bfloat16, gpu_device, i) for i in (1, 2))
     v[3999, 0, 5] = value
     v[3970, 1, 100] = -value
     v[4000 + 4980, 1, 0] = value
+    assert _is_cut(q, k, 2, True)
     _check_varlen(q, k, v, _cu(m, gpu_device), _cu(n, gpu_device), True)
-    assert workspaces
 
 
 def test_varlen_agrees_with_the_rectangular_forward(gpu_device):
@@ -555,6 +558,33 @@ def test_captured_step_follows_the_present_lengths(gpu_device):
         want, want_norm, tol, norm_tol = SO.paged(q, kc, vc, table, lens)
         SO.assert_close(got[0], want, tol)
         SO.assert_close(got[1], want_norm, norm_tol)
+
+
+def test_calls_of_a_known_shape_take_the_present_arguments(gpu_device):
+    """A second call of the same sizes and strides with other tensors, the same call with other flags, and errors after it."""
+    import flag_attn
+
+    k, v, table, lens = _cache((300, 100), 2, 16, 64, torch.bfloat16, "HND", gpu_device)
+    for seed in range(3):
+        q = _randn((2, 8, 64), torch.bfloat16, gpu_device, seed)
+        lens2 = lens - 7 * seed
+        _check_paged(q, k, v, table.clone(), lens2, "HND", None if seed < 2 else 0.3)
+        p = [_randn((130, n, 64), torch.bfloat16, gpu_device, seed + i) for i, n in enumerate((4, 2, 2))]
+        cu = _cu((50 + seed, 80 - seed), gpu_device)
+        for causal in (True, False):
+            _check_varlen(*p, cu, cu, causal, None if seed < 2 else 0.3)
+        kc, vc = (_randn((5, 2, 16, 64), torch.bfloat16, gpu_device, seed + 7 + i) for i in range(2))
+        slots = torch.arange(7, device=gpu_device) + seed
+        flag_attn.append_to_cache(p[1][:7], p[2][:7], kc, vc, slots)
+        assert torch.equal(kc[0, :, seed:seed + 7].transpose(0, 1), p[1][:7]) and torch.equal(vc[0, :, seed:seed + 7].transpose(0, 1), p[2][:7])
+        flag_attn.copy_pages(kc, vc, slots[:1], slots[1:2])
+        assert torch.equal(kc[seed], kc[seed + 1]) and torch.equal(vc[seed], vc[seed + 1])
+    with pytest.raises(NotImplementedError):
+        flag_attn.flash_attention_varlen(p[0].requires_grad_(), p[1], p[2], cu)
+    with pytest.raises(ValueError):
+        flag_attn.paged_attention(q, k, v, table[:1], lens)
+    with pytest.raises(RuntimeError, match="seq_lens is on cpu"):
+        flag_attn.paged_attention(q, k, v, table, lens.cpu())
 
 
 def test_calls_on_another_stream(gpu_device):
