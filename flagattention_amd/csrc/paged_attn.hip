@@ -467,11 +467,14 @@ PagedPlan plan_paged(const sage_paged_params& p) {
     const int64_t most = 0x7fffffffLL - 4 * kChunk;
     plan.capacity = p.table_width > most / p.page_size ? most : p.table_width * p.page_size;
     plan.items = p.seqs * p.heads_kv * plan.row_tiles;
-    // What the sequences could hold at most, in chunks.  Short ones are not cut: a second launch takes as long as four to
-    // six chunks more.
+    // Equal shares, or a workgroup per item?  A workgroup needs about 1.4 us for a chunk, and a launch of items lasts as long as its
+    // longest one (chunks: what a sequence could hold at most) or as all of them over the chip; shares cost a second launch, and
+    // every item in a share a start and an end, about five chunks in all.  Measured, items and shares (bf16, D128): 1 x 32 heads, 700
+    // tokens 14.1 and 11.7 us, 8 x 8, 2000 26.6 and 20.2, 32 x 8, up to 8192 99 and 59, 16 x 32, up to 9000 239 and 192; 32 x 8, up to
+    // 700 15.7 and 19.5, 128 x 8, up to 500 36.5 and 48, 1000 x 8, up to 1500 378 and 451; D64: 128 x 16, up to 2048 111 and 119.
     const int64_t chunks = (plan.capacity + kChunk - 1) / kChunk;
     plan.shares = plan.items * chunks < kPagedShares ? plan.items * chunks : kPagedShares;
-    if (chunks <= 6 || plan.items > 0x7fffffffLL / chunks) plan.shares = 0;
+    if (chunks <= 5 + 6 * plan.items / kPagedShares || plan.items > 0x7fffffffLL / chunks) plan.shares = 0;
     return plan;
 }
 
