@@ -346,6 +346,8 @@ static int check_paged(const char* who, const sage_paged_params* p, bool& nothin
         return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30", who);
     if (misaligned_row(p->q, 2) || misaligned_row(p->out, 2) || misaligned_row(p->k_cache, 2) || misaligned_row(p->v_cache, 2))
         return fail(SAGE_E_INVALID, "%s: rows of q, out and the caches must be 16-byte aligned", who);
+    if (p->k_cache.stride_n < 0 || p->v_cache.stride_n < 0 || p->k_cache.stride_n >= (1LL << 27) || p->v_cache.stride_n >= (1LL << 27))
+        return fail(SAGE_E_UNSUPPORTED, "%s: token stride of a cache out of range for 32-bit offsets within 16 tokens", who);
     return SAGE_OK;
 }
 

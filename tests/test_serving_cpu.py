@@ -201,6 +201,17 @@ def test_paged_validation(field, value, status, message):
     assert lib.sage_paged_attn_workspace_bytes(p) == -1
 
 
+def test_paged_validation_of_rows():
+    from flagattention_amd import _lib
+
+    lib = _lib.load()
+    for name, part, value, status in (("q", "ptr", 4104, -1), ("out", "stride_b", 100, -1), ("k_cache", "stride_b", 4, -1),
+                                      ("v_cache", "stride_n", 1 << 27, -2), ("v_cache", "ptr", None, -1)):
+        p = _paged_params()
+        setattr(getattr(p, name), part, value)
+        assert lib.sage_paged_attn(p, None, 0, None) == status, (name, part)
+
+
 def test_paged_workspace():
     """Long tables share their keys out and need room for two partial results per workgroup; short ones need none."""
     from flagattention_amd import _lib

@@ -57,6 +57,20 @@ def test_varlen_more_or_fewer_keys_than_queries(m, n, d, gpu_device):
         _check_varlen(q, k, v, _cu(m, gpu_device), _cu(n, gpu_device), causal)
 
 
+@pytest.mark.parametrize("h,hk", [(160, 1), (258, 2)])
+def test_more_rows_per_token_than_a_block_holds(h, hk, gpu_device):
+    """So many query heads for one K/V head that a block, or a workgroup's rows, is less than one token."""
+    lengths = (70, 1, 9)
+    q, k, v = (_randn((sum(lengths), n, 64), torch.bfloat16, gpu_device, i) for i, n in enumerate((h, hk, hk)))
+    cu = _cu(lengths, gpu_device)
+    for causal in (False, True):
+        _check_varlen(q, k, v, cu, cu, causal)
+    for width in (None, 1500):
+        kc, vc, table, lens = _cache(lengths, hk, 16, 64, torch.bfloat16, "NHD", gpu_device, width)
+        _check_paged(q[:3], kc, vc, table, lens, "NHD")
+        _check_paged(q[:6].view(3, 2, h, 64), kc, vc, table, lens, "NHD")
+
+
 @pytest.mark.parametrize("seqs", [63, 64, 65, 300, 4097])
 def test_varlen_many_sequences(seqs, gpu_device):
     g = torch.Generator().manual_seed(seqs)
@@ -266,7 +280,7 @@ PAGED_LENGTHS = [(1,), (0, 7, 0), (31, 32, 33), (127, 128, 129, 1, 300), (1000, 
 @pytest.mark.parametrize("layout", ["HND", "NHD"])
 @pytest.mark.parametrize("d,dtype", [(64, "fp16"), (128, "bf16"), (128, "fp16"), (64, "bf16")])
 @pytest.mark.parametrize("heads", [(4, 4), (8, 2), (7, 1), (40, 1)])
-@pytest.mark.parametrize("page", [16, 1, 24, 128])
+@pytest.mark.parametrize("page", [16, 1, 24, 48, 128])
 @pytest.mark.parametrize("lengths", PAGED_LENGTHS)
 def test_paged_lengths(lengths, page, heads, d, dtype, layout, gpu_device):
     """Once with a table as wide as the sequences need (a workgroup per item) and once with a wide one (equal shares)."""
@@ -437,6 +451,17 @@ def test_copy_pages(count, page, d, layers, gpu_device):
             x[:, dst[real].to(gpu_device)] = x[:, src[real].to(gpu_device)]
         flag_attn.copy_pages(k, v, src.to(a).to(gpu_device), dst.to(b).to(gpu_device))
         assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_copy_more_pages_than_a_grid_dimension_holds(gpu_device):
+    import flag_attn
+
+    count = 70001
+    k, v = (_randn((2 * count, 1, 1, 8), torch.float16, gpu_device, i) for i in (1, 2))
+    src, dst = torch.arange(count, device=gpu_device), torch.arange(count, 2 * count, device=gpu_device).flip(0)
+    want = [torch.cat([x[:count], x[:count].flip(0)]) for x in (k, v)]
+    flag_attn.copy_pages(k, v, src, dst)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
 
 
 def test_copy_pages_of_views(gpu_device):
