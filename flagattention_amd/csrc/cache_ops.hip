@@ -86,7 +86,7 @@ int launch_cache_append(const sage_append_params& p, hipStream_t stream) {
     a.page_size = (int)p.page_size; a.heads = (int)p.heads_kv; a.row_pieces = (int)(p.head_dim * e / 16);
     a.pieces = p.tokens * a.heads * a.row_pieces;
     const int64_t wgs = (a.pieces + kThreads - 1) / kThreads;
-    if (wgs > 0x7fffffffLL) return fail(SAGE_E_UNSUPPORTED, "sage_cache_append: too many rows for one launch");
+    if (wgs > kMaxThreads / kThreads) return fail(SAGE_E_UNSUPPORTED, "sage_cache_append: too many rows for one launch");
     hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)wgs), dim3(kThreads), 0, stream, a);
     return check_launch("cache_append_kernel");
 }

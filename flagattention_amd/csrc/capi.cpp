@@ -344,6 +344,8 @@ static int check_paged(const char* who, const sage_paged_params* p, bool& nothin
     if (p->seqs >= lim || p->new_tokens >= lim || p->new_tokens * (p->heads_q / p->heads_kv) >= lim || p->pages >= lim || p->page_size >= lim ||
         p->table_width >= lim)
         return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30", who);
+    if (p->seqs * (p->new_tokens * (p->heads_q / p->heads_kv)) >= (1LL << 40))
+        return fail(SAGE_E_UNSUPPORTED, "%s: seqs x new_tokens x heads_q / heads_kv must stay below 2^40", who);
     if (misaligned_row(p->q, 2) || misaligned_row(p->out, 2) || misaligned_row(p->k_cache, 2) || misaligned_row(p->v_cache, 2))
         return fail(SAGE_E_INVALID, "%s: rows of q, out and the caches must be 16-byte aligned", who);
     if (p->k_cache.stride_n < 0 || p->v_cache.stride_n < 0 || p->k_cache.stride_n >= (1LL << 27) || p->v_cache.stride_n >= (1LL << 27))

@@ -16,6 +16,8 @@ inline int check_launch(const char* what) {
     return SAGE_OK;
 }
 
+constexpr int64_t kMaxThreads = 0xffffffffLL;  // of a launch, along x
+
 inline int dtype_bytes(int dt) { return dt == SAGE_F32 ? 4 : 2; }
 
 // Launchers implemented in the .hip files.

@@ -667,7 +667,7 @@ int launch_d(const VarlenArgs& a, int64_t blocks, hipStream_t stream) {
         hipLaunchKernelGGL((varlen_combine_kernel<D, VT>), dim3((unsigned)a.shares - 1, kVarWaves), dim3(2 * D), 0, stream, a);
         return check_launch("varlen_combine_kernel");
     }
-    if (blocks * a.Hkv > 0x7fffffffLL) return fail(SAGE_E_UNSUPPORTED, "sage_flash_varlen_fwd: too many workgroups for one launch");
+    if (blocks * a.Hkv > kMaxThreads / kVarThreads) return fail(SAGE_E_UNSUPPORTED, "sage_flash_varlen_fwd: too many workgroups for one launch");
     hipLaunchKernelGGL((flash_varlen_kernel<D, VT, false>), dim3((unsigned)(blocks * a.Hkv)), dim3(kVarThreads), 0, stream, a);
     return check_launch("flash_varlen_kernel");
 }

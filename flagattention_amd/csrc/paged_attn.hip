@@ -90,10 +90,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
     int seq, pos, end, seq_begin;  // share of the line; where the sequence begins on it
     if (a.shares == 0) {
         seq = blockIdx.x / per_seq;
-        seq_begin = 0;
-        const int c = seq_chunks(a, seq);
-        pos = blockIdx.x % per_seq * c;
-        end = pos + c;
+        seq_begin = pos = 0;
+        end = seq_chunks(a, seq);
     } else {
         const EqualShares line(line_total(a), a.shares);
         pos = line.begin(blockIdx.x);
@@ -114,7 +112,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
     while (pos < end) {
         // ---- the piece: chunks `first` .. of an item
         const int len = seq_len(a, seq), chunks = seq_chunks(a, seq);
-        const int item = (pos - seq_begin) / chunks, first = pos - seq_begin - item * chunks;
+        // (a workgroup per item: all items at once may be more than 31 bits of chunks)
+        const int item = a.shares == 0 ? blockIdx.x % per_seq : (pos - seq_begin) / chunks;
+        const int first = a.shares == 0 ? 0 : pos - seq_begin - item * chunks;
         const int hk = item / a.row_tiles, row0 = item % a.row_tiles * (16 * row_waves);
         const int n = min(chunks - first, end - pos);
         const bool whole = n == chunks;
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
         const int kbeg = first * kChunk, kend = min((first + n) * kChunk, len);
         const int oseq = seq;
         pos += n;
-        if (pos - seq_begin == chunks * per_seq) {
+        if (a.shares != 0 && pos - seq_begin == chunks * per_seq) {
             seq_begin = pos;
             seq++;
         }
@@ -488,7 +488,7 @@ int64_t paged_workspace_bytes(const sage_paged_params& p) {
 template <int D, typename VT>
 static int launch_paged(const PagedArgs& a, const PagedPlan& plan, hipStream_t stream) {
     const int64_t wgs = plan.shares ? plan.shares : plan.items;
-    if (wgs > 0x7fffffffLL || plan.items > 0x7fffffffLL) return fail(SAGE_E_UNSUPPORTED, "sage_paged_attn: too many workgroups for one launch");
+    if (wgs > kMaxThreads / kPagedThreads) return fail(SAGE_E_UNSUPPORTED, "sage_paged_attn: too many workgroups for one launch");
     const dim3 grid((unsigned)wgs), block(kPagedThreads);
     const bool page16 = a.page_size % 16 == 0;
     if (a.M > 1 && page16) hipLaunchKernelGGL((paged_attn_kernel<D, VT, true, true>), grid, block, 0, stream, a);

@@ -245,6 +245,27 @@ def test_varlen_workspace():
     assert lib.sage_flash_varlen_workspace_bytes(p) == -1
 
 
+def test_launches_too_large():
+    """Calls whose workgroups would need more than 2^32 threads are refused before any launch."""
+    from flagattention_amd import _lib
+
+    lib = _lib.load()
+    p = _varlen_params()
+    p.seqs, p.total_q, p.total_k, p.heads_kv, p.heads_q = 5, 1 << 29, 1 << 29, 32, 32
+    assert lib.sage_flash_varlen_fwd(p, None, 0, None) == -2 and b"too many workgroups" in lib.sage_hip_last_error()
+    p = _paged_params(seqs=1 << 22)
+    assert lib.sage_paged_attn_workspace_bytes(p) == 0
+    assert lib.sage_paged_attn(p, None, 0, None) == -2 and b"too many workgroups" in lib.sage_hip_last_error()
+    p.seqs, p.new_tokens = 1 << 29, 1 << 20
+    assert lib.sage_paged_attn(p, None, 0, None) == -2 and b"2^40" in lib.sage_hip_last_error()
+    p = _lib.AppendParams()
+    for t in (p.k, p.v, p.k_cache, p.v_cache):
+        t.ptr, t.stride_b, t.stride_h, t.stride_n = 4096, 1024, 64, 128
+    p.page_size, p.tokens, p.heads_kv, p.head_dim, p.pages, p.slots = 16, 1 << 29, 1 << 16, 128, 4, 4096
+    p.dtype = _lib.SAGE_BF16
+    assert lib.sage_cache_append(p, None) == -2 and b"too many rows" in lib.sage_hip_last_error()
+
+
 def test_cache_movement_validation():
     from flagattention_amd import _lib
 
