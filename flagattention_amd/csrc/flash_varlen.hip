@@ -18,9 +18,11 @@
 //   reloads per step: 4 documents of 512 to 8192 tokens, H32/8 D128, 593 -> 811 us).  What is rare is therefore kept out of its
 //   registers (careful_row).
 // * Workgroups are handed out longest first over all sequences (find_block).
-// Measured (bf16, D128, causal): those documents 593 us = 1100 TFLOP/s, one sequence of 16384 tokens with H16/2 952 us = 1155 TFLOP/s (a
-// library product of 8192^3 reaches 1356 here); 48 prompts of 1 to 700 tokens 48 us.  Tiles of 32 keys, each multiplied, weighed and
-// added in turn: 811, 1272 and 54 us.  Eight waves per workgroup: 2 % more for long sequences, 28 % less for short ones.
+// Measured (bf16, D128, causal): those documents 590 to 620 us = 1050 to 1100 TFLOP/s, one sequence of 16384 tokens with H16/2 950 to
+// 980 us = 1120 to 1155 TFLOP/s (a library product of 8192^3 reaches 1360 to 1380 here); 48 prompts of 1 to 700 tokens 41 us, of which a
+// workgroup spends 1.7 us on finding its block, 2.2 on its first tile, 1.3 on each further one and 1.4 on its output.  Tiles of 32
+// keys, each multiplied, weighed and added in turn: 811, 1272 and 54 us.  Eight waves per workgroup: 2 % more for long sequences,
+// 28 % less for short ones.
 #include <math.h>
 
 #include "serve_common.h"
@@ -41,7 +43,8 @@ struct VarlenArgs {
     const int32_t* cu_k;
     int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h, os_t, os_h;
     int32_t seqs, total_q, total_k, Hkv, groups, causal;
-    float qk_scale;  // sm_scale * log2(e)
+    float qk_scale;       // sm_scale * log2(e)
+    uint32_t inv_groups;  // 2^16 / groups, rounded down, + 1
     // Cut launch: workgroups that share all steps evenly, tokens of a block (a power of two; log2), partial results.
     int32_t shares, tokens_shift;
     float* part_o;    // [2 * shares][4 waves][D / 32][4][64 lanes][4]: normalized outputs in the order of the accumulator registers
@@ -82,12 +85,13 @@ __device__ __forceinline__ bool find_block(const VarlenArgs& a, int at, int& q0,
     sequence(a.cu_q, min(lane, a.seqs - 1), a.total_q, lq0, lm);
     sequence(a.cu_k, min(lane, a.seqs - 1), a.total_k, lk0, ln);
     if (lane >= a.seqs) lm = 0;
-    const int nb = blocks(lm), rows = lm * a.groups;
+    const int nb = blocks(lm);
     // blocks below `first_of(l)` visit fewer than l key tiles
     auto first_of = [&](int l) {
-        if (!a.causal) return kVarKeys * (l - 1) < ln ? 0 : nb;
-        const int64_t x = ((int64_t)kVarKeys * (l - 1) - (ln - lm)) * a.groups;  // the first row that sees a key of tile l - 1
-        return x >= rows ? nb : x <= 0 ? 0 : (int)(x / kVarRows);
+        const int before = kVarKeys * (l - 1) - ln;  // keys
+        if (!a.causal) return before < 0 ? 0 : nb;
+        const int first = min(max(before, -lm), 0) + lm;  // the first query that sees a key of tile l - 1
+        return first == lm ? nb : first * a.groups / kVarRows;
     };
     if (at >= wave_sum(nb)) return false;
     int low = 0, high = wave_max(ln) / kVarKeys + 2;  // the largest level l with more than `at` blocks of l tiles and more: low <= l < high
@@ -269,9 +273,14 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
         N -= first_tile * kVarKeys;
     }
     const int shift = N - M;
-    const int row = row0 + 32 * wave + l32;
-    const bool row_ok = row < rows;
-    const int my_m = min(row, rows - 1) / a.groups, my_h = hk * a.groups + min(row, rows - 1) % a.groups;
+    // Row row0 + r is head rem0 + r - groups * j of token tok0 + j, j = tokens_on(r): r < 128, so that products of 16 bits divide it
+    // exactly (n inv_groups = 2^16 n / groups + less than n, and n < 256 here) or, for larger groups, a comparison.
+    const int tok0 = CUT ? block << a.tokens_shift : row0 / a.groups, rem0 = row0 - tok0 * a.groups;
+    auto tokens_on = [&](int r) { return a.groups < kVarRows ? (int)((unsigned)(rem0 + r) * a.inv_groups >> 16) : rem0 + r >= a.groups ? 1 : 0; };
+    const int my_row = 32 * wave + l32, last_row = rows - 1 - row0;
+    const bool row_ok = my_row <= last_row;
+    const int my_on = tokens_on(min(my_row, last_row));
+    const int my_m = tok0 + my_on, my_h = hk * a.groups + rem0 + min(my_row, last_row) - my_on * a.groups;
 
     // Q rows as the B operand: lane (row l32, half) holds elements 16 t + 8 half .. + 7 of its row for step t
     vec16 qf[KS];
@@ -286,15 +295,16 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     // keys that any row of the workgroup / of this wave can see, and those that every row of the wave sees
     int n_end = N, wave_end = N, all_see = N;
     if (a.causal) {
-        n_end = max(min(N, (min(row0 + block_rows, rows) - 1) / a.groups + 1 + shift), 0);
-        wave_end = max(min(N, (min(row0 + 32 * wave + 32, rows) - 1) / a.groups + 1 + shift), 0);
-        all_see = max(min(N, min(row0 + 32 * wave, rows - 1) / a.groups + 1 + shift), 0);
+        auto sees = [&](int r) { return max(min(N, tok0 + tokens_on(min(r, last_row)) + 1 + shift), 0); };  // keys that row row0 + r sees
+        n_end = sees(block_rows - 1);
+        wave_end = sees(32 * wave + 31);
+        all_see = sees(32 * wave);
     }
     const int my_lim = a.causal ? min(my_m + shift, N - 1) : N - 1;  // last key this lane's row sees
     int ntiles = (n_end + kVarKeys - 1) / kVarKeys;
     if (CUT) ntiles = min(ntiles, cut_tiles);
     // tiles that this wave multiplies with, and how many of them, the first ones, hide no key
-    const int my_tiles = row0 + 32 * wave < rows ? min((wave_end + kVarKeys - 1) / kVarKeys, ntiles) : 0;
+    const int my_tiles = 32 * wave <= last_row ? min((wave_end + kVarKeys - 1) / kVarKeys, ntiles) : 0;
     const int clear_tiles = min(all_see / kVarKeys, my_tiles);
 
     // Tile t of K and V -> one of the two buffers, straight into LDS (written in assembly, as in attn_fast_kernel.h: the compiler
@@ -376,7 +386,7 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     // to 1, their rounding is relative, and most steps then multiply no accumulator (5 % of the documents' time).  A row's point depends on its own scores alone.
     auto raise = [&](float top) {
         if (__builtin_amdgcn_ballot_w64(top > m_i + kLag) != 0) {
-            top = fmaxf(top, __shfl_xor(top, 32));  // (two lanes share a row)
+            top = fmaxf(top, __shfl_xor(top, 32));
             const float m_new = top > m_i + kLag ? top : m_i;
             // (a row that has seen no key yet keeps m = -inf: every p below is then 0)
             const float alpha = m_i == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_i - m_new);
@@ -419,23 +429,6 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
 #pragma unroll
         for (int c = 0; c < 2 * KT; c++) add_slice(t, c, pf[c]);
     };
-    // An infinity or NaN in V under a hidden key must not reach the rows that do not see it (0 times it is NaN): where a tile that
-    // hides keys holds one, the wave's rows are computed again at the end, key by key.
-    bool again = false;
-    auto look = [&](int t) {
-        unsigned odd = 0;
-#pragma unroll
-        for (int c = 0; c < 2 * KT; c++)
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                const v4i f = v_fragment(t, c, dt);
-#pragma unroll
-                for (int i = 0; i < 4; i++) odd |= nonfinite_halves<VT>((unsigned)f[i]);
-                if (dt % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // (two fragments at a time: registers)
-            }
-        again |= __builtin_amdgcn_ballot_w64(odd != 0) != 0;
-    };
-
     // ---- K of tile t + 1 and V of tile t are in LDS, or on their way, when step t begins; the step fetches K of t + 2 and V of t + 1
     if (ntiles > 0) {
         fetch_k(IC<0>{}, 0);
@@ -467,15 +460,15 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     // A step that hides no key, nor does the next: the scores of the next tile are made while this one's exponentials are.
     auto clear_step = [&](int t, v16f (&cur)[KT], v16f (&nxt)[KT]) {
         vec16 pf[2 * KT];
-        // (in three parts, so that no more than three of the four 32-key score tiles are in registers at a time)
+        // (in two parts, so that no more than three of the four 32-key score tiles are in registers at a time: without the barrier one
+        // sequence of 2000 tokens takes 4 % longer)
         half_scores(t + 1, 0, nxt[0]);
         half_weights(cur[0], pf[0], pf[1]);
         __builtin_amdgcn_sched_barrier(0);
-        half_scores(t + 1, 1, nxt[1]);
         half_weights(cur[1], pf[2], pf[3]);
+        half_scores(t + 1, 1, nxt[1]);
         add_slice(t, 0, pf[0]);
         add_slice(t, 1, pf[1]);
-        __builtin_amdgcn_sched_barrier(0);
         add_slice(t, 2, pf[2]);
         add_slice(t, 3, pf[3]);
         raise(largest(nxt));
@@ -492,7 +485,6 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
         if (t >= my_tiles) continue;
         vec16 pf[2 * KT];
         weights(sa, pf);
-        if (t >= clear_tiles) look(t);
         add(t, pf);
         if (t + 1 < my_tiles) {
             scores(t + 1, sa);
@@ -505,12 +497,32 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     // accumulator i of tile dt: channel 32 dt + 8 (i / 4) + 4 half + i % 4
     float* part_o = whole ? nullptr : a.part_o + ((int64_t)slot * kVarWaves + wave) * (32 * D);
     float* part_lse = whole ? nullptr : a.part_lse + (int64_t)slot * kVarRows + 32 * wave;
-    if (__builtin_expect(again, 0)) {
-        for (int r = 0; r < 32 && row0 + 32 * wave + r < rows; r++) {
-            const int m = (row0 + 32 * wave + r) / a.groups, n = a.causal ? min(m + shift, N - 1) + 1 : N;
-            careful_row<D, VT>(a, q0 + m, hk * a.groups + (row0 + 32 * wave + r) % a.groups, hk, k0, CUT ? min(n, kVarKeys * ntiles) : n, part_o, part_lse, r);
+    // An infinity or NaN in V under a hidden key must not reach the rows that do not see it (0 times it is NaN): where an output is not
+    // finite and a tile that hides keys holds one, the wave's rows are computed again, key by key.  (Looking at those tiles inside the
+    // loop: 48 prompts of 1 to 700 tokens, H32/8 D128, 43.5 us instead of 42.1.)
+    if (clear_tiles < my_tiles) {
+        float zero[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) zero[i & 1] = __builtin_fmaf(acc[dt][i], 0.0f, zero[i & 1]);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(zero[0] + zero[1] != 0.0f) != 0, 0)) {
+            unsigned odd = 0;
+            const int first = kVarKeys * clear_tiles, pieces = (min(kVarKeys * my_tiles, N) - first) * CPR;
+#pragma unroll 1
+            for (int i = lane; i < pieces; i += 64) {
+                const v4i f = *reinterpret_cast<const v4i*>(vbase + (int64_t)(first + i / CPR) * a.vs_t + 8 * (i % CPR));
+#pragma unroll
+                for (int w = 0; w < 4; w++) odd |= nonfinite_halves<VT>((unsigned)f[w]);
+            }
+            if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
+                for (int r = 32 * wave; r < 32 * wave + 32 && r <= last_row; r++) {
+                    const int on = tokens_on(r), m = tok0 + on, n = a.causal ? min(m + shift, N - 1) + 1 : N;
+                    careful_row<D, VT>(a, q0 + m, hk * a.groups + rem0 + r - on * a.groups, hk, k0, CUT ? min(n, kVarKeys * ntiles) : n, part_o, part_lse, r - 32 * wave);
+                }
+                continue;
+            }
         }
-        continue;
     }
     const float l_tot = l_i + __shfl_xor(l_i, 32);
     // l = 0: a row that saw no key: zero row.  (NaN stays.)
@@ -537,7 +549,7 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
             if (a.lse && half == 0) a.lse[(int64_t)my_h * a.total_q + q0 + my_m] = lse2 * 0.693147180559945309f;
         }
     } else {
-        // rows of 256 bytes through LDS, so that sixteen lanes store a whole one (48 prompts of 1 to 700 tokens, H32/8: 48.4 -> 43.5 us;
+        // rows of 256 bytes through LDS, so that sixteen lanes store a whole one (48 prompts of 1 to 700 tokens, H32/8: 11 % less time;
         // at head_dim 64 the stores of 8 bytes from the registers are as fast, 19.6 and 20.6 us with H16)
         constexpr int O_RS = 2 * D + 16;
         unsigned char* mine = &smem[0][0][0] + wave * 32 * O_RS;
@@ -551,12 +563,11 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
         if (a.lse && half == 0 && row_ok) a.lse[(int64_t)my_h * a.total_q + q0 + my_m] = lse2 * 0.693147180559945309f;
 #pragma unroll
         for (int e = 0; e < 32 * CPR / 64; e++) {
-            const int r = (64 / CPR) * e + lane / CPR, at = row0 + 32 * wave + r;
+            const int r = (64 / CPR) * e + lane / CPR, on = tokens_on(32 * wave + r);
             const v4i x = *reinterpret_cast<const v4i*>(mine + r * O_RS + 16 * (lane % CPR));
-            if (at < rows) {
-                const int m = at / a.groups;
-                *reinterpret_cast<v4i*>(static_cast<VT*>(a.out) + (int64_t)(q0 + m) * a.os_t + (int64_t)(hk * a.groups + at - m * a.groups) * a.os_h + 8 * (lane % CPR)) = x;
-            }
+            if (32 * wave + r <= last_row)
+                *reinterpret_cast<v4i*>(static_cast<VT*>(a.out) + (int64_t)(q0 + tok0 + on) * a.os_t +
+                                        (int64_t)(hk * a.groups + rem0 + 32 * wave + r - on * a.groups) * a.os_h + 8 * (lane % CPR)) = x;
         }
     }
   }
@@ -688,6 +699,7 @@ int launch_flash_varlen(const sage_varlen_params& p, void* workspace, int64_t wo
     a.seqs = (int)p.seqs; a.total_q = (int)p.total_q; a.total_k = (int)p.total_k;
     a.Hkv = (int)p.heads_kv; a.groups = (int)(p.heads_q / p.heads_kv); a.causal = p.causal ? 1 : 0;
     a.qk_scale = p.sm_scale * 1.44269504089f;
+    a.inv_groups = (1u << 16) / a.groups + 1;
     a.shares = plan.shares; a.tokens_shift = plan.tokens_shift;
     a.part_o = (float*)workspace;
     a.part_lse = a.part_o + 2LL * plan.shares * kVarRows * p.head_dim;
