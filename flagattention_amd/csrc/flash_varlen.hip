@@ -10,19 +10,18 @@
 // as large as total_q and the number of sequences allow, and a workgroup finds its sequence by itself (find_run).
 //
 // S^T = K.Q^T and O^T += V^T.P^T on v_mfma_f32_32x32x16: a lane owns one row, and P goes from the accumulators to the operand
-// without leaving its registers.  Bound by the matrix cores, with the vector instructions of the softmax in their shadow:
-// * K and V tiles of 64 keys go straight into LDS for the four waves, two of each resident, one barrier per step.  Two workgroups
-//   share a compute unit and are not tied to each other, so one's exponentials meet the other's matrix instructions.
-// * A step makes the scores of the next tile while it takes the exponentials of its own.
-// * Nothing of the step loop is spilled: a reload waits for every tile on its way into LDS, since loads return in order (three
-//   reloads per step: 4 documents of 512 to 8192 tokens, H32/8 D128, 593 -> 811 us).  What is rare is therefore kept out of its
-//   registers (careful_row).
-// * Workgroups are handed out longest first over all sequences (find_block).
-// Measured (bf16, D128, causal): those documents 590 to 620 us = 1050 to 1100 TFLOP/s, one sequence of 16384 tokens with H16/2 950 to
-// 980 us = 1120 to 1155 TFLOP/s (a library product of 8192^3 reaches 1360 to 1380 here); 48 prompts of 1 to 700 tokens 41 us, of which a
-// workgroup spends 1.7 us on finding its block, 2.2 on its first tile, 1.3 on each further one and 1.4 on its output.  Tiles of 32
-// keys, each multiplied, weighed and added in turn: 811, 1272 and 54 us.  Eight waves per workgroup: 2 % more for long sequences,
-// 28 % less for short ones.
+// without leaving its registers.  K and V tiles go straight into LDS for the four waves, two of each resident, one barrier per
+// step.  Bound by the matrix cores, with the vector instructions of the softmax in their shadow, in two forms (launch_d):
+// * Many blocks: tiles of 32 keys, 168 registers, three workgroups on a compute unit.  They are not tied to each other, so that one's
+//   exponentials, barriers, search for a block, first tile and output meet the others' matrix instructions.
+// * Few: tiles of 64 keys, two workgroups on a compute unit.  A step makes the scores of the next tile while it takes the exponentials
+//   of its own.
+// Nothing of the step loop is spilled: a reload waits for every tile on its way into LDS, since loads return in order (three reloads
+// per step: 4 documents of 512 to 8192 tokens, H32/8 D128, 593 -> 811 us).  What is rare is therefore kept out of its registers
+// (careful_row).  Workgroups are handed out longest first over all sequences (find_block).
+// Measured (bf16, D128, causal; a library product of 8192^3 reaches 1360 to 1380 TFLOP/s here): those documents 590 us = 1105 TFLOP/s,
+// one sequence of 16384 tokens with H16/2 960 us = 1145, 48 prompts of 1 to 700 tokens 38 us, 200 of 100 to 200 142 us = 4.2 TB/s.
+// There a workgroup spends 1.7 us on finding its block, 2.2 on its first tile, 1.3 on every further 64 keys and 1.4 on its output.
 #include <math.h>
 
 #include "serve_common.h"
@@ -213,8 +212,9 @@ __device__ void careful_row(const VarlenArgs& a, int qt, int h, int hk, int k0, 
 }
 
 // CUT: a workgroup takes an equal share of the launch's steps instead of a block: the end of one, whole ones, the beginning of another.
-template <int D, typename VT, bool CUT>
-__global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs args) {
+// KEYS: of a tile, 64 or 32.
+template <int D, typename VT, bool CUT, int KEYS>
+__global__ __launch_bounds__(kVarThreads, KEYS == 64 ? 2 : 3) void flash_varlen_kernel(VarlenArgs args) {
     const VarlenArgs& a0 = args;
     using PVT = PV<VT>;
     using vec16 = typename PVT::vec;
@@ -222,11 +222,15 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     constexpr int DT = D / 32;      // 32-channel tiles of the output
     constexpr int RS = 2 * D;       // bytes per K / V row
     constexpr int CPR = RS / 16;    // 16-byte chunks per row
-    constexpr int TILE = kVarKeys * RS;
+    constexpr int TILE = KEYS * RS;
     constexpr int LOADS = TILE / 1024 / kVarWaves;  // 1 KB loads per wave of a K (of a V) tile
-    constexpr int KT = kVarKeys / 32;
-    static_assert(KT == 2, "halves of a tile");
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2][2][TILE];  // [K, V][buffer]
+    constexpr int KT = KEYS / 32;
+    static_assert(KT == 1 || KT == 2, "one or two halves");
+    constexpr int UNIT = kVarKeys / KEYS;  // tiles in a step of the line
+    constexpr int O_RS = 2 * D + 16;  // of an output row on its way through LDS
+    constexpr int OUT = D == 128 ? 32 * kVarWaves * O_RS : 0;
+    __shared__ __attribute__((aligned(16))) unsigned char all_smem[4 * TILE > OUT ? 4 * TILE : OUT];
+    auto smem = reinterpret_cast<unsigned char(*)[2][TILE]>(all_smem);  // [K, V][buffer]
 
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -301,11 +305,11 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
         all_see = sees(32 * wave);
     }
     const int my_lim = a.causal ? min(my_m + shift, N - 1) : N - 1;  // last key this lane's row sees
-    int ntiles = (n_end + kVarKeys - 1) / kVarKeys;
-    if (CUT) ntiles = min(ntiles, cut_tiles);
+    int ntiles = (n_end + KEYS - 1) / KEYS;
+    if (CUT) ntiles = min(ntiles, UNIT * cut_tiles);
     // tiles that this wave multiplies with, and how many of them, the first ones, hide no key
-    const int my_tiles = 32 * wave <= last_row ? min((wave_end + kVarKeys - 1) / kVarKeys, ntiles) : 0;
-    const int clear_tiles = min(all_see / kVarKeys, my_tiles);
+    const int my_tiles = 32 * wave <= last_row ? min((wave_end + KEYS - 1) / KEYS, ntiles) : 0;
+    const int clear_tiles = min(all_see / KEYS, my_tiles);
 
     // Tile t of K and V -> one of the two buffers, straight into LDS (written in assembly, as in attn_fast_kernel.h: the compiler
     // would wait for every outstanding load before each LDS read; m0 holds the LDS address and nothing else here uses it).
@@ -313,15 +317,15 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     // belongs where a lane writes, the fragment reads spread over all banks.  Load e of a wave: kRound rows further on, a whole
     // number of swizzle periods.  Rows past the end re-read the last one.
     constexpr int kRound = kVarWaves * 64 / CPR;
-    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)&smem[0][0][0];
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)all_smem;
     const int frow = (64 / CPR) * wave + lane / CPR;  // row of load 0
     const unsigned kchunk = 16 * ((lane % CPR) ^ (frow & (CPR - 1))), vchunk = 16 * ((lane % CPR) ^ var_v_swizzle<D>(frow));
     const unsigned koff = (unsigned)frow * (unsigned)(a.ks_t * 2) + kchunk, voff = (unsigned)frow * (unsigned)(a.vs_t * 2) + vchunk;
     auto fetch = [&](auto whole, const VT* base, int64_t stride, unsigned off, unsigned chunk, int t, unsigned dst) {
-        const int n0 = kVarKeys * t;
+        const int n0 = KEYS * t;
         const VT* tile = base + (int64_t)n0 * stride;
         const unsigned to = lds0 + dst + 1024 * wave;
-        if (decltype(whole)::value || n0 + kVarKeys <= N) {
+        if (decltype(whole)::value || n0 + KEYS <= N) {
 #pragma unroll
             for (int e = 0; e < LOADS; e++)
                 asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(tile + e * kRound * stride),
@@ -369,7 +373,7 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     auto hide = [&](int t, v16f (&s)[KT]) {
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
-            const int last = my_lim - kVarKeys * t - 32 * kt - 4 * half;
+            const int last = my_lim - KEYS * t - 32 * kt - 4 * half;
 #pragma unroll
             for (int i = 0; i < 16; i++) s[kt][i] = 8 * (i >> 2) + (i & 3) <= last ? s[kt][i] : -INFINITY;
         }
@@ -451,34 +455,54 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
         if (decltype(whole)::value || t + 2 < ntiles) fetch_k(whole, t + 2);
         if (decltype(whole)::value || t + 1 < ntiles) fetch_v(whole, t + 1);
     };
-    v16f sa[KT], sb[KT];
+    v16f sa[KT];
     if (my_tiles > 0) {
         scores(0, sa);
         if (clear_tiles < 1) hide(0, sa);
         raise(largest(sa));
     }
-    // A step that hides no key, nor does the next: the scores of the next tile are made while this one's exponentials are.
-    auto clear_step = [&](int t, v16f (&cur)[KT], v16f (&nxt)[KT]) {
-        vec16 pf[2 * KT];
-        // (in two parts, so that no more than three of the four 32-key score tiles are in registers at a time: without the barrier one
-        // sequence of 2000 tokens takes 4 % longer)
-        half_scores(t + 1, 0, nxt[0]);
-        half_weights(cur[0], pf[0], pf[1]);
-        __builtin_amdgcn_sched_barrier(0);
-        half_weights(cur[1], pf[2], pf[3]);
-        half_scores(t + 1, 1, nxt[1]);
-        add_slice(t, 0, pf[0]);
-        add_slice(t, 1, pf[1]);
-        add_slice(t, 2, pf[2]);
-        add_slice(t, 3, pf[3]);
-        raise(largest(nxt));
-    };
     int t = 0;
-    for (; t + 3 < clear_tiles; t += 2) {
-        next(IC<1>{}, t);
-        clear_step(t, sa, sb);
-        next(IC<1>{}, t + 1);
-        clear_step(t + 1, sb, sa);
+    if constexpr (KT == 2) {
+        v16f sb[KT];
+        // A step that hides no key, nor does the next: the scores of the next tile are made while this one's exponentials are.
+        auto clear_step = [&](int t, v16f (&cur)[KT], v16f (&nxt)[KT]) {
+            vec16 pf[2 * KT];
+            // (in two parts, so that no more than three of the four 32-key score tiles are in registers at a time: without the barrier one
+            // sequence of 2000 tokens takes 4 % longer)
+            half_scores(t + 1, 0, nxt[0]);
+            half_weights(cur[0], pf[0], pf[1]);
+            __builtin_amdgcn_sched_barrier(0);
+            half_weights(cur[1], pf[2], pf[3]);
+            half_scores(t + 1, 1, nxt[1]);
+            add_slice(t, 0, pf[0]);
+            add_slice(t, 1, pf[1]);
+            add_slice(t, 2, pf[2]);
+            add_slice(t, 3, pf[3]);
+            raise(largest(nxt));
+        };
+        for (; t + 3 < clear_tiles; t += 2) {
+            next(IC<1>{}, t);
+            clear_step(t, sa, sb);
+            next(IC<1>{}, t + 1);
+            clear_step(t + 1, sb, sa);
+        }
+    }
+    if constexpr (KT == 1) {
+        // (the matrix instructions one after the other, so that the maximum of the next scores is taken while V is added)
+        auto short_step = [&](int t) {
+            vec16 pf[2];
+            half_weights(sa[0], pf[0], pf[1]);
+            half_scores(t + 1, 0, sa[0]);
+            add_slice(t, 0, pf[0]);
+            add_slice(t, 1, pf[1]);
+            raise(largest(sa));
+        };
+        for (; t + 3 < clear_tiles; t += 2) {
+            next(IC<1>{}, t);
+            short_step(t);
+            next(IC<1>{}, t + 1);
+            short_step(t + 1);
+        }
     }
     for (; t < ntiles; t++) {
         next(IC<0>{}, t);
@@ -508,7 +532,7 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
             for (int i = 0; i < 16; i++) zero[i & 1] = __builtin_fmaf(acc[dt][i], 0.0f, zero[i & 1]);
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(zero[0] + zero[1] != 0.0f) != 0, 0)) {
             unsigned odd = 0;
-            const int first = kVarKeys * clear_tiles, pieces = (min(kVarKeys * my_tiles, N) - first) * CPR;
+            const int first = KEYS * clear_tiles, pieces = (min(KEYS * my_tiles, N) - first) * CPR;
 #pragma unroll 1
             for (int i = lane; i < pieces; i += 64) {
                 const v4i f = *reinterpret_cast<const v4i*>(vbase + (int64_t)(first + i / CPR) * a.vs_t + 8 * (i % CPR));
@@ -518,7 +542,7 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
             if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
                 for (int r = 32 * wave; r < 32 * wave + 32 && r <= last_row; r++) {
                     const int on = tokens_on(r), m = tok0 + on, n = a.causal ? min(m + shift, N - 1) + 1 : N;
-                    careful_row<D, VT>(a, q0 + m, hk * a.groups + rem0 + r - on * a.groups, hk, k0, CUT ? min(n, kVarKeys * ntiles) : n, part_o, part_lse, r - 32 * wave);
+                    careful_row<D, VT>(a, q0 + m, hk * a.groups + rem0 + r - on * a.groups, hk, k0, CUT ? min(n, KEYS * ntiles) : n, part_o, part_lse, r - 32 * wave);
                 }
                 continue;
             }
@@ -551,9 +575,7 @@ __global__ __launch_bounds__(kVarThreads, 2) void flash_varlen_kernel(VarlenArgs
     } else {
         // rows of 256 bytes through LDS, so that sixteen lanes store a whole one (48 prompts of 1 to 700 tokens, H32/8: 11 % less time;
         // at head_dim 64 the stores of 8 bytes from the registers are as fast, 19.6 and 20.6 us with H16)
-        constexpr int O_RS = 2 * D + 16;
-        unsigned char* mine = &smem[0][0][0] + wave * 32 * O_RS;
-        static_assert(kVarWaves * 32 * O_RS <= sizeof(smem), "the output rows fit the tiles");
+        unsigned char* mine = all_smem + wave * 32 * O_RS;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -670,16 +692,26 @@ VarlenPlan plan_varlen(const sage_varlen_params& p, bool with_workspace) {
     return plan;
 }
 
+// Tiles of 32 keys where blocks are many, of 64 where they are few: a workgroup by itself is slower with the former, but three of them
+// share a compute unit instead of two.  Measured, 64 and 32 (H32/8 D128, causal): 1 x 500 tokens 15.4 and 17.0 us, 1 x 3000 80 and 88,
+// 24 x 1 to 700 (860 workgroups) 24.4 and 26.0, 1 x 3500 (880) 107 and 109; 1 x 4000 (1010) 138 and 131, 32 x 1 to 700 (1150) 31.7 and 27.4,
+// 16 x 100 to 2000 139 and 125, 200 x 100 to 200 166 and 142, the documents 626 and 589; H16 D64: 1 x 700 12.3 and 13.0,
+// 2 x 3000 (780) 52.7 and 53.6, 4 x 4096 176 and 170, 48 x 1 to 700 20.4 and 18.6.
+constexpr int64_t kManyBlocks = 1000;
+
 template <int D, typename VT>
 int launch_d(const VarlenArgs& a, int64_t blocks, hipStream_t stream) {
     if (a.shares) {
-        hipLaunchKernelGGL((flash_varlen_kernel<D, VT, true>), dim3((unsigned)a.shares), dim3(kVarThreads), 0, stream, a);
+        hipLaunchKernelGGL((flash_varlen_kernel<D, VT, true, 64>), dim3((unsigned)a.shares), dim3(kVarThreads), 0, stream, a);
         if (int rc = check_launch("flash_varlen_kernel")) return rc;
         hipLaunchKernelGGL((varlen_combine_kernel<D, VT>), dim3((unsigned)a.shares - 1, kVarWaves), dim3(2 * D), 0, stream, a);
         return check_launch("varlen_combine_kernel");
     }
     if (blocks * a.Hkv > kMaxThreads / kVarThreads) return fail(SAGE_E_UNSUPPORTED, "sage_flash_varlen_fwd: too many workgroups for one launch");
-    hipLaunchKernelGGL((flash_varlen_kernel<D, VT, false>), dim3((unsigned)(blocks * a.Hkv)), dim3(kVarThreads), 0, stream, a);
+    if (blocks * a.Hkv > kManyBlocks)
+        hipLaunchKernelGGL((flash_varlen_kernel<D, VT, false, 32>), dim3((unsigned)(blocks * a.Hkv)), dim3(kVarThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((flash_varlen_kernel<D, VT, false, 64>), dim3((unsigned)(blocks * a.Hkv)), dim3(kVarThreads), 0, stream, a);
     return check_launch("flash_varlen_kernel");
 }
 

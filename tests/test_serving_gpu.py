@@ -222,6 +222,76 @@ def test_varlen_cut_with_nonfinite_values(value, gpu_device):
     _check_varlen(q, k, v, _cu(m, gpu_device), _cu(n, gpu_device), True)
 
 
+def _among_many(lengths, seqs=60):
+    """The lengths with empty sequences before, between and behind them, `seqs` in all: with 17 K/V heads or more they count as
+    enough blocks to run in tiles of 32 keys."""
+    gaps, out = seqs - len(lengths), []
+    for i, n in enumerate(lengths):
+        out += [0] * (gaps * (i + 1) // (len(lengths) + 1) - gaps * i // (len(lengths) + 1)) + [n]
+    return tuple(out + [0] * (seqs - len(out)))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads", [(17, 17), (40, 20), (119, 17)])
+@pytest.mark.parametrize("lengths", [(1,), (0, 5, 0, 2), (31, 32, 33, 64, 65), (127, 128, 129, 1), (300, 1, 511), (161,)])
+def test_varlen_many_blocks(lengths, heads, d, dtype, gpu_device):
+    (h, hk), t, dt = heads, sum(lengths), DTYPES[dtype]
+    q, k, v = (_randn((t, n, d), dt, gpu_device, i) for i, n in enumerate((h, hk, hk)))
+    for seqs in (60, 70):  # (in the order of their lengths, in their own order)
+        cu = _cu(_among_many(lengths, seqs), gpu_device)
+        for causal in (False, True):
+            _check_varlen(q, k, v, cu, cu, causal)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("m,n", [((3, 70, 1), (200, 70, 600)), ((5, 100, 40), (0, 33, 7)), ((64, 0, 9), (1, 50, 8)), ((130,), (700,))])
+def test_varlen_many_blocks_of_chunks(m, n, d, gpu_device):
+    q = _randn((sum(m), 40, d), torch.bfloat16, gpu_device, 0)
+    k, v = (_randn((sum(n), 20, d), torch.bfloat16, gpu_device, i) for i in (1, 2))
+    for causal in (False, True):
+        _check_varlen(q, k, v, _cu(_among_many(m), gpu_device), _cu(_among_many(n), gpu_device), causal)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "fp16"), (128, "bf16"), (128, "fp16")])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_varlen_many_blocks_with_nonfinite_values(value, d, dtype, gpu_device):
+    lengths = (70, 45, 200)
+    q, k, v = (_randn((sum(lengths), n, d), DTYPES[dtype], gpu_device, i) for i, n in enumerate((34, 17, 17)))
+    v[69, 0, 5] = value
+    v[70 + 33, 1, d - 1] = value
+    v[115 + 31, 0, 0] = value
+    v[115 + 130, 16, 33] = -value
+    v[115 + 190, 3] = value
+    cu = _cu(_among_many(lengths), gpu_device)
+    for causal in (True, False):
+        _check_varlen(q, k, v, cu, cu, causal)
+
+
+def test_varlen_many_blocks_leave_other_rows_alone(gpu_device):
+    """NaN in a query or a key of the future, slices of one projection, rows behind the last sequence."""
+    import flag_attn
+
+    lengths, h, hk, d = (100, 1, 260), 34, 17, 128
+    t = sum(lengths)
+    qkv = _randn((t + 13, h + 2 * hk, d), torch.bfloat16, gpu_device, 0)
+    qkv[t:] = float("nan")
+    q, k, v = qkv.split([h, hk, hk], dim=1)
+    cu = _cu(_among_many(lengths), gpu_device)
+    out = torch.full((t + 13, 2 * h, d), 3.0, dtype=torch.bfloat16, device=gpu_device)
+    for causal in (False, True):
+        flag_attn.flash_attention_varlen(q, k, v, cu, causal=causal, out=out[:, ::2])
+        want, _, tol, _ = SO.varlen(q[:t], k[:t], v[:t], cu, cu, causal)
+        SO.assert_close(out[:t, ::2], want, tol)
+        assert (out[t:] == 3.0).all() and (out[:, 1::2] == 3.0).all()
+    clean = flag_attn.flash_attention_varlen(q, k, v, cu, causal=True)
+    q[50, 3], k[99, 5], k[101 + 200] = float("nan"), float("nan"), float("inf")
+    o = flag_attn.flash_attention_varlen(q, k, v, cu, causal=True)
+    same = torch.ones(t, h, dtype=torch.bool, device=gpu_device)
+    same[50, 3], same[99, 10:12], same[301:] = False, False, False
+    assert torch.equal(o[:t][same], clean[:t][same]) and o[50, 3].isnan().all() and o[99, 10:12].isnan().all()
+
+
 def test_varlen_agrees_with_the_rectangular_forward(gpu_device):
     """Sequences of one length are a batch: the same answers as flash_attention, to the rounding of P and of the output."""
     import flag_attn
