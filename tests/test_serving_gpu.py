@@ -292,6 +292,17 @@ def test_varlen_many_blocks_leave_other_rows_alone(gpu_device):
     assert torch.equal(o[:t][same], clean[:t][same]) and o[50, 3].isnan().all() and o[99, 10:12].isnan().all()
 
 
+@pytest.mark.parametrize("group", [3, 5, 11, 33, 63, 65, 100, 127, 128, 129])
+def test_varlen_group_sizes(group, gpu_device):
+    """Rows of a block are (query, head) pairs: blocks that begin inside a query, groups around the rows of a block."""
+    lengths = (9, 40, 1)
+    for hk, seqs in ((1, 3), (17, 60)):  # (few blocks, many)
+        q, k, v = (_randn((sum(lengths), n, 64), torch.bfloat16, gpu_device, i) for i, n in enumerate((group * hk, hk, hk)))
+        cu = _cu(_among_many(lengths, seqs), gpu_device)
+        for causal in (False, True):
+            _check_varlen(q, k, v, cu, cu, causal)
+
+
 def test_varlen_agrees_with_the_rectangular_forward(gpu_device):
     """Sequences of one length are a batch: the same answers as flash_attention, to the rounding of P and of the output."""
     import flag_attn
