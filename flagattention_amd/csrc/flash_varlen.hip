@@ -61,13 +61,22 @@ __device__ __forceinline__ void sequence(const int32_t* cu, int s, int total, in
     len = min(max(cu[s + 1], begin), total) - begin;
 }
 
+constexpr unsigned kOrderless = 256;  // workgroups that have a compute unit each: the order in which they start is of no matter
+
 // The block of 128 rows that workgroup `at` (of a K/V head) takes, and its sequence; false: there is none.
 // Up to 64 sequences, a lane each: the blocks that see the most keys first, so that the last workgroups to start are the short
-// ones.  With more of them: sequence after sequence, each from its last block on.
+// ones.  With more of them, and where the order is of no matter (3 x 100 to 300 tokens 12.0 -> 11.5 us): sequence after sequence,
+// each from its last block on.
 __device__ __forceinline__ bool find_block(const VarlenArgs& a, int at, int& q0, int& M, int& k0, int& N, int& block) {
     const int lane = threadIdx.x & 63;
     auto blocks = [&](int m) { return (int)(((int64_t)m * a.groups + kVarRows - 1) / kVarRows); };
-    if (a.seqs > 64) {
+    if (a.seqs == 1) {  // (the search for one of several takes 1 us: 77 tokens 7.2 -> 6.4 us, 500 15.4 -> 14.3)
+        sequence(a.cu_q, 0, a.total_q, q0, M);
+        sequence(a.cu_k, 0, a.total_k, k0, N);
+        block = blocks(M) - 1 - at;
+        return block >= 0;
+    }
+    if (a.seqs > 64 || gridDim.x <= kOrderless) {
         auto count = [&](int s) {
             int begin, len;
             sequence(a.cu_q, s, a.total_q, begin, len);

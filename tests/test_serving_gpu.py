@@ -224,7 +224,7 @@ def test_varlen_cut_with_nonfinite_values(value, gpu_device):
 
 def _among_many(lengths, seqs=60):
     """The lengths with empty sequences before, between and behind them, `seqs` in all: with 17 K/V heads or more they count as
-    enough blocks to run in tiles of 32 keys."""
+    enough blocks to run in tiles of 32 keys, with 5 as enough to be sorted."""
     gaps, out = seqs - len(lengths), []
     for i, n in enumerate(lengths):
         out += [0] * (gaps * (i + 1) // (len(lengths) + 1) - gaps * i // (len(lengths) + 1)) + [n]
@@ -233,7 +233,7 @@ def _among_many(lengths, seqs=60):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("heads", [(17, 17), (40, 20), (119, 17)])
+@pytest.mark.parametrize("heads", [(17, 17), (40, 20), (119, 17), (5, 5), (24, 8)])
 @pytest.mark.parametrize("lengths", [(1,), (0, 5, 0, 2), (31, 32, 33, 64, 65), (127, 128, 129, 1), (300, 1, 511), (161,)])
 def test_varlen_many_blocks(lengths, heads, d, dtype, gpu_device):
     (h, hk), t, dt = heads, sum(lengths), DTYPES[dtype]
