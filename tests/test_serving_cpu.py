@@ -291,6 +291,37 @@ def test_cache_movement_validation():
 
 
 @pytest.mark.skipif(not os.path.exists("/opt/rocm/bin/hipcc"), reason="needs hipcc")
+@pytest.mark.parametrize("causal", [False, True])
+def test_the_oracle_agrees_with_torch_in_64_bits(causal):
+    """The formulas that the GPU tests compare with, against torch's attention sequence by sequence, packed and in pages."""
+    from oracle import serving_oracle as SO
+
+    m, n, h, hk, d, page = (5, 0, 17), (9, 3, 17), 6, 2, 16, 4
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(t, heads, d, generator=g).to(torch.bfloat16) for t, heads in ((sum(m), h), (sum(n), hk), (sum(n), hk)))
+    cu_q, cu_k = (torch.tensor([0] + list(x)).cumsum(0).to(torch.int32) for x in (m, n))
+    o, norm, _, _ = SO.varlen(q, k, v, cu_q, cu_k, causal)
+    for s in range(len(m)):
+        qs, ks, vs = (x[cu[s]:cu[s + 1]].double().transpose(0, 1) for x, cu in ((q, cu_q), (k, cu_k), (v, cu_k)))
+        ks, vs = (x.repeat_interleave(h // hk, 0) for x in (ks, vs))
+        sees = torch.ones(m[s], n[s], dtype=torch.bool).tril(n[s] - m[s]) if causal else torch.ones(m[s], n[s], dtype=torch.bool)
+        want = torch.nn.functional.scaled_dot_product_attention(qs[None], ks[None], vs[None], attn_mask=sees)[0].transpose(0, 1)
+        logits = (qs @ ks.transpose(1, 2) * d ** -0.5).masked_fill(~sees, float("-inf"))
+        rows = slice(cu_q[s], cu_q[s + 1])
+        assert torch.allclose(o[rows], want, rtol=1e-12, atol=1e-12)
+        assert torch.allclose(norm[:, rows], torch.logsumexp(logits, -1), rtol=1e-12, atol=1e-12)
+        if not causal or m[s] == 0:
+            continue
+        # the same keys in pages, in an order of their own
+        table = torch.randperm(8, generator=g)[: -(-n[s] // page)].to(torch.int32)
+        caches = [torch.full((8, page, hk, d), float("nan"), dtype=torch.bfloat16) for _ in range(2)]
+        for c, x in zip(caches, (k, v)):
+            for j in range(n[s]):
+                c[table[j // page], j % page] = x[cu_k[s] + j]
+        paged = SO.paged(q[rows][None], *caches, table[None], torch.tensor([n[s]]), layout="NHD")
+        assert torch.allclose(paged[0][0], want, rtol=1e-12, atol=1e-12) and torch.allclose(paged[1][0], norm[:, rows])
+
+
 def test_only_the_lds_load_sequence_touches_m0(tmp_path):
     """The packed forward sets m0 in inline assembly, which the compiler cannot be told about: in its assembly m0 appears
     only as the destination of the move that precedes each direct-to-LDS load."""
