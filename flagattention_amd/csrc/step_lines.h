@@ -35,7 +35,11 @@ struct Steps {
         : M(m), N(n), nb((m + (1 << tokens_shift) - 1) >> tokens_shift), shift(tokens_shift), causal(causal_) {}
     __host__ __device__ int end(int j) const { return causal ? min((j + 1) << shift, M) + N - M : N; }  // keys that block j sees (0 or less: none)
     __host__ __device__ int tiles(int j) const { return max((end(j) + kVarKeys - 1) / kVarKeys, 1); }
-    // tiles of the first j < nb blocks: the first `ones` of them one each, block i of the others ceil(((i + 1) 2^shift + N - M) / 64)
+    // 1 + 2 + .. + n modulo 2^32: the even one of n and n + 1 is halved before the product
+    __host__ __device__ static unsigned triangle(unsigned n) { return n & 1 ? (n + 1) / 2 * n : n / 2 * (n + 1); }
+    // tiles of the first j < nb blocks: the first `ones` of them one each, block i of the others ceil(((i + 1) 2^shift + N - M) / 64).
+    // (Sums from the sequence's first tile on pass 32 bits where a block sees 3 million keys; modulo 2^32 their differences, which do
+    // not, are exact.)
     __host__ __device__ int tiles_before(int j) const {
         if (!causal) return j * max((N + kVarKeys - 1) / kVarKeys, 1);
         const int d = N - M;
@@ -43,13 +47,13 @@ struct Steps {
         const int over = j - ones;
         if (over == 0) return ones;
         static_assert(kVarKeys == 64, "2^6 keys");
-        if (shift > 6) return ones + ((j * (j + 1) - ones * (ones + 1)) / 2 << (shift - 6)) + over * ((d + kVarKeys - 1) >> 6);
+        if (shift > 6) return (int)(ones + ((triangle(j) - triangle(ones)) << (shift - 6)) + (unsigned)over * (unsigned)((d + kVarKeys - 1) >> 6));
         const int q = 6 - shift, c = -(-d >> shift);  // 2^q blocks a tile; d / 2^shift rounded up
         auto sum = [&](int n) {  // of ceil(k / 2^q) for k = 1 .. n
-            const int m = n >> q, r = n & ((1 << q) - 1);
-            return ((m * (m + 1) / 2) << q) + r * (m + 1);
+            const unsigned m = (unsigned)n >> q, r = (unsigned)n & ((1u << q) - 1);
+            return (triangle(m) << q) + r * (m + 1);
         };
-        return ones + sum(j + c) - sum(ones + c);
+        return (int)(ones + (sum(j + c) - sum(ones + c)));
     }
     __host__ __device__ int before(int j) const { return tiles_before(j) + kStart * j; }  // steps of the first j < nb blocks
     __host__ __device__ int total() const { return nb == 0 ? 0 : before(nb - 1) + tiles(nb - 1) + kStart; }
