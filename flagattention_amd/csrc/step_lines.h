@@ -14,10 +14,13 @@ namespace attn {
 
 // A line of steps in equal shares: share w has `base` of them, one more for w < rest.
 struct EqualShares {
-    int base, rest;
-    __host__ __device__ EqualShares(int total, int shares) : base(total / shares), rest(total % shares) {}
+    int total, base, rest;
+    __host__ __device__ EqualShares(int total_, int shares) : total(total_), base(total_ / shares), rest(total_ % shares) {}
     __host__ __device__ int begin(int w) const { return w * base + (w < rest ? w : rest); }
-    __host__ __device__ int owner(int pos) const {  // the share that holds step pos
+    // The share that holds step pos.  (One outside the line belongs to its first or last share: sequences whose offsets overlap can
+    // have more steps than 31 bits count, and lie on the line anywhere; what is read for them has to exist all the same.)
+    __host__ __device__ int owner(int pos) const {
+        pos = max(min(pos, total - 1), 0);
         const int longer = rest * (base + 1);
         return pos < longer ? pos / (base + 1) : rest + (pos - longer) / base;
     }
