@@ -17,7 +17,7 @@ import math
 import torch
 
 from . import _lib
-from .sage_attention._common import DTYPE_CODE, current_stream_ptr, device_guard, require_gpu, rows_aligned, split_workspace
+from .sage_attention._common import DTYPE_CODE, current_stream_ptr, device_guard, require_gpu, split_workspace
 
 __all__ = ["flash_attention_varlen", "paged_attention", "append_to_cache", "copy_pages"]
 
@@ -54,14 +54,27 @@ def _index_list(t, name):
     return t.contiguous()
 
 
+def _stride(t, dim):
+    """A dimension of one entry has no stride: what torch keeps there is arbitrary."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def _aligned(t):
+    """Rows on 16-byte boundaries that run along the last axis (which the kernels read 16 bytes at a time)."""
+    e = t.element_size()
+    if t.data_ptr() % 16 != 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        return False
+    return t.numel() == 0 or all(s * e % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()) if n > 1)
+
+
 def _rows16(t):
-    return t if rows_aligned(t) else t.contiguous()
+    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_out(out, like):
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError("out must have the shape, dtype and device of q")
-    if not rows_aligned(out):
+    if not _aligned(out):
         raise ValueError("out: rows must be 16-byte aligned, with a unit innermost stride")
 
 
@@ -78,12 +91,12 @@ def _check_float16s(q, k, v):
 
 
 def _token_desc(t):  # [tokens, heads, head_dim]
-    return _lib.SageTensor(t.data_ptr(), 0, t.stride(1), t.stride(0))
+    return _lib.SageTensor(t.data_ptr(), 0, _stride(t, 1), _stride(t, 0))
 
 
 def _cache_desc(t, hnd):
-    s = t.stride()
-    return _lib.SageTensor(t.data_ptr(), s[0], s[1] if hnd else s[2], s[2] if hnd else s[1])
+    head, place = (1, 2) if hnd else (2, 1)
+    return _lib.SageTensor(t.data_ptr(), _stride(t, 0), _stride(t, head), _stride(t, place))
 
 
 def _layout(tensor_layout):
@@ -100,7 +113,7 @@ def _check_caches(k_cache, v_cache, hnd):
     if k_cache.shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have the same shape")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if not rows_aligned(t):
+        if not _aligned(t):
             raise ValueError(f"{name}: rows must be 16-byte aligned, with a unit innermost stride (a cache is not copied)")
     p, a, b, d = k_cache.shape
     return (p, a, b, d) if hnd else (p, b, a, d)
@@ -236,7 +249,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
         if return_log_normalizer:
             L = torch.empty((S, H) if q.dim() == 3 else (S, H, M), dtype=torch.float32, device=q.device)
         p = _lib.PagedParams()
-        p.q, p.out = (_lib.SageTensor(t.data_ptr(), t.stride(0), t.stride(-2), t.stride(1) if t.dim() == 4 else 0) for t in (q, o))
+        p.q, p.out = (_lib.SageTensor(t.data_ptr(), _stride(t, 0), _stride(t, t.dim() - 2), _stride(t, 1) if t.dim() == 4 else 0) for t in (q, o))
         p.k_cache, p.v_cache = _cache_desc(k_cache, hnd), _cache_desc(v_cache, hnd)
         p.log_normalizer = L.data_ptr() if L is not None else None
         p.block_table, p.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
@@ -339,8 +352,8 @@ def copy_pages(k_cache, v_cache, src, dst):
         if any(s < 0 for s in t.stride()) or (p.pages > 1 and t.stride(1 if layered else 0) * e < p.page_bytes):
             raise ValueError(f"{name}_cache: pages overlap")
         setattr(p, f"{name}_cache", t.data_ptr())
-        setattr(p, f"{name}_stride_layer", t.stride(0) * e if layered else 0)
-        setattr(p, f"{name}_stride_page", t.stride(1 if layered else 0) * e)
+        setattr(p, f"{name}_stride_layer", _stride(t, 0) * e if layered else 0)
+        setattr(p, f"{name}_stride_page", _stride(t, 1 if layered else 0) * e)
     p.src, p.src_int64 = src.data_ptr(), 1 if src.dtype == torch.int64 else 0
     p.dst, p.dst_int64 = dst.data_ptr(), 1 if dst.dtype == torch.int64 else 0
     if src is call[2] and dst is call[3]:  # (nothing was copied)

@@ -50,3 +50,85 @@ def test_varlen_a_chunk_against_millions_of_keys(n, gpu_device):
     for i in range(h):
         SO.assert_close(o[:, i], want, tol, i)
         SO.assert_close(norm[i], 64.0 + count[:, 0].double().log(), norm_tol, i)
+
+
+def _randn(shape, dtype, device, seed):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(device)
+
+
+def _odd(t, offset=1):
+    """The tensor, contiguous, `offset` elements behind a 16-byte boundary."""
+    buf = torch.zeros(t.numel() + offset, dtype=t.dtype, device=t.device)
+    return buf[offset:].view(t.shape).copy_(t)
+
+
+def _lone(t, dim, stride):
+    """The tensor, one entry long in `dim`, with an odd stride there."""
+    strides = list(t.stride())
+    strides[dim] = stride
+    return torch.as_strided(t, t.shape, strides, t.storage_offset())
+
+
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_contiguous_tensors_at_odd_offsets(d, gpu_device):
+    import flag_attn
+
+    q, k, v = (_odd(_randn((70, n, d), torch.float16, gpu_device, i), 1 + 2 * i) for i, n in enumerate((4, 2, 2)))
+    cu = _cu((50, 20), gpu_device)
+    for _ in range(2):  # (and once more as a call of a known shape)
+        o, norm = flag_attn.flash_attention_varlen(q, k, v, cu, causal=True, return_log_normalizer=True)
+        want, want_norm, tol, norm_tol = SO.varlen(q, k, v, cu, cu, True)
+        SO.assert_close(o, want, tol)
+        SO.assert_close(norm, want_norm, norm_tol)
+    aligned = [x.clone() for x in (q, k, v)]  # (a plan of aligned tensors of these sizes serves no others)
+    assert torch.equal(flag_attn.flash_attention_varlen(*aligned, cu, causal=True), o)
+    assert torch.equal(flag_attn.flash_attention_varlen(q, k, v, cu, causal=True), o)
+    with pytest.raises(ValueError, match="out: rows"):
+        flag_attn.flash_attention_varlen(q, k, v, cu, causal=True, out=_odd(torch.zeros_like(q)))
+    kc, vc = (torch.zeros(5, 2, 16, d, dtype=torch.float16, device=gpu_device) for _ in range(2))
+    flag_attn.append_to_cache(k, v, kc, vc, torch.arange(70, device=gpu_device))
+    assert torch.equal(kc.transpose(1, 2).reshape(80, 2, d)[:70], k) and torch.equal(vc.transpose(1, 2).reshape(80, 2, d)[:70], v)
+    if d == 16:
+        return
+    table, lens = torch.arange(5, dtype=torch.int32, device=gpu_device)[None].repeat(3, 1), torch.tensor([70, 3, 17], dtype=torch.int32, device=gpu_device)
+    p = _odd(q[:3].clone())
+    want, _, tol, _ = SO.paged(p, kc, vc, table, lens)
+    SO.assert_close(flag_attn.paged_attention(p, kc, vc, table, lens), want, tol)
+
+
+def test_strides_of_dimensions_with_one_entry(gpu_device):
+    """One token, one head, one sequence, one page: what a tensor's stride is there does not matter, 2^40 neither."""
+    import flag_attn
+
+    for stride in (3, 1 << 40):
+        for h, hk, t in ((4, 2, 1), (1, 1, 5), (1, 1, 1)):
+            q, k, v = (_randn((t, n, 64), torch.bfloat16, gpu_device, i) for i, n in enumerate((h, hk, hk)))
+            cu = _cu((t,), gpu_device)
+            want, _, tol, _ = SO.varlen(q, k, v, cu, cu, True)
+            out = torch.zeros_like(q)
+            dims = [i for i, n in ((0, t), (1, h)) if n == 1]
+            for dim in dims:
+                q, out = _lone(q, dim, stride), _lone(out, dim, stride)
+            for dim in [i for i, n in ((0, t), (1, hk)) if n == 1]:
+                k, v = _lone(k, dim, stride), _lone(v, dim, stride)
+            SO.assert_close(flag_attn.flash_attention_varlen(q, k, v, cu, causal=True), want, tol)
+            flag_attn.flash_attention_varlen(q, k, v, cu, causal=True, out=out)
+            SO.assert_close(out, want, tol)
+        for layout in ("HND", "NHD"):
+            # one page of one head, one sequence of one new token
+            kc, vc = (_lone(_lone(torch.zeros((1, 1, 16, 64) if layout == "HND" else (1, 16, 1, 64), dtype=torch.bfloat16, device=gpu_device), 0, stride),
+                            1 if layout == "HND" else 2, stride) for _ in range(2))
+            k, v = (_randn((9, 1, 64), torch.bfloat16, gpu_device, i) for i in (5, 6))
+            flag_attn.append_to_cache(_lone(k, 1, stride), _lone(v, 1, stride), kc, vc, torch.arange(9, device=gpu_device), layout)
+            assert torch.equal(kc.reshape(16, 1, 64)[:9], k) and torch.equal(vc.reshape(16, 1, 64)[:9], v)
+            q = _randn((1, 1, 1, 64), torch.bfloat16, gpu_device, 7)
+            table, lens = torch.zeros(1, 1, dtype=torch.int32, device=gpu_device), torch.tensor([9], dtype=torch.int32, device=gpu_device)
+            want, _, tol, _ = SO.paged(q, kc, vc, table, lens, layout=layout)
+            for dim in range(3):
+                q = _lone(q, dim, stride)
+            SO.assert_close(flag_attn.paged_attention(q, kc, vc, _lone(table, 1, 3), lens, tensor_layout=layout), want, tol)
+        both = [_lone(_randn((1, 2, 3, 8), torch.float32, gpu_device, i)[None], 0, stride) for i in (8, 9)]
+        both = [torch.as_strided(x, (1, 1, 2, 3, 8), (stride, stride, 24, 8, 1)) for x in both]
+        before = [x.clone() for x in both]
+        flag_attn.copy_pages(*both, torch.zeros(1, dtype=torch.int32, device=gpu_device), torch.zeros(1, dtype=torch.int32, device=gpu_device))
+        assert all(torch.equal(x, y) for x, y in zip(both, before))
