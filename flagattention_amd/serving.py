@@ -205,7 +205,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
     aligned rows, any page size; head_dim 64 or 128.  ``block_table`` ``[S, width]`` int32: the pages of every sequence in order.
     ``seq_lens`` ``[S]`` int32: tokens of every sequence in the cache, the new ones among them (write those with
     ``append_to_cache`` first).  Of M new tokens, token m sees the keys up to ``seq_lens - M + m``.  A sequence of length 0 (a slot
-    that is not in use) gets zero rows; table entries that are no page of the cache hide their tokens.
+    that is not in use) gets zero rows; table entries that are no page of the cache hide their tokens; lengths beyond the table are
+    cut to it, to 0 where it has no entries or the cache no pages.
 
     Returns ``o`` in the shape of ``q``, or ``(o, log_normalizer)`` with the natural log-sum-exp ``[S, H]`` (``[S, H, M]``) in fp32.
     ``out``: where to write instead of a new tensor.
@@ -248,6 +249,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
         L = None
         if return_log_normalizer:
             L = torch.empty((S, H) if q.dim() == 3 else (S, H, M), dtype=torch.float32, device=q.device)
+        if page_size > 0 and (pages == 0 or block_table.shape[1] == 0):  # (no place for a key)
+            o.fill_(0)
+            return (o, L.fill_(-math.inf)) if return_log_normalizer else o
         p = _lib.PagedParams()
         p.q, p.out = (_lib.SageTensor(t.data_ptr(), _stride(t, 0), _stride(t, t.dim() - 2), _stride(t, 1) if t.dim() == 4 else 0) for t in (q, o))
         p.k_cache, p.v_cache = _cache_desc(k_cache, hnd), _cache_desc(v_cache, hnd)

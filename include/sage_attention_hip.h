@@ -309,6 +309,7 @@ int sage_flash_varlen_fwd(const sage_varlen_params* p, void* workspace, int64_t 
  *   block_table  [seqs, table_width] int32 on the device, rows table_stride entries apart; entries past a sequence's last page have no
  *                effect.  The tokens of an entry that is no page of the cache (negative, or pages and more) take no part.
  *   seq_lens     [seqs] int32 on the device, clamped to 0 .. table_width * page_size
+ *   A cache without pages or a table without entries is refused (SAGE_E_INVALID): there is no key, and no kernel to launch.
  *   log_normalizer  optional [seqs, Hq, new_tokens] fp32 contiguous, natural log; NULL = none
  * The table and the lengths are read by the kernels: a captured graph follows their present values.  Zero rows, infinities and
  * NaN as for sage_flash_varlen_fwd.  head_dim 64 or 128; any page_size.

@@ -132,3 +132,23 @@ def test_strides_of_dimensions_with_one_entry(gpu_device):
         before = [x.clone() for x in both]
         flag_attn.copy_pages(*both, torch.zeros(1, dtype=torch.int32, device=gpu_device), torch.zeros(1, dtype=torch.int32, device=gpu_device))
         assert all(torch.equal(x, y) for x, y in zip(both, before))
+
+
+@pytest.mark.parametrize("pages,width", [(6, 0), (0, 3), (0, 0)])
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+def test_paged_without_a_place_for_a_key(layout, pages, width, gpu_device):
+    """All slots idle and a table as wide as the longest sequence needs; a cache that has no pages yet."""
+    import flag_attn
+
+    kc, vc = (torch.zeros((pages, 2, 16, 64) if layout == "HND" else (pages, 16, 2, 64), dtype=torch.bfloat16, device=gpu_device) for _ in range(2))
+    table, lens = torch.zeros(3, width, dtype=torch.int32, device=gpu_device), torch.tensor([0, 5, 0], dtype=torch.int32, device=gpu_device)
+    for shape in ((3, 4, 64), (3, 2, 4, 64)):
+        q = _randn(shape, torch.bfloat16, gpu_device, 1)
+        o, norm = flag_attn.paged_attention(q, kc, vc, table, lens, tensor_layout=layout, return_log_normalizer=True)
+        assert o.shape == q.shape and (o == 0).all()
+        assert norm.shape == ((3, 4) if len(shape) == 3 else (3, 4, 2)) and (norm == float("-inf")).all()
+        wide = torch.full((*shape[:-1], 128), 7.0, dtype=torch.bfloat16, device=gpu_device)
+        assert flag_attn.paged_attention(q, kc, vc, table, lens, tensor_layout=layout, out=wide[..., :64]).data_ptr() == wide.data_ptr()
+        assert (wide[..., :64] == 0).all() and (wide[..., 64:] == 7.0).all()
+    with pytest.raises(ValueError):
+        flag_attn.paged_attention(q, kc, vc, table[:2], lens, tensor_layout=layout)
