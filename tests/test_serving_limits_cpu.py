@@ -52,3 +52,25 @@ def test_rows_are_aligned_or_copied():
     assert not S._aligned(torch.as_strided(buf, (2, 4, 64), (260, 64, 1)))
     assert not S._aligned(torch.as_strided(buf, (2, 4, 64), (256, 64, 2)))
     assert S._aligned(torch.zeros(0, 4, 64)) and S._aligned(torch.zeros(3, 0, 64))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_the_oracle_is_torchs_attention(causal):
+    """What the GPU tests compare with, against torch's attention in 64 bits (needs no compiler)."""
+    from oracle import serving_oracle as SO
+
+    m, n, h, hk, d = (1, 12, 0, 20), (30, 5, 4, 20), 4, 2, 8
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(sum(x), heads, d, generator=g).to(torch.float16) for x, heads in ((m, h), (n, hk), (n, hk)))
+    cu_q, cu_k = (torch.tensor([0] + list(x)).cumsum(0) for x in (m, n))
+    o, norm, _, _ = SO.varlen(q, k, v, cu_q, cu_k, causal)
+    for s in range(len(m)):
+        rows = slice(cu_q[s], cu_q[s + 1])
+        qs, ks, vs = (x.double().transpose(0, 1) for x in (q[rows], k[cu_k[s]:cu_k[s + 1]], v[cu_k[s]:cu_k[s + 1]]))
+        ks, vs = (x.repeat_interleave(h // hk, 0) for x in (ks, vs))
+        sees = torch.ones(m[s], n[s], dtype=torch.bool).tril(n[s] - m[s]) if causal else torch.ones(m[s], n[s], dtype=torch.bool)
+        want = torch.nn.functional.scaled_dot_product_attention(qs, ks, vs, attn_mask=sees).transpose(0, 1)
+        want = torch.where(sees.any(1)[:, None, None], want, 0.0)  # (rows that see nothing are zeros here)
+        logits = (qs @ ks.transpose(1, 2) * d ** -0.5).masked_fill(~sees, float("-inf"))
+        assert torch.allclose(o[rows], want, rtol=1e-12, atol=1e-12)
+        assert torch.allclose(norm[:, rows], torch.logsumexp(logits, -1), rtol=1e-12, atol=1e-12)
