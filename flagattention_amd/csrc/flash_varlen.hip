@@ -54,6 +54,9 @@ constexpr int kVarWaves = 4;
 constexpr int kVarThreads = 64 * kVarWaves;
 constexpr int kVarRows = 32 * kVarWaves;
 constexpr float kLag = 8.0f;
+// From this size of a row's reference point on (in base 2) its rounding to 24 bits, which shifts all exponents of the row alike, can
+// take P out of its range: by up to 4 below it.
+constexpr float kHuge = 134217728.0f;
 
 // Sequence s of a packed axis.  (Offsets out of order or past the end give no rows that do not exist.)
 __device__ __forceinline__ void sequence(const int32_t* cu, int s, int total, int& begin, int& len) {
@@ -165,8 +168,8 @@ struct BlockAt {
 
 // One row by one wave, from its keys alone: query token qt, head h, the first n keys from k0 on.  A lane is a key for the scores,
 // and D / 64 channels for the output.  part_o: where the wave's partial results begin and the row's log-sum-exp goes, for row r of
-// the wave, or null.  For rows whose tiles hold infinities or NaN in V: a thousand times slower than a tile's share
-// of the kernel below, and hardly ever called.
+// the wave, or null.  For rows whose tiles hold infinities or NaN in V and for huge scores: a hundred times and more slower
+// than the kernel below, and hardly ever called.
 template <int D, typename VT>
 __device__ void careful_row(const VarlenArgs& a, int qt, int h, int hk, int k0, int n, float* part_o, float* part_lse, int r) {
     constexpr int CH = D / 64;
@@ -533,22 +536,34 @@ __global__ __launch_bounds__(kVarThreads, KEYS == 64 ? 2 : 3) void flash_varlen_
     // An infinity or NaN in V under a hidden key must not reach the rows that do not see it (0 times it is NaN): where an output is not
     // finite and a tile that hides keys holds one, the wave's rows are computed again, key by key.  (Looking at those tiles inside the
     // loop: 48 prompts of 1 to 700 tokens, H32/8 D128, 43.5 us instead of 42.1.)
-    if (clear_tiles < my_tiles) {
+    // So they are where a reference point is huge, or was: infinite P leave a NaN sum then, though neither Q nor K holds one.
+    auto any_odd = [&](const VT* base, int64_t stride, int first, int end) {
+        unsigned odd = 0;
+#pragma unroll 1
+        for (int n = first + lane / CPR; n < end; n += 64 / CPR) {
+            const v4i f = *reinterpret_cast<const v4i*>(base + (int64_t)n * stride + 8 * (lane % CPR));
+#pragma unroll
+            for (int w = 0; w < 4; w++) odd |= nonfinite_halves<VT>((unsigned)f[w]);
+        }
+        return __builtin_amdgcn_ballot_w64(odd != 0) != 0;
+    };
+    const bool huge = __builtin_amdgcn_ballot_w64(__builtin_fabsf(m_i) >= kHuge && __builtin_fabsf(m_i) < INFINITY) != 0;
+    if (clear_tiles < my_tiles || huge || __builtin_amdgcn_ballot_w64(l_i != l_i) != 0) {
         float zero[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) zero[i & 1] = __builtin_fmaf(acc[dt][i], 0.0f, zero[i & 1]);
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(zero[0] + zero[1] != 0.0f) != 0, 0)) {
-            unsigned odd = 0;
-            const int first = KEYS * clear_tiles, pieces = (min(KEYS * my_tiles, N) - first) * CPR;
-#pragma unroll 1
-            for (int i = lane; i < pieces; i += 64) {
-                const v4i f = *reinterpret_cast<const v4i*>(vbase + (int64_t)(first + i / CPR) * a.vs_t + 8 * (i % CPR));
+        if (__builtin_expect(huge || __builtin_amdgcn_ballot_w64(zero[0] + zero[1] != 0.0f) != 0, 0)) {
+            unsigned odd_q = 0;
 #pragma unroll
-                for (int w = 0; w < 4; w++) odd |= nonfinite_halves<VT>((unsigned)f[w]);
-            }
-            if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) odd_q |= nonfinite_halves<VT>((unsigned)__builtin_bit_cast(v4i, qf[t])[w]);
+            odd_q |= __shfl_xor((int)odd_q, 32);
+            const int end = min(KEYS * my_tiles, N);
+            if (huge || any_odd(vbase, a.vs_t, KEYS * clear_tiles, end) ||
+                (__builtin_amdgcn_ballot_w64(l_i != l_i && odd_q == 0) != 0 && !any_odd(kbase, a.ks_t, 0, end))) {
                 for (int r = 32 * wave; r < 32 * wave + 32 && r <= last_row; r++) {
                     const int on = tokens_on(r), m = tok0 + on, n = a.causal ? min(m + shift, N - 1) + 1 : N;
                     careful_row<D, VT>(a, q0 + m, hk * a.groups + rem0 + r - on * a.groups, hk, k0, CUT ? min(n, KEYS * ntiles) : n, part_o, part_lse, r - 32 * wave);

@@ -152,3 +152,106 @@ def test_paged_without_a_place_for_a_key(layout, pages, width, gpu_device):
         assert (wide[..., :64] == 0).all() and (wide[..., 64:] == 7.0).all()
     with pytest.raises(ValueError):
         flag_attn.paged_attention(q, kc, vc, table[:2], lens, tensor_layout=layout)
+
+
+# Scores so far from 0 that their rounding to 24 bits is worth many powers of two: the weights are 0 or 1 then (or equal, for equal keys).
+
+def _means(q, k, v, causal):
+    """softmax(q k^T) v for q, k whose rows are multiples of the vector of ones, in 64 bits; the mean of |v| under the weights; the
+    log normalizer [H, M]."""
+    m, h, d = q.shape
+    n, hk = k.shape[:2]
+    s = q[:, :, :1].double() * k[:, :, :1].double().repeat_interleave(h // hk, 1).permute(2, 1, 0) * d  # [M, H, N]
+    if causal:
+        s = s.masked_fill((torch.arange(n, device=q.device)[None] > torch.arange(m, device=q.device)[:, None] + n - m)[:, None], float("-inf"))
+    w, vv = torch.softmax(s, -1), v.double().repeat_interleave(h // hk, 1)
+    return torch.einsum("mhn,nhd->mhd", w, vv), torch.einsum("mhn,nhd->mhd", w, vv.abs()), torch.logsumexp(s, -1).t()
+
+
+def _check_means(o, norm, want, half_step):
+    """P and o are rounded by half a step; weights are added up in fp32, 300 at most that are not 0; a score is the sum of at most 128
+    products in fp32, times a scale."""
+    o_want, size, norm_want = want
+    SO.assert_close(o, o_want, half_step * (o_want.abs() + size) + 300 * 2.0 ** -24 * size)
+    SO.assert_close(norm, norm_want, 140 * 2.0 ** -24 * norm_want.abs() + 300 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("heads,seqs", [((4, 2), 1), ((34, 17), 60)])  # (few blocks, many)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 2000.0), (torch.float16, 4000.0), (torch.float16, 60000.0),
+                                        (torch.bfloat16, 16000.0), (torch.bfloat16, 2.0 ** 56)])
+def test_varlen_huge_scores(dtype, size, d, heads, seqs, gpu_device):
+    import flag_attn
+
+    (h, hk), n = heads, 300
+    g = torch.Generator().manual_seed(0)
+    keys = (1 - torch.randperm(n, generator=g) / 512).to(gpu_device)
+    v = _randn((n, hk, d), dtype, gpu_device, 1)
+    cu = torch.tensor([0] * seqs + [n], dtype=torch.int32, device=gpu_device)
+    for sign in (1, -1):
+        q = torch.full((n, h, d), sign * size, dtype=dtype, device=gpu_device)
+        k = (size * keys)[:, None, None].expand(n, hk, d).to(dtype).contiguous()
+        for causal in (True, False):
+            o, norm = flag_attn.flash_attention_varlen(q, k, v, cu, causal=causal, sm_scale=1.0, return_log_normalizer=True)
+            _check_means(o, norm, _means(q, k, v, causal), torch.finfo(dtype).eps / 2)
+
+
+@pytest.mark.parametrize("heads,seqs", [((4, 2), 1), ((34, 17), 60)])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 2000.0), (torch.bfloat16, 16000.0), (torch.bfloat16, 2.0 ** 56)])
+def test_varlen_scores_that_rise_from_far_below(dtype, size, heads, seqs, gpu_device):
+    """Keys whose weights are infinite against the first reference point, and 0 against the one of the rows that see more; a
+    query among them that is NaN, and stays alone."""
+    import flag_attn
+
+    (h, hk), n, d = heads, 300, 128
+    q = torch.full((n, h, d), size, dtype=dtype, device=gpu_device)
+    k = torch.zeros(n, hk, d, dtype=dtype, device=gpu_device)
+    k[:100] = (-size * (1 - torch.arange(100, device=gpu_device) / 512))[:, None, None]
+    v = _randn((n, hk, d), dtype, gpu_device, 1)
+    cu = torch.tensor([0] * seqs + [n], dtype=torch.int32, device=gpu_device)
+    for causal in (True, False):
+        clean = flag_attn.flash_attention_varlen(q, k, v, cu, causal=causal, sm_scale=1.0, return_log_normalizer=True)
+        _check_means(*clean, _means(q, k, v, causal), torch.finfo(dtype).eps / 2)
+    clean = flag_attn.flash_attention_varlen(q, k, v, cu, causal=True, sm_scale=1.0)
+    q[150, 1] = float("nan")
+    o = flag_attn.flash_attention_varlen(q, k, v, cu, causal=True, sm_scale=1.0)
+    bad = torch.zeros(n, h, dtype=torch.bool, device=gpu_device)
+    bad[150, 1] = True
+    assert o[bad].isnan().all() and torch.equal(o[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 4000.0), (torch.bfloat16, 16000.0)])
+def test_varlen_huge_scores_in_shares(dtype, size, gpu_device):
+    import flag_attn
+
+    m, n, h, hk, d = 70, 9000, 4, 2, 128
+    g = torch.Generator().manual_seed(0)
+    keys = 0.5 + torch.rand(n, generator=g) / 4
+    keys[777] = 1.0
+    q = torch.full((m, h, d), size, dtype=dtype, device=gpu_device)
+    k = (size * keys.to(gpu_device))[:, None, None].expand(n, hk, d).to(dtype).contiguous()
+    v = _randn((n, hk, d), dtype, gpu_device, 1)
+    assert _is_cut(q, k, 1, True)
+    for causal in (True, False):
+        o, norm = flag_attn.flash_attention_varlen(q, k, v, _cu((m,), gpu_device), _cu((n,), gpu_device), causal, 1.0, True)
+        _check_means(o, norm, _means(q, k, v, causal), torch.finfo(dtype).eps / 2)
+
+
+@pytest.mark.parametrize("width", [20, 600])  # (a workgroup per item, equal shares)
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 4000.0), (torch.bfloat16, 16000.0), (torch.bfloat16, 2.0 ** 56)])
+def test_paged_huge_scores(dtype, size, width, gpu_device):
+    import flag_attn
+
+    n, m, h, hk, d = 300, 3, 8, 2, 128
+    g = torch.Generator().manual_seed(0)
+    keys = 0.5 + torch.rand(320, generator=g) / 4
+    keys[:5], keys[77] = -1.0, 1.0
+    kc = (size * keys.to(gpu_device))[:, None, None].expand(320, hk, d).to(dtype).contiguous().view(20, 16, hk, d)
+    vc = _randn((20, 16, hk, d), dtype, gpu_device, 1)
+    q = torch.full((1, m, h, d), size, dtype=dtype, device=gpu_device)
+    table = torch.full((1, width), -1, dtype=torch.int32, device=gpu_device)
+    table[0, :20] = torch.arange(20)
+    lens = torch.tensor([n], dtype=torch.int32, device=gpu_device)
+    o, norm = flag_attn.paged_attention(q, kc, vc, table, lens, 1.0, "NHD", True)
+    want = _means(q[0], kc.view(320, hk, d)[:n], vc.view(320, hk, d)[:n], True)
+    _check_means(o[0], norm[0], want, torch.finfo(dtype).eps / 2)
