@@ -382,12 +382,12 @@ bool add_scale(Key& key, PyObject* o) {
     return true;
 }
 
-// Tensors a[from] .. a[to - 1], without gradients, into the key.
+// Tensors a[from] .. a[to - 1], without gradients and tangents, into the key.
 bool add_tensors(Key& key, PyObject* const* a, int from, int to, const at::Tensor** t) {
     for (int i = from; i < to; i++) {
         if (!plain(a[i])) return false;
         t[i] = &THPVariable_Unpack(a[i]);
-        if (t[i]->requires_grad()) return false;
+        if (t[i]->requires_grad() || t[i]->_fw_grad(0).defined()) return false;
         key.add(*t[i]);
     }
     key.add((int64_t)t[from]->device().index());

@@ -8,13 +8,14 @@ keys and values in pages with the attention of new tokens over it.
 
 Lengths, tables, slots and page lists stay on the device: no call waits for the GPU, and a captured graph follows their present
 values.  Entries that lead nowhere (a negative slot, a page that the cache does not have) move and read nothing.  The cache
-belongs to the caller; these functions allocate outputs and scratch memory only.  Forward only: tensors that require grad raise.
+belongs to the caller; these functions allocate outputs and scratch memory only.  Forward only: tensors that require grad raise, and so do those with a tangent.
 """
 from __future__ import annotations
 
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .sage_attention._common import DTYPE_CODE, current_stream_ptr, device_guard, require_gpu, split_workspace
@@ -27,9 +28,11 @@ def _host():
 
 
 def _no_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError(f"{what}: forward only (no backward pass is built); call it under torch.no_grad() or on "
                                   "tensors that do not require grad")
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: tangents of forward-mode differentiation are not carried on")
 
 
 def _same_device(device, **tensors):
@@ -159,7 +162,7 @@ def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fals
     _int32(cu_seqlens_k, "cu_seqlens_k", 1)
     if cu_seqlens_q.numel() != cu_seqlens_k.numel() or cu_seqlens_q.numel() == 0:
         raise ValueError("cu_seqlens_q and cu_seqlens_k must have one entry more than there are sequences")
-    _no_grad("flash_attention_varlen", q, k, v)
+    _no_grad("flash_attention_varlen", q, k, v, out)
     _same_device(q.device, q=q, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k)
     if out is not None:
         _check_out(out, q)
@@ -234,7 +237,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
     _int32(seq_lens, "seq_lens", 1)
     if block_table.shape[0] != S or seq_lens.shape[0] != S:
         raise ValueError("block_table and seq_lens must have a row for every sequence of q")
-    _no_grad("paged_attention", q, k_cache, v_cache)
+    _no_grad("paged_attention", q, k_cache, v_cache, out)
     _same_device(q.device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, seq_lens=seq_lens)
     if out is not None:
         _check_out(out, q)

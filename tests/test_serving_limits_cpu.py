@@ -74,3 +74,45 @@ def test_the_oracle_is_torchs_attention(causal):
         logits = (qs @ ks.transpose(1, 2) * d ** -0.5).masked_fill(~sees, float("-inf"))
         assert torch.allclose(o[rows], want, rtol=1e-12, atol=1e-12)
         assert torch.allclose(norm[:, rows], torch.logsumexp(logits, -1), rtol=1e-12, atol=1e-12)
+
+
+def _calls(grad=(), tangent=()):
+    """A call of each operator on CPU tensors, those named with a gradient or a tangent: (function, arguments)."""
+    import flag_attn
+    from torch.autograd import forward_ad
+
+    def t(name, *shape):
+        x = torch.zeros(shape, dtype=torch.bfloat16)
+        if name in tangent:
+            x = forward_ad.make_dual(x, torch.ones_like(x))
+        return x.requires_grad_() if name in grad else x
+
+    cu, lens = torch.tensor([0, 5], dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    caches = {n: t(n, 4, 2, 16, 64) for n in ("k_cache", "v_cache")}
+    return [
+        (flag_attn.flash_attention_varlen, dict(q=t("q", 5, 4, 64), k=t("k", 5, 2, 64), v=t("v", 5, 2, 64), cu_seqlens_q=cu, out=t("out", 5, 4, 64))),
+        (flag_attn.paged_attention, dict(q=t("q", 3, 4, 64), **caches, block_table=torch.zeros(3, 2, dtype=torch.int32), seq_lens=lens, out=t("out", 3, 4, 64))),
+        (flag_attn.append_to_cache, dict(k=t("k", 5, 2, 64), v=t("v", 5, 2, 64), **caches, slots=torch.arange(5))),
+        (flag_attn.copy_pages, dict(**caches, src=torch.tensor([0]), dst=torch.tensor([1]))),
+    ]
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "k_cache", "v_cache", "out"])
+def test_gradients_and_tangents_raise(name):
+    """Nothing that takes part in differentiation, in either mode, is taken and dropped."""
+    from torch.autograd import forward_ad
+
+    for f, args in _calls(grad=(name,)):
+        if name in args:
+            with pytest.raises(NotImplementedError, match="no backward pass"):
+                f(**args)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+                f(**args)
+    with forward_ad.dual_level():
+        for f, args in _calls(tangent=(name,)):
+            if name in args:
+                with pytest.raises(NotImplementedError, match="tangents"):
+                    f(**args)
+        for f, args in _calls():
+            with pytest.raises(RuntimeError, match="no CPU fallback"):
+                f(**args)

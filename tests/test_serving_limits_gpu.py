@@ -255,3 +255,24 @@ def test_paged_huge_scores(dtype, size, width, gpu_device):
     o, norm = flag_attn.paged_attention(q, kc, vc, table, lens, 1.0, "NHD", True)
     want = _means(q[0], kc.view(320, hk, d)[:n], vc.view(320, hk, d)[:n], True)
     _check_means(o[0], norm[0], want, torch.finfo(dtype).eps / 2)
+
+
+def test_tangents_raise_in_calls_of_a_known_shape_too(gpu_device):
+    import flag_attn
+    from torch.autograd import forward_ad
+
+    q, k, v = (_randn((30, n, 64), torch.bfloat16, gpu_device, i) for i, n in enumerate((4, 2, 2)))
+    kc, vc = (torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device=gpu_device) for _ in range(2))
+    cu, slots = _cu((30,), gpu_device), torch.arange(30, device=gpu_device)
+    table, lens = torch.arange(4, dtype=torch.int32, device=gpu_device)[None], torch.tensor([30], dtype=torch.int32, device=gpu_device)
+    pages = slots[:1], slots[3:4]
+    calls = [lambda x: flag_attn.flash_attention_varlen(x(q), k, v, cu), lambda x: flag_attn.append_to_cache(k, x(v), kc, vc, slots),
+             lambda x: flag_attn.paged_attention(q[:1], kc, x(vc), table, lens), lambda x: flag_attn.copy_pages(x(kc), vc, *pages)]
+    for _ in range(2):
+        for call in calls:
+            call(lambda t: t)
+    with forward_ad.dual_level():
+        for call in calls:
+            call(lambda t: t)
+            with pytest.raises(NotImplementedError, match="tangents"):
+                call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
