@@ -404,6 +404,11 @@ bool all_ready(const at::Tensor* const* t, int rows, int all, const at::Device& 
     return true;
 }
 
+// Autograd's notice of a tensor that a kernel has changed in place (tensors made in inference mode take none).
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- packed sequences: (q, k, v, cu_seqlens_q, cu_seqlens_k, causal, sm_scale, want_log_normalizer)
 struct VarlenCall {
     const at::Tensor* t[5];
@@ -520,7 +525,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         auto& p = *reinterpret_cast<sage_append_params*>(&plan->params[0]);
         p.k.ptr = c.t[0]->data_ptr(); p.v.ptr = c.t[1]->data_ptr(); p.k_cache.ptr = c.t[2]->data_ptr(); p.v_cache.ptr = c.t[3]->data_ptr();
         p.slots = c.t[4]->data_ptr();
-        return PyLong_FromLong(sage_cache_append(&p, c10::hip::getCurrentHIPStream(dev.index()).stream()));
+        const int rc = sage_cache_append(&p, c10::hip::getCurrentHIPStream(dev.index()).stream());
+        written(*c.t[2]);
+        written(*c.t[3]);
+        return PyLong_FromLong(rc);
     });
 }
 
@@ -541,7 +549,10 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!plan || !all_ready(c.t, 2, 4, dev)) return none();
         auto& p = *reinterpret_cast<sage_copy_params*>(&plan->params[0]);
         p.k_cache = c.t[0]->data_ptr(); p.v_cache = c.t[1]->data_ptr(); p.src = c.t[2]->data_ptr(); p.dst = c.t[3]->data_ptr();
-        return PyLong_FromLong(sage_cache_copy_pages(&p, c10::hip::getCurrentHIPStream(dev.index()).stream()));
+        const int rc = sage_cache_copy_pages(&p, c10::hip::getCurrentHIPStream(dev.index()).stream());
+        written(*c.t[0]);
+        written(*c.t[1]);
+        return PyLong_FromLong(rc);
     });
 }
 

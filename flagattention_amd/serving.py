@@ -35,6 +35,12 @@ def _no_grad(what, *tensors):
         raise NotImplementedError(f"{what}: tangents of forward-mode differentiation are not carried on")
 
 
+def _written(*tensors):
+    """Autograd's notice of tensors that a kernel has changed in place: a graph that kept one for its backward pass then raises
+    instead of using the new contents."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def _same_device(device, **tensors):
     for name, t in tensors.items():
         require_gpu(t, name)
@@ -196,6 +202,8 @@ def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fals
                    "sage_flash_varlen_fwd")
         if D < 64:
             o = o[..., :D].contiguous() if out is None else out.copy_(o[..., :D])
+        elif out is not None:
+            _written(out)
     return (o, L) if return_log_normalizer else o
 
 
@@ -272,6 +280,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
         ws = split_workspace(q.device, ws_bytes) if ws_bytes else None
         _lib.check(lib.sage_paged_attn(p, ws.data_ptr() if ws is not None else None, ws_bytes, current_stream_ptr(q.device)),
                    "sage_paged_attn")
+        if out is not None:
+            _written(out)
     return (o, L) if return_log_normalizer else o
 
 
@@ -311,6 +321,7 @@ def append_to_cache(k, v, k_cache, v_cache, slots, tensor_layout="HND"):
         if k is call[0] and v is call[1] and slots is call[4]:  # (nothing was copied)
             _host().put_append(*call, bytes(p))
         _lib.check(_lib.load().sage_cache_append(p, current_stream_ptr(k.device)), "sage_cache_append")
+        _written(k_cache, v_cache)
 
 
 def _page_bytes(t):
@@ -367,3 +378,4 @@ def copy_pages(k_cache, v_cache, src, dst):
         _host().put_copy(*call, bytes(p))
     with device_guard(k_cache.device):
         _lib.check(_lib.load().sage_cache_copy_pages(p, current_stream_ptr(k_cache.device)), "sage_cache_copy_pages")
+        _written(k_cache, v_cache)

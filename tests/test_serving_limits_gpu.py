@@ -276,3 +276,33 @@ def test_tangents_raise_in_calls_of_a_known_shape_too(gpu_device):
             call(lambda t: t)
             with pytest.raises(NotImplementedError, match="tangents"):
                 call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+
+
+def test_autograd_knows_what_was_written(gpu_device):
+    """A graph that keeps a cache or an output for its backward pass raises once the operators have changed it, in first calls and in
+    calls of a known shape; tensors made in inference mode are written as well."""
+    import flag_attn
+
+    q, k, v = (_randn((30, n, 64), torch.bfloat16, gpu_device, i) for i, n in enumerate((4, 2, 2)))
+    cu, slots = _cu((30,), gpu_device), torch.arange(30, device=gpu_device)
+    table, lens = torch.arange(4, dtype=torch.int32, device=gpu_device)[None], torch.tensor([30], dtype=torch.int32, device=gpu_device)
+    w = torch.ones(1, device=gpu_device, requires_grad=True)
+    for i in range(3):
+        kc, vc = (torch.ones(4, 2, 16, 64, dtype=torch.bfloat16, device=gpu_device) for _ in range(2))
+        out, out1 = torch.ones_like(q), torch.ones_like(q[:1])
+        writes = [((kc, vc), lambda: flag_attn.append_to_cache(k, v, kc, vc, slots)), ((kc, vc), lambda: flag_attn.copy_pages(kc, vc, slots[:1], slots[3:4])),
+                  ((out,), lambda: flag_attn.flash_attention_varlen(q, k, v, cu, out=out)),
+                  ((out1,), lambda: flag_attn.paged_attention(q[:1], kc, vc, table, lens, out=out1))]
+        for kept, write in writes:
+            for x in kept:
+                y, version = (w * x.float()).sum() + (w * x).sum(), x._version
+                write()
+                assert x._version > version
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    y.backward()
+        with torch.inference_mode():
+            kc, vc = (torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device=gpu_device) for _ in range(2))
+        for _ in range(2):
+            flag_attn.append_to_cache(k, v, kc, vc, slots)
+            flag_attn.copy_pages(kc, vc, slots[:1], slots[3:4])
+        assert torch.equal(kc.transpose(1, 2).reshape(64, 2, 64)[:30], k) and torch.equal(vc[3], vc[0])
