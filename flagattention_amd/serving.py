@@ -80,11 +80,17 @@ def _rows16(t):
     return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+def _no_overlap(t, name):
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"{name}: entries share memory (an expanded tensor) and cannot be written one by one")
+
+
 def _check_out(out, like):
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError("out must have the shape, dtype and device of q")
     if not _aligned(out):
         raise ValueError("out: rows must be 16-byte aligned, with a unit innermost stride")
+    _no_overlap(out, "out")
 
 
 def _check_heads(hq, hkv, hv):
@@ -305,6 +311,8 @@ def append_to_cache(k, v, k_cache, v_cache, slots, tensor_layout="HND"):
         raise ValueError("heads and head_dim of k, v and the caches should be equal")
     if k.dtype not in DTYPE_CODE or any(t.dtype != k.dtype for t in (v, k_cache, v_cache)):
         raise TypeError("k, v and the caches must share one of torch.float16 / torch.bfloat16 / torch.float32")
+    _no_overlap(k_cache, "k_cache")
+    _no_overlap(v_cache, "v_cache")
     slots = _index_list(slots, "slots")
     if slots.shape[0] != k.shape[0]:
         raise ValueError("slots must have an entry for every token")
@@ -367,8 +375,9 @@ def copy_pages(k_cache, v_cache, src, dst):
             raise ValueError("a page of k_cache or v_cache does not lie in one piece of memory")
         p.page_bytes = nbytes
     for name, t in (("k", k_cache), ("v", v_cache)):
-        if any(s < 0 for s in t.stride()) or (p.pages > 1 and t.stride(1 if layered else 0) * e < p.page_bytes):
+        if p.pages > 1 and t.stride(1 if layered else 0) * e < p.page_bytes:
             raise ValueError(f"{name}_cache: pages overlap")
+        _no_overlap(t, f"{name}_cache")
         setattr(p, f"{name}_cache", t.data_ptr())
         setattr(p, f"{name}_stride_layer", _stride(t, 0) * e if layered else 0)
         setattr(p, f"{name}_stride_page", _stride(t, 1 if layered else 0) * e)

@@ -306,3 +306,30 @@ def test_autograd_knows_what_was_written(gpu_device):
             flag_attn.append_to_cache(k, v, kc, vc, slots)
             flag_attn.copy_pages(kc, vc, slots[:1], slots[3:4])
         assert torch.equal(kc.transpose(1, 2).reshape(64, 2, 64)[:30], k) and torch.equal(vc[3], vc[0])
+
+
+def test_expanded_tensors_are_read_and_not_written(gpu_device):
+    import flag_attn
+
+    q, k, v = (_randn((30, n, 64), torch.bfloat16, gpu_device, i) for i, n in enumerate((4, 2, 2)))
+    cu, slots = _cu((30,), gpu_device), torch.arange(30, device=gpu_device)
+    table, lens = torch.arange(4, dtype=torch.int32, device=gpu_device)[None], torch.tensor([30], dtype=torch.int32, device=gpu_device)
+    kc, vc = (_randn((4, 2, 16, 64), torch.bfloat16, gpu_device, i) for i in (5, 6))
+    # one K/V head, one page, one table row for all: the answers are those of the copies
+    for x, y in ((k[:, :1].expand(30, 2, 64), v), (k, v[:1].expand(30, 2, 64))):
+        assert torch.equal(flag_attn.flash_attention_varlen(q, x, y, cu), flag_attn.flash_attention_varlen(q, x.contiguous(), y.contiguous(), cu))
+    for x in (vc[:1].expand_as(vc), vc[:, :1].expand_as(vc), vc[:, :, :1].expand_as(vc)):
+        assert torch.equal(flag_attn.paged_attention(q[:1], kc, x, table, lens), flag_attn.paged_attention(q[:1], kc, x.contiguous(), table, lens))
+        with pytest.raises(ValueError, match="share memory"):
+            flag_attn.append_to_cache(k, v, kc, x, slots)
+        with pytest.raises(ValueError):
+            flag_attn.copy_pages(kc, x, slots[:1], slots[3:4])
+    both = flag_attn.paged_attention(q[:1].expand(3, 4, 64), kc, vc, table.expand(3, 4), lens.expand(3))
+    assert all(torch.equal(row, flag_attn.paged_attention(q[:1], kc, vc, table, lens)[0]) for row in both)
+    for out in (q[:1].clone().expand_as(q), q[:, :1].clone().expand_as(q)):
+        with pytest.raises(ValueError, match="share memory"):
+            flag_attn.flash_attention_varlen(q, k, v, cu, out=out)
+    with pytest.raises(ValueError, match="share memory"):
+        flag_attn.paged_attention(q[:3], kc, vc, table.expand(3, 4), lens.expand(3), out=q[:1].clone().expand(3, 4, 64))
+    with pytest.raises(ValueError, match="share memory"):
+        flag_attn.copy_pages(kc[None].expand(3, 4, 2, 16, 64), vc[None].expand(3, 4, 2, 16, 64), slots[:1], slots[3:4])
