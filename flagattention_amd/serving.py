@@ -63,17 +63,21 @@ def _index_list(t, name):
     return t.contiguous()
 
 
-def _stride(t, dim):
-    """A dimension of one entry has no stride: what torch keeps there is arbitrary."""
-    return t.stride(dim) if t.shape[dim] > 1 else 0
+def _strides(t):
+    """The strides of a tensor, 0 for a dimension of one entry: what torch keeps there is arbitrary."""
+    shape, strides = t.shape, t.stride()
+    return [s if n > 1 else 0 for n, s in zip(shape, strides)] if 1 in shape else strides
 
 
 def _aligned(t):
     """Rows on 16-byte boundaries that run along the last axis (which the kernels read 16 bytes at a time)."""
     e = t.element_size()
-    if t.data_ptr() % 16 != 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
+    if t.data_ptr() % 16 != 0:
         return False
-    return t.numel() == 0 or all(s * e % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()) if n > 1)
+    if t.is_contiguous() and t.shape[-1] * e % 16 == 0:  # (the common case, decided without walking the strides)
+        return True
+    s = _strides(t)
+    return (s[-1] == 1 or t.shape[-1] == 1) and (t.numel() == 0 or all(x * e % 16 == 0 for x in s[:-1]))
 
 
 def _rows16(t):
@@ -81,7 +85,7 @@ def _rows16(t):
 
 
 def _no_overlap(t, name):
-    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+    if not t.is_contiguous() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
         raise ValueError(f"{name}: entries share memory (an expanded tensor) and cannot be written one by one")
 
 
@@ -106,12 +110,18 @@ def _check_float16s(q, k, v):
 
 
 def _token_desc(t):  # [tokens, heads, head_dim]
-    return _lib.SageTensor(t.data_ptr(), 0, _stride(t, 1), _stride(t, 0))
+    s = _strides(t)
+    return _lib.SageTensor(t.data_ptr(), 0, s[1], s[0])
 
 
 def _cache_desc(t, hnd):
-    head, place = (1, 2) if hnd else (2, 1)
-    return _lib.SageTensor(t.data_ptr(), _stride(t, 0), _stride(t, head), _stride(t, place))
+    s = _strides(t)
+    return _lib.SageTensor(t.data_ptr(), s[0], s[1] if hnd else s[2], s[2] if hnd else s[1])
+
+
+def _row_desc(t):  # [sequences, heads, head_dim] or [sequences, new tokens, heads, head_dim]
+    s = _strides(t)
+    return _lib.SageTensor(t.data_ptr(), s[0], s[-2], s[1] if len(s) == 4 else 0)
 
 
 def _layout(tensor_layout):
@@ -270,7 +280,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
             o.fill_(0)
             return (o, L.fill_(-math.inf)) if return_log_normalizer else o
         p = _lib.PagedParams()
-        p.q, p.out = (_lib.SageTensor(t.data_ptr(), _stride(t, 0), _stride(t, t.dim() - 2), _stride(t, 1) if t.dim() == 4 else 0) for t in (q, o))
+        p.q, p.out = _row_desc(q), _row_desc(o)
         p.k_cache, p.v_cache = _cache_desc(k_cache, hnd), _cache_desc(v_cache, hnd)
         p.log_normalizer = L.data_ptr() if L is not None else None
         p.block_table, p.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
@@ -379,8 +389,9 @@ def copy_pages(k_cache, v_cache, src, dst):
             raise ValueError(f"{name}_cache: pages overlap")
         _no_overlap(t, f"{name}_cache")
         setattr(p, f"{name}_cache", t.data_ptr())
-        setattr(p, f"{name}_stride_layer", _stride(t, 0) * e if layered else 0)
-        setattr(p, f"{name}_stride_page", _stride(t, 1 if layered else 0) * e)
+        strides = _strides(t)
+        setattr(p, f"{name}_stride_layer", strides[0] * e if layered else 0)
+        setattr(p, f"{name}_stride_page", strides[1 if layered else 0] * e)
     p.src, p.src_int64 = src.data_ptr(), 1 if src.dtype == torch.int64 else 0
     p.dst, p.dst_int64 = dst.data_ptr(), 1 if dst.dtype == torch.int64 else 0
     if src is call[2] and dst is call[3]:  # (nothing was copied)
