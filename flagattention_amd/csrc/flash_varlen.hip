@@ -538,10 +538,12 @@ __global__ __launch_bounds__(kVarThreads, KEYS == 64 ? 2 : 3) void flash_varlen_
     // loop: 48 prompts of 1 to 700 tokens, H32/8 D128, 43.5 us instead of 42.1.)
     // So they are where a reference point is huge, or was: infinite P leave a NaN sum then, though neither Q nor K holds one.
     auto any_odd = [&](const VT* base, int64_t stride, int first, int end) {
+        // (the lane anew in tiles of 32 keys: kept through the steps it is spilled)
+        const int me = KEYS == 32 ? __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)) : lane;
         unsigned odd = 0;
 #pragma unroll 1
-        for (int n = first + lane / CPR; n < end; n += 64 / CPR) {
-            const v4i f = *reinterpret_cast<const v4i*>(base + (int64_t)n * stride + 8 * (lane % CPR));
+        for (int n = first + me / CPR; n < end; n += 64 / CPR) {
+            const v4i f = *reinterpret_cast<const v4i*>(base + (int64_t)n * stride + 8 * (me % CPR));
 #pragma unroll
             for (int w = 0; w < 4; w++) odd |= nonfinite_halves<VT>((unsigned)f[w]);
         }

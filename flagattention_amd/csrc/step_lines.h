@@ -38,8 +38,8 @@ struct Steps {
         : M(m), N(n), nb((m + (1 << tokens_shift) - 1) >> tokens_shift), shift(tokens_shift), causal(causal_) {}
     __host__ __device__ int end(int j) const { return causal ? min((j + 1) << shift, M) + N - M : N; }  // keys that block j sees (0 or less: none)
     __host__ __device__ int tiles(int j) const { return max((end(j) + kVarKeys - 1) / kVarKeys, 1); }
-    // 1 + 2 + .. + n modulo 2^32: the even one of n and n + 1 is halved before the product
-    __host__ __device__ static unsigned triangle(unsigned n) { return n & 1 ? (n + 1) / 2 * n : n / 2 * (n + 1); }
+    // 1 + 2 + .. + n modulo 2^32: the odd one of n and n + 1 times half of the even one
+    __host__ __device__ static unsigned triangle(unsigned n) { return (n | 1) * ((n + 1) / 2); }
     // tiles of the first j < nb blocks: the first `ones` of them one each, block i of the others ceil(((i + 1) 2^shift + N - M) / 64).
     // (Sums from the sequence's first tile on pass 32 bits where a block sees 3 million keys; modulo 2^32 their differences, which do
     // not, are exact.)
