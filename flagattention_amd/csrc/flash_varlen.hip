@@ -201,6 +201,14 @@ __device__ void careful_row(const VarlenArgs& a, int qt, int h, int hk, int k0, 
 #pragma unroll
         for (int i = 0; i < CH; i++) o[i] *= alpha;
         m = top;
+        // (an output that is NaN stays so: where all of the row's are, only its statistics can still change)
+        bool lost = true;
+#pragma unroll
+        for (int i = 0; i < CH; i++) lost = lost && o[i] != o[i];
+        if (__builtin_amdgcn_ballot_w64(!lost) == 0) {
+            if (!part_o && !a.lse) break;
+            continue;
+        }
 #pragma unroll 1
         for (int j = 0; j < min(64, n - n0); j++) {
             const float pj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j));

@@ -333,3 +333,42 @@ def test_expanded_tensors_are_read_and_not_written(gpu_device):
         flag_attn.paged_attention(q[:3], kc, vc, table.expand(3, 4), lens.expand(3), out=q[:1].clone().expand(3, 4, 64))
     with pytest.raises(ValueError, match="share memory"):
         flag_attn.copy_pages(kc[None].expand(3, 4, 2, 16, 64), vc[None].expand(3, 4, 2, 16, 64), slots[:1], slots[3:4])
+
+
+@pytest.mark.parametrize("heads,seqs", [((4, 2), 1), ((34, 17), 60)])
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_varlen_rows_that_are_nan_throughout(d, dtype, heads, seqs, gpu_device):
+    """All values NaN from some token on, of one head or of all: the rows that see one are NaN in every channel, whatever their log
+    normalizer; those before are as ever."""
+    import flag_attn
+
+    (h, hk), n = heads, 400
+    q, k, v = (_randn((n, x, d), dtype, gpu_device, i) for i, x in enumerate((h, hk, hk)))
+    cu = torch.tensor([0] * seqs + [150, n], dtype=torch.int32, device=gpu_device)
+    v[77:100, 1] = float("nan")
+    v[150 + 201:] = float("nan")
+    o, norm = flag_attn.flash_attention_varlen(q, k, v, cu, causal=True, return_log_normalizer=True)
+    want, want_norm, tol, norm_tol = SO.varlen(q, k, v, cu, cu, True)
+    SO.assert_close(o, want, tol)
+    SO.assert_close(norm, want_norm, norm_tol)
+    alone = flag_attn.flash_attention_varlen(q, k, v, cu, causal=True)
+    SO.assert_close(alone, want, tol)
+    lost = [torch.full_like(x, float("nan")) for x in (q, k, v)]
+    o, norm = flag_attn.flash_attention_varlen(*lost, cu, causal=True, return_log_normalizer=True)
+    assert o.isnan().all() and norm.isnan().all()
+
+
+def test_varlen_parts_that_are_nan_throughout(gpu_device):
+    import flag_attn
+
+    m, n = (70, 33), (4000, 5000)
+    q = _randn((sum(m), 8, 128), torch.bfloat16, gpu_device, 0)
+    k, v = (_randn((sum(n), 2, 128), torch.bfloat16, gpu_device, i) for i in (1, 2))
+    assert _is_cut(q, k, 2, True)
+    v[3960:4000, 0] = float("nan")
+    v[4000 + 4990:, 1] = float("nan")
+    cu_q, cu_k = _cu(m, gpu_device), _cu(n, gpu_device)
+    o, norm = flag_attn.flash_attention_varlen(q, k, v, cu_q, cu_k, True, return_log_normalizer=True)
+    want, want_norm, tol, norm_tol = SO.varlen(q, k, v, cu_q, cu_k, True)
+    SO.assert_close(o, want, tol)
+    SO.assert_close(norm, want_norm, norm_tol)
