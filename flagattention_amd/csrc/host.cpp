@@ -9,8 +9,8 @@
 // function takes the call from the start.  Nothing of a call's data is kept.
 //
 // Host time of a call, Python before -> here: per_block_int8 with smoothing 24.7 -> 6.4 us, sage_attention 12.9 -> 4.0 us, flash_attention 13.6 -> 3.7 us,
-// flash_attention_varlen 12.9 -> 4.2 us, paged_attention 14.9 -> 4.3 us, append_to_cache 10.7 -> 3.7 us, copy_pages 10.3 -> 3.9 us (mostly the
-// launches and the allocation of the outputs).
+// flash_attention_varlen 12.9 -> 3.7 us, paged_attention 15.2 -> 3.8 us, append_to_cache 11.7 -> 2.9 us, copy_pages 10.7 -> 2.9 us (mostly the
+// launches and the allocation of the outputs).  Prompts of a number of tokens that has not been seen pay the former, once.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 

@@ -1,4 +1,4 @@
-// Device helpers shared by the kernels for packed sequences (flash_varlen.hip) and paged caches (paged_attn.hip), gfx950.
+// Device helpers of the kernels for packed sequences (flash_varlen.hip) and paged caches (paged_attn.hip), gfx950.
 #pragma once
 #include <type_traits>
 
@@ -10,7 +10,6 @@ namespace attn {
 namespace {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
 
 // Inclusive scan over the lanes of a wave (0: what joins nothing), by lane moves inside the vector unit.
@@ -74,7 +73,7 @@ __device__ __forceinline__ unsigned nonfinite_halves(unsigned w) {
     return (t - 0x00010001u) & ~t & 0x80008000u;
 }
 
-// The eight numbers with zeros for infinities and NaN.
+// (paged_attn.hip) The eight numbers with zeros for infinities and NaN.
 template <typename VT>
 __device__ __forceinline__ v4i finite_only(v4i x) {
 #pragma unroll
@@ -85,7 +84,7 @@ __device__ __forceinline__ v4i finite_only(v4i x) {
     return x;
 }
 
-// What the infinities and NaN of a 32-key V tile in LDS add to the outputs of a lane's row (16x16 layout: accumulator i of tile ct is
+// (paged_attn.hip) What the infinities and NaN of a 32-key V tile in LDS add to the outputs of a lane's row (16x16 layout: accumulator i of tile ct is
 // channel 16 ct + 4 quad + i): for every key j < see_end of the tile and every channel that the lane holds.  p: the lane's P of the
 // keys 16 (e / 4) + 4 quad + e % 4.  V row j, chunk c lies at row j * 2 D + 16 (c ^ swizzle(j)).  Slow, and hardly ever called.
 template <int D, typename VT, typename Swizzle>

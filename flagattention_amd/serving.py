@@ -157,7 +157,8 @@ def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fals
 
     Returns ``o`` ``[total_q, H, D]``, or ``(o, log_normalizer)`` with the natural log-sum-exp ``[H, total_q]`` in fp32 (-inf where no
     key is seen).  ``out``: where to write instead of a new tensor.  Rows behind the last sequence are not written: those of
-    ``out`` stay as they were, those of a new tensor and of the log normalizer are undefined.
+    ``out`` stay as they were, those of a new tensor and of the log normalizer are undefined.  The softmax's weights are rounded to
+    16 bits before they multiply V, as in ``flash_attention``; maxima and sums are fp32.
     """
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q
@@ -236,7 +237,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
     cut to it, to 0 where it has no entries or the cache no pages.
 
     Returns ``o`` in the shape of ``q``, or ``(o, log_normalizer)`` with the natural log-sum-exp ``[S, H]`` (``[S, H, M]``) in fp32.
-    ``out``: where to write instead of a new tensor.
+    ``out``: where to write instead of a new tensor.  Roundings as in ``flash_attention_varlen``.
     """
     call = (q, k_cache, v_cache, block_table, seq_lens, sm_scale, tensor_layout, return_log_normalizer)
     if out is None:
