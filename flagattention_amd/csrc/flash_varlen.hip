@@ -18,9 +18,11 @@
 //   of its own.
 // No vector register is spilled (13 to 28 scalar ones, to lanes of vector registers, in the cut forms and the 64-key form at head_dim
 // 128): a reload waits for every tile on its way into LDS, since loads return in order (three reloads per step: 4 documents of 512 to
-// 8192 tokens, H32/8 D128, 593 -> 811 us).  What is rare is therefore kept out of its registers (careful_row).  Workgroups are handed out longest first over all sequences (find_block).
-// Measured (bf16, D128, causal; a library product of 8192^3 reaches 1360 to 1380 TFLOP/s here): those documents 577 to 600 us = 1085 to 1130 TFLOP/s,
-// one sequence of 16384 tokens with H16/2 960 us = 1145, 48 prompts of 1 to 700 tokens 38 us, 200 of 100 to 200 142 us = 4.2 TB/s.
+// 8192 tokens, H32/8 D128, 593 -> 811 us).  What is rare is therefore kept out of its registers (careful_row).  Workgroups are handed
+// out longest first over all sequences (find_block).
+// Measured (bf16, D128, causal; a library product of 8192^3 reaches 1360 to 1380 TFLOP/s here): those documents 577 to 600 us = 1085 to
+// 1130 TFLOP/s, one sequence of 16384 tokens with H16/2 960 us = 1145, 48 prompts of 1 to 700 tokens 39 us, 200 of 100 to 200 142 us =
+// 4.2 TB/s.
 // There a workgroup spends 1.7 us on finding its block, 2.2 on its first tile, 1.3 on every further 64 keys and 1.4 on its output.
 #include <math.h>
 

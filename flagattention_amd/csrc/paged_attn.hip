@@ -6,8 +6,8 @@
 //
 // Bound by the bytes of K and V: the rows of all query heads that share a K/V head (row r = query r / group, head r % group) are
 // multiplied from the same tiles, sixteen by a wave and up to 64 by a workgroup, so that the cache is read from memory once (by two
-// waves beyond 16 rows and four beyond 32, each for itself: 8 new tokens of 4 heads a group 72 us where one takes 57).  A workgroup is four
-// waves.  They share the rows, sixteen each, and then the keys, and a wave walks over its 32-key tiles without a barrier:
+// waves beyond 16 rows and four beyond 32, each for itself: 8 new tokens of 4 heads a group 72 us where one takes 57).  A workgroup is
+// four waves.  They share the rows, sixteen each, and then the keys, and a wave walks over its 32-key tiles without a barrier:
 // S^T = K.Q^T and O^T += V^T.P^T on the 16x16 matrix instructions, K rows straight into the operand, V through the wave's slice of
 // LDS, from where it is read transposed.  The registers of a tile are requested anew as soon as their contents are used up, and the
 // entries of the block table a tile ahead of the rows they lead to.
@@ -17,9 +17,9 @@
 // whatever the lengths are, which only the device knows: the end of one item, whole ones, the beginning of another.  Items that are
 // cut leave partial results, normalized outputs in fp32 and their base-2 log-sum-exps, for a second kernel.
 //
-// Measured (contiguous K and V are read at 5.3 TB/s by attn_decode.hip): 128 sequences of 512 to 2048 tokens, 16 heads, D64, fp16 111 us = 5.2 TB/s; 32
-// of up to 8192, H32/8, D128, bf16 57 us = 4.3 TB/s, 5 of them the second kernel; 2 of 50000 to 65536, H32/4 57 us = 4.15 TB/s, 6 of
-// them the second kernel; one of 300 tokens 9.5 us: a launch, the first tile, and 1.4 us for every further 128 keys.
+// Measured (contiguous K and V are read at 5.3 TB/s by attn_decode.hip): 128 sequences of 512 to 2048 tokens, 16 heads, D64, fp16
+// 111 us = 5.2 TB/s; 32 of up to 8192, H32/8, D128, bf16 57 us = 4.3 TB/s, 5 of them the second kernel; 2 of 50000 to 65536, H32/4
+// 57 us = 4.15 TB/s, 6 of them the second kernel; one of 300 tokens 9.5 us: a launch, the first tile, and 1.4 us for every further 128 keys.
 #include "serve_common.h"
 
 namespace sage {

@@ -84,9 +84,10 @@ __device__ __forceinline__ v4i finite_only(v4i x) {
     return x;
 }
 
-// (paged_attn.hip) What the infinities and NaN of a 32-key V tile in LDS add to the outputs of a lane's row (16x16 layout: accumulator i of tile ct is
-// channel 16 ct + 4 quad + i): for every key j < see_end of the tile and every channel that the lane holds.  p: the lane's P of the
-// keys 16 (e / 4) + 4 quad + e % 4.  V row j, chunk c lies at row j * 2 D + 16 (c ^ swizzle(j)).  Slow, and hardly ever called.
+// (paged_attn.hip) What the infinities and NaN of a 32-key V tile in LDS add to the outputs of a lane's row (16x16 layout: accumulator i
+// of tile ct is channel 16 ct + 4 quad + i): for every key j < see_end of the tile and every channel that the lane holds.  p: the
+// lane's P of the keys 16 (e / 4) + 4 quad + e % 4.  V row j, chunk c lies at row j * 2 D + 16 (c ^ swizzle(j)).  Slow, and hardly ever
+// called.
 template <int D, typename VT, typename Swizzle>
 __device__ __forceinline__ void add_nonfinite(const unsigned char* vtile, Swizzle&& swizzle, typename PV<VT>::vec p, int see_end, v4f (&acc)[D / 16]) {
     const int lane = threadIdx.x & 63, quad = lane >> 4;

@@ -8,7 +8,8 @@ keys and values in pages with the attention of new tokens over it.
 
 Lengths, tables, slots and page lists stay on the device: no call waits for the GPU, and a captured graph follows their present
 values.  Entries that lead nowhere (a negative slot, a page that the cache does not have) move and read nothing.  The cache
-belongs to the caller; these functions allocate outputs and scratch memory only.  Forward only: tensors that require grad raise, and so do those with a tangent.
+belongs to the caller; these functions allocate outputs and scratch memory only.  Forward only: tensors that require grad raise,
+and so do those with a tangent.
 """
 from __future__ import annotations
 

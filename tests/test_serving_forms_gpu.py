@@ -123,3 +123,75 @@ def test_cut_launches_of_many_sequences(heads, d, dtype, seqs, gpu_device):
         want, want_norm, tol, norm_tol = SO.varlen(q, k, v, cu_q, cu_k, causal)
         SO.assert_close(o, want, tol)
         SO.assert_close(norm, want_norm, norm_tol)
+
+
+def _work(seed, device):
+    """A cut packed call and a paged call in shares, on inputs of their own: a function without arguments, and its tensors."""
+    import flag_attn
+
+    q, k, v = (_randn((t, n, 128), torch.bfloat16, device, seed + i) for i, (t, n) in enumerate(((70, 8), (9000, 2), (9000, 2))))
+    cu_q, cu_k = _cu((40, 30), device), _cu((3000, 6000), device)
+    kc, vc, table, lens = _cache((5000 + seed, 900), 2, 16, 128, torch.bfloat16, "HND", device, 1300)
+    q1 = _randn((2, 8, 128), torch.bfloat16, device, seed + 9)
+
+    def work():
+        return (flag_attn.flash_attention_varlen(q, k, v, cu_q, cu_k, True), flag_attn.paged_attention(q1, kc, vc, table, lens))
+
+    return work, (q, q1)
+
+
+def test_two_graphs_at_once(gpu_device):
+    """Two captured graphs, each with partial results of its own, replayed at the same time on two streams, with eager calls between."""
+    works = [_work(10 * i, gpu_device) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in works]
+    for work, _ in works:
+        work()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for work, _ in works:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(work())
+        graphs.append(g)
+    for turn in range(4):
+        for i, (work, inputs) in enumerate(works):
+            for x in inputs:
+                x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(100 * turn + i)))
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for s, g in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+        eager = [work() for work, _ in works]  # (beside the replays)
+        torch.cuda.synchronize()
+        for got, want in zip(outs, eager):
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+
+
+def test_two_threads_at_once(gpu_device):
+    """Calls of the same and of other shapes from two threads, a stream each."""
+    import threading
+
+    works = [_work(20 * i, gpu_device) for i in range(2)]
+    want = [work() for work, _ in works]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    got[i].append(works[i][0]())
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for i in range(2):
+        for res in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
