@@ -9,7 +9,7 @@ call fails loudly if the compiled library is missing.
 """
 from . import sage_attention  # noqa: F401
 from .flash import attention as flash_attention  # noqa: F401
-from .serving import append_to_cache, copy_pages, flash_attention_varlen, paged_attention  # noqa: F401
+from .serving import append_to_cache, copy_pages, flash_attention_varlen, paged_attention, read_cache  # noqa: F401
 
 # Same metadata strings the reference package exposes (src/flag_attn/__init__.py:22-25).
 device = "cuda"
@@ -17,5 +17,5 @@ vendor = "amd"
 vendor_name = "amd"
 backend_info = "hip-gfx950"
 
-__all__ = ["sage_attention", "flash_attention", "flash_attention_varlen", "paged_attention", "append_to_cache", "copy_pages",
+__all__ = ["sage_attention", "flash_attention", "flash_attention_varlen", "paged_attention", "append_to_cache", "read_cache", "copy_pages",
            "device", "vendor", "vendor_name", "backend_info"]

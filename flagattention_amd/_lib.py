@@ -104,6 +104,44 @@ class CopyParams(ctypes.Structure):
     ]
 
 
+SAGE_CODE_INT8, SAGE_CODE_E4M3, SAGE_CODE_NONE = 0, 1, -1
+
+
+class CacheScales(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_stride_page", c_i64), ("k_stride_head", c_i64), ("k_stride_block", c_i64),
+        ("v_stride_page", c_i64), ("v_stride_head", c_i64), ("v_stride_block", c_i64), ("blocks", c_i64),
+        ("codes", c_i32), ("reserved", c_i32),
+    ]
+
+
+class Paged8Params(ctypes.Structure):
+    _fields_ = [("paged", PagedParams), ("scales", CacheScales)]
+
+
+class Append8Params(ctypes.Structure):
+    _fields_ = [("append", AppendParams), ("scales", CacheScales)]
+
+
+class ReadParams(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", SageTensor), ("v_cache", SageTensor), ("k_out", SageTensor), ("v_out", SageTensor),
+        ("block_table", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
+        ("table_stride", c_i64), ("seqs", c_i64), ("total", c_i64), ("heads_kv", c_i64), ("head_dim", c_i64), ("pages", c_i64),
+        ("page_size", c_i64), ("table_width", c_i64),
+        ("out_dtype", c_i32), ("reserved", c_i32), ("scales", CacheScales),
+    ]
+
+
+class Copy8Params(ctypes.Structure):
+    _fields_ = [
+        ("copy", CopyParams), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("k_scale_stride_layer", c_i64), ("k_scale_stride_page", c_i64), ("v_scale_stride_layer", c_i64), ("v_scale_stride_page", c_i64),
+        ("scale_words", c_i64),
+    ]
+
+
 EXPORTS = (
     "sage_per_block_int8",
     "sage_per_block_int8_smooth_k",
@@ -129,6 +167,12 @@ EXPORTS = (
     "sage_paged_attn",
     "sage_cache_append",
     "sage_cache_copy_pages",
+    "sage_paged8_attn_workspace_bytes",
+    "sage_paged8_attn",
+    "sage_cache8_append_workspace_bytes",
+    "sage_cache8_append",
+    "sage_cache_read",
+    "sage_cache8_copy_pages",
     "sage_hip_last_error",
     "sage_hip_abi_version",
 )
@@ -206,6 +250,18 @@ def load():
     lib.sage_cache_append.restype = ctypes.c_int
     lib.sage_cache_copy_pages.argtypes = [ctypes.POINTER(CopyParams), ctypes.c_void_p]
     lib.sage_cache_copy_pages.restype = ctypes.c_int
+    lib.sage_paged8_attn_workspace_bytes.argtypes = [ctypes.POINTER(Paged8Params)]
+    lib.sage_paged8_attn_workspace_bytes.restype = c_i64
+    lib.sage_paged8_attn.argtypes = [ctypes.POINTER(Paged8Params), ctypes.c_void_p, c_i64, ctypes.c_void_p]
+    lib.sage_paged8_attn.restype = ctypes.c_int
+    lib.sage_cache8_append_workspace_bytes.argtypes = [ctypes.POINTER(Append8Params)]
+    lib.sage_cache8_append_workspace_bytes.restype = c_i64
+    lib.sage_cache8_append.argtypes = [ctypes.POINTER(Append8Params), ctypes.c_void_p, c_i64, ctypes.c_void_p]
+    lib.sage_cache8_append.restype = ctypes.c_int
+    lib.sage_cache_read.argtypes = [ctypes.POINTER(ReadParams), ctypes.c_void_p]
+    lib.sage_cache_read.restype = ctypes.c_int
+    lib.sage_cache8_copy_pages.argtypes = [ctypes.POINTER(Copy8Params), ctypes.c_void_p]
+    lib.sage_cache8_copy_pages.restype = ctypes.c_int
     if lib.sage_hip_abi_version() != ABI_VERSION:
         raise ImportError(f"{LIB_PATH}: ABI version {lib.sage_hip_abi_version()} != {ABI_VERSION}; rebuild it")
     _lib = lib
@@ -222,8 +278,9 @@ class _PythonHost:
     def quant(*call):
         return None
 
-    attn = flash = varlen = paged = append = copy = quant
+    attn = flash = varlen = paged = append = copy = paged8 = append8 = read = copy8 = quant
     put_quant = put_attn = put_flash = put_varlen = put_paged = put_append = put_copy = quant
+    put_paged8 = put_append8 = put_read = put_copy8 = quant
 
 
 def host():

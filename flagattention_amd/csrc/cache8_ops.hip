@@ -1,0 +1,547 @@
+// A paged cache of 8-bit codes for gfx950: rows of new tokens quantized into it, tokens read back into packed rows, pages copied with
+// their scales.  All are bound by bytes.
+//
+// Quantizing.  A block's scale is s = a / L, a the largest |x| of the call's tokens for it and head (at least 2^-100), L = 127 or 448, or
+// what it was where that is more and the block goes on; codes are x / s to the nearest, ties to even.  x / s is x times the rounded
+// 1 / s first, off by at most 2^-22 of itself; only where that lies next to the middle between two codes (a wave in sixteen) the
+// remainder x - c s, which is exact in an fma, decides.  Codes that stay when a scale grows are c s_old / s, decided by a remainder in 64 bits.
+#include "cache8_common.h"
+
+namespace sage {
+namespace {
+
+using namespace attn;
+
+constexpr int kOpThreads = 256;
+constexpr int kMostBlock = 1024;     // tokens that share a scale
+constexpr int kScanTokens = 1024;    // calls of up to so many tokens look their slots over instead of mapping them
+constexpr float kSmallest = 0x1p-100f;
+
+__device__ __forceinline__ int64_t index_at(const void* list, int wide, int64_t i) {
+    return wide ? static_cast<const int64_t*>(list)[i] : (int64_t) static_cast<const int32_t*>(list)[i];
+}
+
+// Sixteen entries of a row.
+template <typename T> struct Row16;
+template <typename T> struct Row16_16 {
+    v4i w[2];
+    __device__ __forceinline__ void load(const unsigned char* p) {
+        w[0] = reinterpret_cast<const v4i*>(p)[0];
+        w[1] = reinterpret_cast<const v4i*>(p)[1];
+    }
+    __device__ __forceinline__ void clear() { w[0] = w[1] = v4i{0, 0, 0, 0}; }
+    __device__ __forceinline__ float at(int i) const {
+        const unsigned x = (unsigned)w[i / 8][i % 8 / 2];
+        return (float)__builtin_bit_cast(T, (unsigned short)(i & 1 ? x >> 16 : x));
+    }
+    // the largest absolute value, as the bits of |x| in T: NaN above infinity above the finite ones
+    __device__ __forceinline__ unsigned top(unsigned so_far) const {
+        typedef unsigned short v2s __attribute__((ext_vector_type(2)));
+        v2s m = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(v2s, (unsigned)w[i / 4][i % 4] & 0x7fff7fffu));
+        return max(so_far, max((unsigned)m[0], (unsigned)m[1]));
+    }
+    static __device__ __forceinline__ float size(unsigned top) { return (float)__builtin_bit_cast(T, (unsigned short)top); }
+};
+template <> struct Row16<__bf16> : Row16_16<__bf16> {};
+template <> struct Row16<_Float16> : Row16_16<_Float16> {};
+template <> struct Row16<float> {
+    v4f w[4];
+    __device__ __forceinline__ void load(const unsigned char* p) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = reinterpret_cast<const v4f*>(p)[i];
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __device__ __forceinline__ float at(int i) const { return w[i / 4][i % 4]; }
+    __device__ __forceinline__ unsigned top(unsigned so_far) const {
+#pragma unroll
+        for (int i = 0; i < 16; i++) so_far = max(so_far, __builtin_bit_cast(unsigned, at(i)) & 0x7fffffffu);
+        return so_far;
+    }
+    static __device__ __forceinline__ float size(unsigned top) { return __builtin_bit_cast(float, top); }
+};
+
+// The scale that new rows, whose largest entry has the size `top`, ask for.
+template <typename Code>
+__device__ __forceinline__ float scale_for(float top) {
+    return top < INFINITY ? fmaxf(top, kSmallest) / Code::kLargest : NAN;
+}
+
+// x / s to the nearest integer, ties to even, for |x| <= 127.5 s (codes of int8) or |x| <= 16 s (an e4m3 number in steps of its own): n is
+// next to it or it, and the remainder x - n s exact, a multiple of the last place of s or of x and no larger than s.
+__device__ __forceinline__ float settle(float x, float s, float n) {
+    const float r = __builtin_fmaf(-n, s, x), h = 0.5f * s;
+    const bool odd = ((int)n & 1) != 0;
+    if (r > h || (r == h && odd)) n += 1.0f;
+    if (r < -h || (r == -h && odd)) n -= 1.0f;
+    return n;
+}
+// The same with 64 bits, where x is code * old scale, 31 bits.
+__device__ __forceinline__ double settle(double x, double s, double n) {
+    const double r = __builtin_fma(-n, s, x), h = 0.5 * s;
+    const bool odd = ((int)n & 1) != 0;
+    if (r > h || (r == h && odd)) n += 1.0;
+    if (r < -h || (r == -h && odd)) n -= 1.0;
+    return n;
+}
+
+template <typename Code> struct Rounding;
+template <> struct Rounding<Int8> {
+    // Sixteen codes of x, s > 0 (or inv = 0: codes 0).  x inv + 1.5 2^23 is an integer in its low bits.
+    template <typename Row>
+    static __device__ __forceinline__ v4i codes(const Row& x, float s, float inv) {
+        constexpr float magic = 12582912.0f;
+        float z[16], far = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            z[i] = __builtin_fmaf(x.at(i), inv, magic);
+            far = fmaxf(far, __builtin_fabsf(__builtin_fmaf(x.at(i), inv, -(z[i] - magic))));
+        }
+        if (__builtin_amdgcn_ballot_w64(far > 0.5f - 0x1p-15f) != 0) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) z[i] = settle(x.at(i), s, z[i] - magic) + magic;
+        }
+        v4i w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const unsigned lo = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, z[4 * i + 1]), __builtin_bit_cast(unsigned, z[4 * i]), 0x0c0c0400u);
+            const unsigned hi = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, z[4 * i + 3]), __builtin_bit_cast(unsigned, z[4 * i + 2]), 0x04000c0cu);
+            w[i] = (int)(lo | hi);
+        }
+        return w;
+    }
+    // A word of codes that stand for numbers in units of `was`, in units of s >= was.
+    static __device__ __forceinline__ unsigned again(unsigned w, double was, double s) {
+        const double ratio = was / s;
+        unsigned to = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const double c = (double)(int8_t)(w >> (8 * i));
+            const double n = settle(c * was, s, __builtin_rint(c * ratio));
+            to |= ((unsigned)(int)n & 255u) << (8 * i);
+        }
+        return to;
+    }
+};
+template <> struct Rounding<E4m3> {
+    // The step between e4m3 numbers around y: 2^-3 of its power of two, at least 2^-9.
+    static __device__ __forceinline__ float step(float y) {
+        return __builtin_amdgcn_ldexpf(1.0f, max(__builtin_amdgcn_frexp_expf(y) - 1, -6) - 3);
+    }
+    template <typename Row>
+    static __device__ __forceinline__ v4i codes(const Row& x, float s, float inv) {
+        float y[16];
+        unsigned close = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            y[i] = x.at(i) * inv;
+            // Next to the middle between two numbers (the 20 bits that are rounded away are 2^19, or some less or more), or among the small
+            // numbers, whose steps are all the same, and not zero.
+            const unsigned b = __builtin_bit_cast(unsigned, y[i]) & 0x7fffffffu;
+            close |= ((b - 0x7fff8u) & 0xfffffu) <= 16 || b - 1 < 0x3c7fffffu ? 1 : 0;
+        }
+        if (__builtin_amdgcn_ballot_w64(close != 0) != 0) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float u = step(y[i]);
+                y[i] = inv != 0.0f ? settle(x.at(i), s * u, __builtin_rintf(y[i] / u)) * u : 0.0f;
+            }
+        }
+        v4i w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            int z = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
+            w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], z, true);
+        }
+        return w;
+    }
+    static __device__ __forceinline__ unsigned again(unsigned w, double was, double s) {
+        const double ratio = was / s;
+        const v2i h = E4m3::halves(w);
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const double c = (double)__builtin_bit_cast(_Float16, (unsigned short)((unsigned)h[i / 2] >> (16 * (i & 1))));
+            const double u = step((float)(c * ratio));
+            y[i] = (float)(settle(c * was, s * u, __builtin_rint(c * ratio / u)) * u);
+        }
+        int z = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], z, true);
+    }
+};
+
+struct WriteArgs {
+    const unsigned char* src[2];  // k, v
+    unsigned char* dst[2];        // caches
+    int64_t ss_t[2], ss_h[2], ds_p[2], ds_h[2], ds_n[2];  // bytes
+    BlockScales scales;
+    const void* slots;
+    int32_t* map;  // [slots of the cache]: token that goes there, where that token's slot says so too; null: few tokens
+    int64_t slot_limit, rows;  // rows: tokens * heads
+    int32_t wide, tokens, page_size, heads, pieces, group;  // pieces: of 16 entries, of a row; group: tokens a workgroup looks at
+};
+
+__device__ __forceinline__ float& scale_of(const WriteArgs& a, int x, int64_t page, int h, int block) {
+    return x ? a.scales.v[page * a.scales.v_p + h * a.scales.v_h + block * a.scales.v_b]
+             : a.scales.k[page * a.scales.k_p + h * a.scales.k_h + block * a.scales.k_b];
+}
+
+// A scale for every token: LPR lanes take a row of k and the same one of v, 16 entries each.
+template <int LPR, typename T, typename Code>
+__global__ __launch_bounds__(kOpThreads) void cache8_write_rows_kernel(WriteArgs a) {
+    const int64_t row = ((int64_t)blockIdx.x * kOpThreads + threadIdx.x) / LPR;
+    const int c = threadIdx.x % LPR;
+    int64_t slot = -1, t = 0;
+    int h = 0;
+    if (row < a.rows) {
+        t = row / a.heads;
+        h = (int)(row - t * a.heads);
+        slot = index_at(a.slots, a.wide, t);
+    }
+    const bool ok = slot >= 0 && slot < a.slot_limit, mine = ok && c < a.pieces;
+    const int64_t page = ok ? slot / a.page_size : 0;
+    const int place = ok ? (int)(slot - page * a.page_size) : 0;
+    Row16<T> x[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if (mine) x[i].load(a.src[i] + t * a.ss_t[i] + h * a.ss_h[i] + c * (16 * (int)sizeof(T)));
+        else x[i].clear();
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        unsigned top = x[i].top(0);
+#pragma unroll
+        for (int d = 1; d < LPR; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
+        const float s = scale_for<Code>(Row16<T>::size(top));
+        const float inv = s < INFINITY ? 1.0f / s : 0.0f;
+        if (!(s < INFINITY)) x[i].clear();  // (NaN: an entry was not finite)
+        const v4i w = Rounding<Code>::codes(x[i], s, inv);
+        if (mine) *reinterpret_cast<v4i*>(a.dst[i] + page * a.ds_p[i] + h * a.ds_h[i] + place * a.ds_n[i] + 16 * c) = w;
+        if (mine && c == 0) scale_of(a, i, page, h, place) = s;
+    }
+}
+
+__global__ __launch_bounds__(kOpThreads) void cache8_map_kernel(WriteArgs a) {
+    const int t = blockIdx.x * kOpThreads + threadIdx.x;
+    if (t >= a.tokens) return;
+    const int64_t slot = index_at(a.slots, a.wide, t);
+    if (slot >= 0 && slot < a.slot_limit) a.map[slot] = t;
+}
+
+// Blocks of several tokens.  A workgroup looks at `group` tokens; the one with the lowest place of those of the call that go to a block
+// takes care of the block: its tokens are looked for among all of them (SCAN) or through the map, which is not cleared before, since an entry counts
+// only where its token's slot leads back to it.  A wave takes a head of K or of V.
+template <int LPR, typename T, typename Code, bool SCAN>
+__global__ __launch_bounds__(kOpThreads) void cache8_write_blocks_kernel(WriteArgs a) {
+    constexpr int ROWS = 64 / LPR, KEEP = 4;  // rows of a step; steps whose rows are kept in registers
+    __shared__ int token[kMostBlock];
+    __shared__ int lowest;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int block = a.scales.block;
+    const int rr = lane / LPR, c = lane % LPR;
+    for (int g = 0; g < a.group; g++) {
+        const int64_t t = (int64_t)blockIdx.x * a.group + g;
+        if (t >= a.tokens) return;
+        const int64_t slot = index_at(a.slots, a.wide, t);
+        if (slot < 0 || slot >= a.slot_limit) continue;
+        const int64_t page = slot / a.page_size;
+        const int place = (int)(slot - page * a.page_size), b = a.scales.of(place);
+        // (the token before it goes to the place before its own: that one, or one before it, takes care)
+        if (place != b * block && t > 0 && index_at(a.slots, a.wide, t - 1) == slot - 1) continue;
+        const int64_t base = page * a.page_size + (int64_t)b * block;
+        __syncthreads();  // (the tokens of the block before have been read)
+        for (int p = tid; p < block; p += kOpThreads) {
+            int who = -1;
+            if (!SCAN) {
+                who = a.map[base + p];
+                if (who < 0 || who >= a.tokens || index_at(a.slots, a.wide, who) != base + p) who = -1;
+            }
+            token[p] = who;
+        }
+        if (tid == 0) lowest = block;
+        __syncthreads();
+        if (SCAN) {
+            for (int i = tid; i < a.tokens; i += kOpThreads) {
+                const int64_t d = index_at(a.slots, a.wide, i) - base;
+                if (d >= 0 && d < block) atomicMax(&token[d], i);  // (slots that occur twice: the last one)
+            }
+            __syncthreads();
+        }
+        for (int p = tid; p < block; p += kOpThreads)
+            if (token[p] >= 0) atomicMin(&lowest, p);
+        __syncthreads();
+        if (token[lowest] != t) continue;
+        const bool begun = lowest == 0;
+        for (int unit = blockIdx.y * (kOpThreads / 64) + wave; unit < 2 * a.heads; unit += gridDim.y * (kOpThreads / 64)) {
+            const int x = unit & 1, h = unit >> 1;
+            const unsigned char* src = a.src[x] + h * a.ss_h[x] + c * (16 * (int)sizeof(T));
+            unsigned char* dst = a.dst[x] + page * a.ds_p[x] + h * a.ds_h[x] + (int64_t)b * block * a.ds_n[x] + 16 * c;
+            Row16<T> rows[KEEP];
+            int who[KEEP];
+            auto load = [&](int p0) {  // rows of places p0 ..; who: their tokens, -1: none, -2: no such place
+#pragma unroll
+                for (int e = 0; e < KEEP; e++) {
+                    const int p = p0 + e * ROWS + rr;
+                    who[e] = p < block && c < a.pieces ? token[p] : -2;
+                    if (who[e] >= 0) rows[e].load(src + who[e] * a.ss_t[x]);
+                    else rows[e].clear();
+                }
+            };
+            unsigned top = 0;
+            for (int p0 = 0; p0 < block; p0 += KEEP * ROWS) {
+                load(p0);
+#pragma unroll
+                for (int e = 0; e < KEEP; e++) top = rows[e].top(top);
+            }
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
+            const float asked = scale_for<Code>(Row16<T>::size(top));
+            const float was = begun ? 0.0f : scale_of(a, x, page, h, b);
+            const float s = was >= asked || was != was ? was : asked;
+            const float inv = s < INFINITY ? 1.0f / s : 0.0f;
+            const bool grown = s != was && s == s;
+            for (int p0 = 0; p0 < block; p0 += KEEP * ROWS) {
+                if (block > KEEP * ROWS) load(p0);
+#pragma unroll
+                for (int e = 0; e < KEEP; e++) {
+                    v4i* to = reinterpret_cast<v4i*>(dst + (p0 + e * ROWS + rr) * a.ds_n[x]);
+                    if (!(s < INFINITY)) rows[e].clear();  // (NaN: an entry was not finite)
+                    const v4i w = Rounding<Code>::codes(rows[e], s, inv);
+                    if (who[e] >= 0 || (who[e] == -1 && begun)) *to = w;  // (zeros where a block begins)
+                    else if (who[e] == -1 && grown) {
+                        v4i old = *to;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) old[i] = (int)Rounding<Code>::again((unsigned)old[i], was, s);
+                        *to = old;
+                    }
+                }
+            }
+            if (lane == 0) scale_of(a, x, page, h, b) = s;
+        }
+    }
+}
+
+// Packed rows of sequences from the pages of a cache.  A workgroup takes kReadRows rows: one search over the sequences for the first,
+// the others go on from there.
+constexpr int kReadRows = 16;
+
+struct ReadArgs {
+    const unsigned char* src[2];  // caches
+    unsigned char* dst[2];
+    int64_t ss_p[2], ss_h[2], ss_n[2], ds_t[2], ds_h[2];  // bytes
+    BlockScales scales;
+    const int32_t* table;
+    const int32_t* cu;
+    int64_t table_stride, capacity;
+    int32_t seqs, total, page_size, pages, heads, pieces;  // pieces: of 8 codes, or 16 bytes, of a row
+};
+
+// OutT: codes become numbers of it; Code void: 16 bytes of a row are copied.
+template <typename OutT, typename Code>
+__global__ __launch_bounds__(kOpThreads) void cache_read_kernel(ReadArgs a) {
+    __shared__ int page_of[kReadRows], place_of[kReadRows];  // page -1: a row of zeros, -2: no row
+    __shared__ int ends;
+    const int tid = threadIdx.x, t0 = blockIdx.x * kReadRows;
+    if (tid == 0) ends = 0;
+    __syncthreads();
+    int before = 0;  // sequences that end at or before row t0
+    for (int s = tid; s < a.seqs; s += kOpThreads) before += a.cu[s + 1] <= t0 ? 1 : 0;
+    if (before) atomicAdd(&ends, before);
+    __syncthreads();
+    if (tid < kReadRows) {
+        const int t = t0 + tid;
+        int seq = ends;
+        while (seq < a.seqs && a.cu[seq + 1] <= t) seq++;
+        int page = -2, place = 0;
+        if (t < a.total && seq < a.seqs) {
+            const int64_t pos = (int64_t)t - a.cu[seq];
+            page = pos >= 0 ? -1 : -2;
+            if (pos >= 0 && pos < a.capacity) {
+                const int64_t e = pos / a.page_size;
+                place = (int)(pos - e * a.page_size);
+                const int p = a.table[seq * a.table_stride + e];
+                if (p >= 0 && p < a.pages) page = p;
+            }
+        }
+        page_of[tid] = page;
+        place_of[tid] = place;
+    }
+    __syncthreads();
+    const int per_row = a.heads * a.pieces;
+    for (int i = tid; i < kReadRows * per_row; i += kOpThreads) {
+        const int r = i / per_row, q = i - r * per_row, h = q / a.pieces, c = q - h * a.pieces;
+        const int64_t page = page_of[r];
+        const int place = place_of[r];
+        if (page == -2) continue;
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            unsigned char* to = a.dst[x] + (int64_t)(t0 + r) * a.ds_t[x] + h * a.ds_h[x];
+            const unsigned char* from = a.src[x] + page * a.ss_p[x] + h * a.ss_h[x] + place * a.ss_n[x];
+            if constexpr (std::is_same<Code, void>::value) {
+                *reinterpret_cast<v4i*>(to + 16 * c) = page >= 0 ? *reinterpret_cast<const v4i*>(from + 16 * c) : v4i{0, 0, 0, 0};
+            } else {
+                typedef OutT v8 __attribute__((ext_vector_type(8)));
+                v8 out = {};
+                if (page >= 0) {
+                    const BlockScales& b = a.scales;
+                    const float s = x ? b.v[page * b.v_p + h * b.v_h + b.of(place) * b.v_b] : b.k[page * b.k_p + h * b.k_h + b.of(place) * b.k_b];
+                    const f16x8 codes = to_f16<Code>(*reinterpret_cast<const v2i*>(from + 8 * c));
+#pragma unroll
+                    for (int j = 0; j < 8; j++) out[j] = (OutT)((float)codes[j] * s);
+                }
+                *reinterpret_cast<v8*>(to + 8 * c * (int)sizeof(OutT)) = out;
+            }
+        }
+    }
+}
+
+struct Copy8Args {
+    unsigned char* cache[2];
+    float* scale[2];
+    int64_t stride_l[2], stride_p[2];    // bytes
+    int64_t sstride_l[2], sstride_p[2];  // floats
+    const void* src;
+    const void* dst;
+    int64_t pages;
+    int32_t src_wide, dst_wide, page_pieces, count, words;
+};
+
+constexpr int kCopyPieces = 4;  // per thread, on their way together
+
+// blockIdx: part of a page, pair, layer * 2 + cache; the first part of a page copies its scales too
+__global__ __launch_bounds__(kOpThreads) void cache8_copy_kernel(Copy8Args a) {
+    const int which = blockIdx.z & 1;
+    const int64_t layer = blockIdx.z >> 1;
+    const int first = blockIdx.x * (kOpThreads * kCopyPieces) + threadIdx.x;
+    for (int i = blockIdx.y; i < a.count; i += gridDim.y) {
+        const int64_t from = index_at(a.src, a.src_wide, i), to = index_at(a.dst, a.dst_wide, i);
+        if (from < 0 || from >= a.pages || to < 0 || to >= a.pages) continue;
+        unsigned char* base = a.cache[which] + layer * a.stride_l[which];
+        const v4i* s = reinterpret_cast<const v4i*>(base + from * a.stride_p[which]);
+        v4i* d = reinterpret_cast<v4i*>(base + to * a.stride_p[which]);
+        v4i x[kCopyPieces];
+#pragma unroll
+        for (int e = 0; e < kCopyPieces; e++)
+            if (first + e * kOpThreads < a.page_pieces) x[e] = s[first + e * kOpThreads];
+        if (blockIdx.x == 0) {
+            float* scale = a.scale[which] + layer * a.sstride_l[which];
+            for (int w = threadIdx.x; w < a.words; w += kOpThreads) scale[to * a.sstride_p[which] + w] = scale[from * a.sstride_p[which] + w];
+        }
+#pragma unroll
+        for (int e = 0; e < kCopyPieces; e++)
+            if (first + e * kOpThreads < a.page_pieces) d[first + e * kOpThreads] = x[e];
+    }
+}
+
+bool maps_tokens(const sage_append8_params& p) { return p.scales.blocks != p.append.page_size && p.append.tokens > kScanTokens; }
+
+}  // namespace
+
+int64_t append8_workspace_bytes(const sage_append8_params& p) { return maps_tokens(p) ? p.append.pages * p.append.page_size * (int64_t)sizeof(int32_t) : 0; }
+
+template <int LPR, typename T, typename Code>
+static int launch_write(WriteArgs a, hipStream_t stream) {
+    if (a.scales.block == 1) {
+        const int64_t wgs = (a.rows * LPR + kOpThreads - 1) / kOpThreads;
+        if (wgs > kMaxThreads / kOpThreads) return fail(SAGE_E_UNSUPPORTED, "sage_cache8_append: too many rows for one launch");
+        hipLaunchKernelGGL((cache8_write_rows_kernel<LPR, T, Code>), dim3((unsigned)wgs), dim3(kOpThreads), 0, stream, a);
+        return check_launch("cache8_write_rows_kernel");
+    }
+    const int units = (2 * a.heads + kOpThreads / 64 - 1) / (kOpThreads / 64);
+    a.group = a.map ? 16 : 1;
+    const dim3 grid((unsigned)((a.tokens + a.group - 1) / a.group), (unsigned)(units < 65535 ? units : 65535));
+    if ((int64_t)grid.x > kMaxThreads / kOpThreads) return fail(SAGE_E_UNSUPPORTED, "sage_cache8_append: too many rows for one launch");
+    if (a.map) {
+        hipLaunchKernelGGL(cache8_map_kernel, dim3((unsigned)((a.tokens + kOpThreads - 1) / kOpThreads)), dim3(kOpThreads), 0, stream, a);
+        if (int rc = check_launch("cache8_map_kernel")) return rc;
+        hipLaunchKernelGGL((cache8_write_blocks_kernel<LPR, T, Code, false>), grid, dim3(kOpThreads), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((cache8_write_blocks_kernel<LPR, T, Code, true>), grid, dim3(kOpThreads), 0, stream, a);
+    }
+    return check_launch("cache8_write_blocks_kernel");
+}
+
+template <typename T, typename Code>
+static int launch_write(const WriteArgs& a, hipStream_t stream) {
+    if (a.pieces <= 4) return launch_write<4, T, Code>(a, stream);
+    if (a.pieces <= 8) return launch_write<8, T, Code>(a, stream);
+    if (a.pieces <= 16) return launch_write<16, T, Code>(a, stream);
+    return launch_write<32, T, Code>(a, stream);
+}
+
+template <typename Code>
+static int launch_write(const WriteArgs& a, int dtype, hipStream_t stream) {
+    return dtype == SAGE_BF16 ? launch_write<__bf16, Code>(a, stream) : dtype == SAGE_F16 ? launch_write<_Float16, Code>(a, stream)
+                                                                                          : launch_write<float, Code>(a, stream);
+}
+
+int launch_cache8_append(const sage_append8_params& p8, void* workspace, hipStream_t stream) {
+    const sage_append_params& p = p8.append;
+    WriteArgs a{};
+    const sage_tensor* src[2] = {&p.k, &p.v};
+    const sage_tensor* dst[2] = {&p.k_cache, &p.v_cache};
+    const int64_t e = dtype_bytes(p.dtype);
+    for (int x = 0; x < 2; x++) {
+        a.src[x] = (const unsigned char*)src[x]->ptr; a.ss_t[x] = e * src[x]->stride_n; a.ss_h[x] = e * src[x]->stride_h;
+        a.dst[x] = (unsigned char*)dst[x]->ptr; a.ds_p[x] = dst[x]->stride_b; a.ds_h[x] = dst[x]->stride_h; a.ds_n[x] = dst[x]->stride_n;
+    }
+    a.scales = block_scales(p8.scales, p.page_size);
+    a.slots = p.slots; a.wide = p.slots_int64 ? 1 : 0;
+    a.map = maps_tokens(p8) ? (int32_t*)workspace : nullptr;
+    a.slot_limit = p.pages * p.page_size; a.rows = p.tokens * p.heads_kv;
+    a.tokens = (int)p.tokens; a.page_size = (int)p.page_size; a.heads = (int)p.heads_kv; a.pieces = (int)(p.head_dim / 16);
+    return p8.scales.codes == SAGE_CODE_INT8 ? launch_write<Int8>(a, p.dtype, stream) : launch_write<E4m3>(a, p.dtype, stream);
+}
+
+template <typename Code>
+static void launch_read(const ReadArgs& a, int dtype, dim3 grid, hipStream_t stream) {
+    if (dtype == SAGE_BF16) hipLaunchKernelGGL((cache_read_kernel<__bf16, Code>), grid, dim3(kOpThreads), 0, stream, a);
+    else if (dtype == SAGE_F16) hipLaunchKernelGGL((cache_read_kernel<_Float16, Code>), grid, dim3(kOpThreads), 0, stream, a);
+    else hipLaunchKernelGGL((cache_read_kernel<float, Code>), grid, dim3(kOpThreads), 0, stream, a);
+}
+
+int launch_cache_read(const sage_read_params& p, hipStream_t stream) {
+    ReadArgs a{};
+    const sage_tensor* src[2] = {&p.k_cache, &p.v_cache};
+    const sage_tensor* dst[2] = {&p.k_out, &p.v_out};
+    const bool coded = p.scales.codes != SAGE_CODE_NONE;
+    const int64_t e = dtype_bytes(p.out_dtype), ce = coded ? 1 : e;
+    for (int x = 0; x < 2; x++) {
+        a.src[x] = (const unsigned char*)src[x]->ptr; a.ss_p[x] = ce * src[x]->stride_b; a.ss_h[x] = ce * src[x]->stride_h; a.ss_n[x] = ce * src[x]->stride_n;
+        a.dst[x] = (unsigned char*)dst[x]->ptr; a.ds_t[x] = e * dst[x]->stride_n; a.ds_h[x] = e * dst[x]->stride_h;
+    }
+    if (coded) a.scales = block_scales(p.scales, p.page_size);
+    a.table = p.block_table; a.cu = p.cu_seqlens; a.table_stride = p.table_stride;
+    a.capacity = p.pages > 0 ? p.table_width * p.page_size : 0;
+    a.seqs = (int)p.seqs; a.total = (int)p.total; a.page_size = (int)p.page_size; a.pages = (int)p.pages; a.heads = (int)p.heads_kv;
+    a.pieces = (int)(coded ? p.head_dim / 8 : p.head_dim * e / 16);
+    const dim3 grid((unsigned)((p.total + kReadRows - 1) / kReadRows));
+    if ((int64_t)grid.x > kMaxThreads / kOpThreads) return fail(SAGE_E_UNSUPPORTED, "sage_cache_read: too many rows for one launch");
+    if (p.scales.codes == SAGE_CODE_INT8) launch_read<Int8>(a, p.out_dtype, grid, stream);
+    else if (coded) launch_read<E4m3>(a, p.out_dtype, grid, stream);
+    else hipLaunchKernelGGL((cache_read_kernel<float, void>), grid, dim3(kOpThreads), 0, stream, a);
+    return check_launch("cache_read_kernel");
+}
+
+int launch_cache8_copy(const sage_copy8_params& p8, hipStream_t stream) {
+    const sage_copy_params& p = p8.copy;
+    Copy8Args a{};
+    a.cache[0] = (unsigned char*)p.k_cache; a.cache[1] = (unsigned char*)p.v_cache;
+    a.stride_l[0] = p.k_stride_layer; a.stride_l[1] = p.v_stride_layer;
+    a.stride_p[0] = p.k_stride_page; a.stride_p[1] = p.v_stride_page;
+    a.scale[0] = p8.k_scale; a.scale[1] = p8.v_scale;
+    a.sstride_l[0] = p8.k_scale_stride_layer; a.sstride_l[1] = p8.v_scale_stride_layer;
+    a.sstride_p[0] = p8.k_scale_stride_page; a.sstride_p[1] = p8.v_scale_stride_page;
+    a.src = p.src; a.dst = p.dst; a.src_wide = p.src_int64 ? 1 : 0; a.dst_wide = p.dst_int64 ? 1 : 0;
+    a.pages = p.pages; a.page_pieces = (int)(p.page_bytes / 16); a.count = (int)p.count; a.words = (int)p8.scale_words;
+    const int parts = (a.page_pieces + kOpThreads * kCopyPieces - 1) / (kOpThreads * kCopyPieces);
+    const unsigned pairs = (unsigned)(p.count < 65535 ? p.count : 65535);
+    hipLaunchKernelGGL(cache8_copy_kernel, dim3((unsigned)parts, pairs, (unsigned)(2 * p.layers)), dim3(kOpThreads), 0, stream, a);
+    return check_launch("cache8_copy_kernel");
+}
+
+}  // namespace sage

@@ -329,7 +329,8 @@ extern "C" int sage_flash_varlen_fwd(const sage_varlen_params* p, void* workspac
     return nothing ? SAGE_OK : launch_flash_varlen(*p, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-static int check_paged(const char* who, const sage_paged_params* p, bool& nothing) {
+// e: bytes of an entry of the caches
+static int check_paged(const char* who, const sage_paged_params* p, bool& nothing, int e = 2) {
     nothing = false;
     if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
     if (int rc = check_heads(who, p->heads_q, p->heads_kv, p->head_dim, p->dtype, p->sm_scale)) return rc;
@@ -346,7 +347,7 @@ static int check_paged(const char* who, const sage_paged_params* p, bool& nothin
         return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30", who);
     if (p->seqs * (p->new_tokens * (p->heads_q / p->heads_kv)) >= (1LL << 40))
         return fail(SAGE_E_UNSUPPORTED, "%s: seqs x new_tokens x heads_q / heads_kv must stay below 2^40", who);
-    if (misaligned_row(p->q, 2) || misaligned_row(p->out, 2) || misaligned_row(p->k_cache, 2) || misaligned_row(p->v_cache, 2))
+    if (misaligned_row(p->q, 2) || misaligned_row(p->out, 2) || misaligned_row(p->k_cache, e) || misaligned_row(p->v_cache, e))
         return fail(SAGE_E_INVALID, "%s: rows of q, out and the caches must be 16-byte aligned", who);
     if (p->k_cache.stride_n < 0 || p->v_cache.stride_n < 0 || p->k_cache.stride_n >= (1LL << 27) || p->v_cache.stride_n >= (1LL << 27))
         return fail(SAGE_E_UNSUPPORTED, "%s: token stride of a cache out of range for 32-bit offsets within 16 tokens", who);
@@ -366,8 +367,9 @@ extern "C" int sage_paged_attn(const sage_paged_params* p, void* workspace, int6
     return nothing ? SAGE_OK : launch_paged_attn(*p, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-extern "C" int sage_cache_append(const sage_append_params* p, void* stream) {
-    const char* who = "sage_cache_append";
+// ce: bytes of an entry of the caches, 0: those of dtype
+static int check_append(const char* who, const sage_append_params* p, bool& nothing, int ce = 0) {
+    nothing = false;
     if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
     if (!float_dtype_ok(p->dtype)) return fail(SAGE_E_INVALID, "%s: bad dtype %d", who, p->dtype);
     if (p->tokens < 0 || p->heads_kv < 0 || p->head_dim < 0 || p->pages < 0) return fail(SAGE_E_INVALID, "%s: negative size", who);
@@ -376,22 +378,130 @@ extern "C" int sage_cache_append(const sage_append_params* p, void* stream) {
     const int64_t lim = 1LL << 30;
     if (p->tokens >= lim || p->pages >= lim || p->page_size >= lim || p->heads_kv > (1 << 16) || p->head_dim > (1 << 12))
         return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30, heads_kv at most 65536, head_dim at most 4096", who);
-    if (p->tokens == 0 || p->heads_kv == 0 || p->head_dim == 0 || p->pages == 0) return SAGE_OK;
+    nothing = p->tokens == 0 || p->heads_kv == 0 || p->head_dim == 0 || p->pages == 0;
+    if (nothing) return SAGE_OK;
     if (!p->k.ptr || !p->v.ptr || !p->k_cache.ptr || !p->v_cache.ptr || !p->slots) return fail(SAGE_E_INVALID, "%s: null pointer", who);
-    if (p->head_dim * e % 16 != 0 || misaligned_row(p->k, e) || misaligned_row(p->v, e) || misaligned_row(p->k_cache, e) || misaligned_row(p->v_cache, e))
+    if (ce == 0) ce = e;
+    if (p->head_dim * ce % 16 != 0 || misaligned_row(p->k, e) || misaligned_row(p->v, e) || misaligned_row(p->k_cache, ce) || misaligned_row(p->v_cache, ce))
         return fail(SAGE_E_INVALID, "%s: rows of k, v and the caches must be 16-byte aligned and a multiple of 16 bytes long", who);
-    return launch_cache_append(*p, (hipStream_t)stream);
+    return SAGE_OK;
 }
 
-extern "C" int sage_cache_copy_pages(const sage_copy_params* p, void* stream) {
-    const char* who = "sage_cache_copy_pages";
+extern "C" int sage_cache_append(const sage_append_params* p, void* stream) {
+    bool nothing;
+    if (int rc = check_append("sage_cache_append", p, nothing)) return rc;
+    return nothing ? SAGE_OK : launch_cache_append(*p, (hipStream_t)stream);
+}
+
+
+static int check_copy(const char* who, const sage_copy_params* p, bool& nothing) {
+    nothing = false;
     if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
     if (p->count < 0 || p->layers < 0 || p->pages < 0 || p->page_bytes < 0) return fail(SAGE_E_INVALID, "%s: negative size", who);
     if (p->count >= (1LL << 30) || p->pages >= (1LL << 30) || p->page_bytes >= (1LL << 30) || p->layers > 32767)
         return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30, layers at most 32767", who);
-    if (p->count == 0 || p->layers == 0 || p->pages == 0 || p->page_bytes == 0) return SAGE_OK;
+    nothing = p->count == 0 || p->layers == 0 || p->pages == 0 || p->page_bytes == 0;
+    if (nothing) return SAGE_OK;
     if (!p->k_cache || !p->v_cache || !p->src || !p->dst) return fail(SAGE_E_INVALID, "%s: null pointer", who);
     if (p->page_bytes % 16 != 0 || ((uintptr_t)p->k_cache | (uintptr_t)p->v_cache | p->k_stride_layer | p->k_stride_page | p->v_stride_layer | p->v_stride_page) % 16 != 0)
         return fail(SAGE_E_INVALID, "%s: pages must be 16-byte aligned and a multiple of 16 bytes long", who);
-    return launch_cache_copy(*p, (hipStream_t)stream);
+    return SAGE_OK;
+}
+
+extern "C" int sage_cache_copy_pages(const sage_copy_params* p, void* stream) {
+    bool nothing;
+    if (int rc = check_copy("sage_cache_copy_pages", p, nothing)) return rc;
+    return nothing ? SAGE_OK : launch_cache_copy(*p, (hipStream_t)stream);
+}
+
+// ---- caches of 8-bit codes
+static int check_scales(const char* who, const sage_cache_scales& s, int64_t page_size) {
+    if (s.codes != SAGE_CODE_INT8 && s.codes != SAGE_CODE_E4M3) return fail(SAGE_E_INVALID, "%s: unknown kind of codes %d", who, s.codes);
+    if (s.blocks <= 0 || page_size % s.blocks != 0) return fail(SAGE_E_INVALID, "%s: the blocks of a page must divide page_size", who);
+    if (!s.k || !s.v) return fail(SAGE_E_INVALID, "%s: null scales", who);
+    const int64_t strides[] = {s.k_stride_page, s.k_stride_head, s.k_stride_block, s.v_stride_page, s.v_stride_head, s.v_stride_block};
+    for (int64_t x : strides)
+        if (x < 0 || x >= (1LL << 31)) return fail(SAGE_E_UNSUPPORTED, "%s: strides of the scales must stay between 0 and 2^31", who);
+    return SAGE_OK;
+}
+
+static int check_paged8(const char* who, const sage_paged8_params* p, bool& nothing) {
+    if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
+    if (int rc = check_paged(who, &p->paged, nothing, 1)) return rc;
+    return nothing ? SAGE_OK : check_scales(who, p->scales, p->paged.page_size);
+}
+
+extern "C" int64_t sage_paged8_attn_workspace_bytes(const sage_paged8_params* p) {
+    bool nothing;
+    if (check_paged8("sage_paged8_attn_workspace_bytes", p, nothing)) return -1;
+    return nothing ? 0 : paged8_workspace_bytes(*p);
+}
+
+extern "C" int sage_paged8_attn(const sage_paged8_params* p, void* workspace, int64_t workspace_bytes, void* stream) {
+    bool nothing;
+    if (int rc = check_paged8("sage_paged8_attn", p, nothing)) return rc;
+    if (int rc = check_workspace("sage_paged8_attn", workspace, workspace_bytes)) return rc;
+    return nothing ? SAGE_OK : launch_paged8_attn(*p, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+static int check_append8(const char* who, const sage_append8_params* p, bool& nothing) {
+    if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
+    if (int rc = check_append(who, &p->append, nothing, 1)) return rc;
+    if (nothing) return SAGE_OK;
+    if (int rc = check_scales(who, p->scales, p->append.page_size)) return rc;
+    if (p->append.head_dim > 512) return fail(SAGE_E_UNSUPPORTED, "%s: head_dim at most 512", who);
+    if (p->append.page_size / p->scales.blocks > 1024) return fail(SAGE_E_UNSUPPORTED, "%s: blocks of at most 1024 tokens", who);
+    if (append8_workspace_bytes(*p) > (1LL << 34)) return fail(SAGE_E_UNSUPPORTED, "%s: a cache of at most 2^32 tokens where blocks are of several", who);
+    return SAGE_OK;
+}
+
+extern "C" int64_t sage_cache8_append_workspace_bytes(const sage_append8_params* p) {
+    bool nothing;
+    if (check_append8("sage_cache8_append_workspace_bytes", p, nothing)) return -1;
+    return nothing ? 0 : append8_workspace_bytes(*p);
+}
+
+extern "C" int sage_cache8_append(const sage_append8_params* p, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* who = "sage_cache8_append";
+    bool nothing;
+    if (int rc = check_append8(who, p, nothing)) return rc;
+    if (int rc = check_workspace(who, workspace, workspace_bytes)) return rc;
+    if (nothing) return SAGE_OK;
+    const int64_t need = append8_workspace_bytes(*p);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return fail(SAGE_E_INVALID, "%s: needs a workspace of %lld bytes", who, (long long)need);
+    return launch_cache8_append(*p, workspace, (hipStream_t)stream);
+}
+
+extern "C" int sage_cache_read(const sage_read_params* p, void* stream) {
+    const char* who = "sage_cache_read";
+    if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
+    if (!float_dtype_ok(p->out_dtype)) return fail(SAGE_E_INVALID, "%s: bad out_dtype %d", who, p->out_dtype);
+    if (p->seqs < 0 || p->total < 0 || p->heads_kv < 0 || p->head_dim < 0 || p->pages < 0 || p->table_width < 0)
+        return fail(SAGE_E_INVALID, "%s: negative size", who);
+    if (p->page_size <= 0) return fail(SAGE_E_INVALID, "%s: page_size must be positive", who);
+    const int64_t lim = 1LL << 30;
+    if (p->seqs >= lim || p->total >= lim || p->pages >= lim || p->page_size >= lim || p->table_width >= lim || p->heads_kv > (1 << 16) || p->head_dim > (1 << 12))
+        return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30, heads_kv at most 65536, head_dim at most 4096", who);
+    if (p->seqs == 0 || p->total == 0 || p->heads_kv == 0 || p->head_dim == 0) return SAGE_OK;
+    const bool somewhere = p->pages > 0 && p->table_width > 0;  // (else every row is zeros)
+    if (!p->k_out.ptr || !p->v_out.ptr || !p->cu_seqlens || (somewhere && (!p->k_cache.ptr || !p->v_cache.ptr || !p->block_table)))
+        return fail(SAGE_E_INVALID, "%s: null pointer", who);
+    const int e = dtype_bytes(p->out_dtype), ce = p->scales.codes == SAGE_CODE_NONE ? e : 1;
+    if (p->head_dim * ce % 16 != 0 || misaligned_row(p->k_out, e) || misaligned_row(p->v_out, e) || misaligned_row(p->k_cache, ce) || misaligned_row(p->v_cache, ce))
+        return fail(SAGE_E_INVALID, "%s: rows of the caches and outputs must be 16-byte aligned and a multiple of 16 bytes long", who);
+    if (p->scales.codes != SAGE_CODE_NONE && somewhere)
+        if (int rc = check_scales(who, p->scales, p->page_size)) return rc;
+    return launch_cache_read(*p, (hipStream_t)stream);
+}
+
+extern "C" int sage_cache8_copy_pages(const sage_copy8_params* p, void* stream) {
+    const char* who = "sage_cache8_copy_pages";
+    bool nothing;
+    if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
+    if (int rc = check_copy(who, &p->copy, nothing)) return rc;
+    if (p->scale_words < 0) return fail(SAGE_E_INVALID, "%s: negative size", who);
+    if (p->scale_words >= (1LL << 30)) return fail(SAGE_E_UNSUPPORTED, "%s: sizes must stay below 2^30", who);
+    if (nothing) return SAGE_OK;
+    if (!p->k_scale || !p->v_scale) return fail(SAGE_E_INVALID, "%s: null scales", who);
+    return launch_cache8_copy(*p, (hipStream_t)stream);
 }

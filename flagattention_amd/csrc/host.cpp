@@ -564,6 +564,174 @@ PyObject* put_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params)
     });
 }
 
+// ---- caches of codes: the calls above with their scales behind the other arguments, and the reading of a cache, with scales or without:
+//      paged8 (q, k_cache, v_cache, block_table, seq_lens, sm_scale, layout, want_log_normalizer, k_scale, v_scale)
+struct Paged8Call {
+    const at::Tensor* t[10];
+    bool hnd, want_l;
+    Key key;
+    bool parse(PyObject* const* a, Py_ssize_t n) {
+        if (n < 10 || !is_hnd(a[6], hnd) || !is_bool(a[7], want_l)) return false;
+        key.add((int64_t)6);
+        if (!add_tensors(key, a, 0, 5, t) || !add_tensors(key, a, 8, 10, t) || !add_scale(key, a[5])) return false;
+        key.add((int64_t)hnd);
+        return true;
+    }
+};
+
+PyObject* paged8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Paged8Call c;
+        if (!c.parse(a, n)) return none();
+        Plan* plan = find(c.key);
+        if (!plan) return none();
+        const at::Device dev = c.t[0]->device();
+        if (!all_ready(c.t, 3, 5, dev) || !all_ready(c.t + 8, 0, 2, dev)) return none();
+        auto& p8 = *reinterpret_cast<sage_paged8_params*>(&plan->params[0]);
+        sage_paged_params& p = p8.paged;
+        const at::Tensor o = at::empty(c.t[0]->sizes(), options(dev, c.t[0]->scalar_type()));
+        at::Tensor l;
+        if (c.want_l) l = c.t[0]->dim() == 3 ? at::empty({p.seqs, p.heads_q}, options(dev, at::kFloat))
+                                             : at::empty({p.seqs, p.heads_q, p.new_tokens}, options(dev, at::kFloat));
+        p.q.ptr = c.t[0]->data_ptr(); p.out.ptr = o.data_ptr(); p.k_cache.ptr = c.t[1]->data_ptr(); p.v_cache.ptr = c.t[2]->data_ptr();
+        p.log_normalizer = c.want_l ? (float*)l.data_ptr() : nullptr;
+        p.block_table = (const int32_t*)c.t[3]->data_ptr(); p.seq_lens = (const int32_t*)c.t[4]->data_ptr();
+        p8.scales.k = (float*)c.t[8]->data_ptr(); p8.scales.v = (float*)c.t[9]->data_ptr();
+        void* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+        at::Tensor ws;
+        if (plan->workspace > 0) ws = workspace(dev, plan->workspace);
+        if (int rc = sage_paged8_attn(&p8, plan->workspace > 0 ? ws.data_ptr() : nullptr, plan->workspace, stream)) return PyLong_FromLong(rc);
+        return pack({&o, c.want_l ? &l : nullptr});
+    });
+}
+
+PyObject* put_paged8(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params, workspace bytes)
+    return guarded([&]() -> PyObject* {
+        Paged8Call c;
+        if (n != 12 || !c.parse(a, n)) return none();
+        return put(c.key, a[10], a[11], false);
+    });
+}
+
+//      append8 (k, v, k_cache, v_cache, slots, layout, k_scale, v_scale), copy8 (k_cache, v_cache, src, dst, k_scale, v_scale)
+struct Move8Call {
+    const at::Tensor* t[8];
+    Key key;
+    bool parse(PyObject* const* a, Py_ssize_t n, int tensors) {
+        bool hnd = false;
+        const int scales = tensors + (tensors == 5);
+        if (n < scales + 2 || (tensors == 5 && !is_hnd(a[5], hnd))) return false;
+        key.add((int64_t)(1 + tensors + 2 * hnd) << 16);
+        return add_tensors(key, a, 0, tensors, t) && add_tensors(key, a, scales, scales + 2, t);
+    }
+};
+
+PyObject* append8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Move8Call c;
+        if (!c.parse(a, n, 5)) return none();
+        Plan* plan = find(c.key);
+        const at::Device dev = c.t[0]->device();
+        if (!plan || !all_ready(c.t, 4, 5, dev) || !all_ready(c.t + 6, 0, 2, dev)) return none();
+        auto& p8 = *reinterpret_cast<sage_append8_params*>(&plan->params[0]);
+        sage_append_params& p = p8.append;
+        p.k.ptr = c.t[0]->data_ptr(); p.v.ptr = c.t[1]->data_ptr(); p.k_cache.ptr = c.t[2]->data_ptr(); p.v_cache.ptr = c.t[3]->data_ptr();
+        p.slots = c.t[4]->data_ptr();
+        p8.scales.k = (float*)c.t[6]->data_ptr(); p8.scales.v = (float*)c.t[7]->data_ptr();
+        at::Tensor ws;
+        if (plan->workspace > 0) ws = workspace(dev, plan->workspace);
+        const int rc = sage_cache8_append(&p8, plan->workspace > 0 ? ws.data_ptr() : nullptr, plan->workspace, c10::hip::getCurrentHIPStream(dev.index()).stream());
+        for (int i : {2, 3, 6, 7}) written(*c.t[i]);
+        return PyLong_FromLong(rc);
+    });
+}
+
+PyObject* put_append8(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params, workspace bytes)
+    return guarded([&]() -> PyObject* {
+        Move8Call c;
+        if (n != 10 || !c.parse(a, n, 5)) return none();
+        return put(c.key, a[8], a[9], false);
+    });
+}
+
+PyObject* copy8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Move8Call c;
+        if (!c.parse(a, n, 4)) return none();
+        Plan* plan = find(c.key);
+        const at::Device dev = c.t[0]->device();
+        if (!plan || !all_ready(c.t, 2, 6, dev)) return none();
+        auto& p8 = *reinterpret_cast<sage_copy8_params*>(&plan->params[0]);
+        sage_copy_params& p = p8.copy;
+        p.k_cache = c.t[0]->data_ptr(); p.v_cache = c.t[1]->data_ptr(); p.src = c.t[2]->data_ptr(); p.dst = c.t[3]->data_ptr();
+        p8.k_scale = (float*)c.t[4]->data_ptr(); p8.v_scale = (float*)c.t[5]->data_ptr();
+        const int rc = sage_cache8_copy_pages(&p8, c10::hip::getCurrentHIPStream(dev.index()).stream());
+        for (int i : {0, 1, 4, 5}) written(*c.t[i]);
+        return PyLong_FromLong(rc);
+    });
+}
+
+PyObject* put_copy8(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params)
+    return guarded([&]() -> PyObject* {
+        Move8Call c;
+        if (n != 7 || !c.parse(a, n, 4)) return none();
+        return put(c.key, a[6], nullptr, false);
+    });
+}
+
+//      read (k_cache, v_cache, block_table, cu_seqlens, total, layout, dtype), and (.., k_scale, v_scale)
+struct ReadCall {
+    const at::Tensor* t[9];
+    bool hnd, coded;
+    int64_t total;
+    at::ScalarType dtype;
+    Key key;
+    bool parse(PyObject* const* a, Py_ssize_t n) {
+        if ((n != 7 && n != 9) || !PyLong_CheckExact(a[4]) || !is_hnd(a[5], hnd) || !THPDtype_Check(a[6])) return false;
+        total = PyLong_AsLongLong(a[4]);
+        if (PyErr_Occurred()) {
+            PyErr_Clear();
+            return false;
+        }
+        dtype = reinterpret_cast<THPDtype*>(a[6])->scalar_type;
+        coded = n == 9;
+        key.add((int64_t)7);
+        if (!add_tensors(key, a, 0, 4, t) || (coded && !add_tensors(key, a, 7, 9, t))) return false;
+        key.add(total);
+        key.add((int64_t)dtype);
+        key.add((int64_t)(hnd | coded << 1));
+        return true;
+    }
+};
+
+PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        ReadCall c;
+        if (!c.parse(a, n)) return none();
+        Plan* plan = find(c.key);
+        const at::Device dev = c.t[0]->device();
+        if (!plan || !all_ready(c.t, 2, 4, dev) || (c.coded && !all_ready(c.t + 7, 0, 2, dev))) return none();
+        auto& p = *reinterpret_cast<sage_read_params*>(&plan->params[0]);
+        const at::Tensor k = at::empty({p.total, p.heads_kv, p.head_dim}, options(dev, c.dtype)), v = at::empty({p.total, p.heads_kv, p.head_dim}, options(dev, c.dtype));
+        p.k_cache.ptr = c.t[0]->data_ptr(); p.v_cache.ptr = c.t[1]->data_ptr(); p.k_out.ptr = k.data_ptr(); p.v_out.ptr = v.data_ptr();
+        p.block_table = (const int32_t*)c.t[2]->data_ptr(); p.cu_seqlens = (const int32_t*)c.t[3]->data_ptr();
+        if (c.coded) {
+            p.scales.k = (float*)c.t[7]->data_ptr();
+            p.scales.v = (float*)c.t[8]->data_ptr();
+        }
+        if (int rc = sage_cache_read(&p, c10::hip::getCurrentHIPStream(dev.index()).stream())) return PyLong_FromLong(rc);
+        return pack({&k, &v});
+    });
+}
+
+PyObject* put_read(PyObject*, PyObject* const* a, Py_ssize_t n) {  // + (params)
+    return guarded([&]() -> PyObject* {
+        ReadCall c;
+        if (n < 8 || !c.parse(a, n - 1)) return none();
+        return put(c.key, a[n - 1], nullptr, false);
+    });
+}
+
 PyMethodDef methods[] = {
     {"quant", (PyCFunction)(void (*)(void))quant, METH_FASTCALL, "outputs of a quantizer call whose plan is known, None, or a status"},
     {"put_quant", (PyCFunction)(void (*)(void))put_quant, METH_FASTCALL, "registers the plan of a quantizer call"},
@@ -579,6 +747,14 @@ PyMethodDef methods[] = {
     {"put_append", (PyCFunction)(void (*)(void))put_append, METH_FASTCALL, "registers the plan of a cache write"},
     {"copy", (PyCFunction)(void (*)(void))copy, METH_FASTCALL, "status of a page copy whose plan is known, or None"},
     {"put_copy", (PyCFunction)(void (*)(void))put_copy, METH_FASTCALL, "registers the plan of a page copy"},
+    {"paged8", (PyCFunction)(void (*)(void))paged8, METH_FASTCALL, "outputs of an attention call over a cache of codes whose plan is known, None, or a status"},
+    {"put_paged8", (PyCFunction)(void (*)(void))put_paged8, METH_FASTCALL, "registers the plan of an attention call over a cache of codes"},
+    {"append8", (PyCFunction)(void (*)(void))append8, METH_FASTCALL, "status of a quantized cache write whose plan is known, or None"},
+    {"put_append8", (PyCFunction)(void (*)(void))put_append8, METH_FASTCALL, "registers the plan of a quantized cache write"},
+    {"copy8", (PyCFunction)(void (*)(void))copy8, METH_FASTCALL, "status of a page copy with scales whose plan is known, or None"},
+    {"put_copy8", (PyCFunction)(void (*)(void))put_copy8, METH_FASTCALL, "registers the plan of a page copy with scales"},
+    {"read", (PyCFunction)(void (*)(void))read, METH_FASTCALL, "outputs of a cache read whose plan is known, None, or a status"},
+    {"put_read", (PyCFunction)(void (*)(void))put_read, METH_FASTCALL, "registers the plan of a cache read"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "native host side of calls whose shape has been seen before", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -4,7 +4,11 @@ keys and values in pages with the attention of new tokens over it.
 * ``flash_attention_varlen``  the dense forward over packed sequences,
 * ``paged_attention``         the newest token (or tokens) of every sequence against its cached keys and values,
 * ``append_to_cache``         rows of new tokens into the pages,
+* ``read_cache``              tokens of sequences out of the pages, packed (the keys of a prompt's next chunk),
 * ``copy_pages``              pages to other pages (sequences that split, pages moved together).
+
+A cache holds 16-bit numbers, or codes of 8 bits (int8 or e4m3) with a scale in fp32 for every block of tokens of a page and every
+head: the functions that take a cache take the scales with it (``k_scale``, ``v_scale``), and its entries are then code * scale.
 
 Lengths, tables, slots and page lists stay on the device: no call waits for the GPU, and a captured graph follows their present
 values.  Entries that lead nowhere (a negative slot, a page that the cache does not have) move and read nothing.  The cache
@@ -21,7 +25,9 @@ from torch.autograd import forward_ad
 from . import _lib
 from .sage_attention._common import DTYPE_CODE, current_stream_ptr, device_guard, require_gpu, split_workspace
 
-__all__ = ["flash_attention_varlen", "paged_attention", "append_to_cache", "copy_pages"]
+__all__ = ["flash_attention_varlen", "paged_attention", "append_to_cache", "read_cache", "copy_pages"]
+
+CODES = {torch.int8: _lib.SAGE_CODE_INT8, torch.float8_e4m3fn: _lib.SAGE_CODE_E4M3}
 
 
 def _host():
@@ -145,6 +151,40 @@ def _check_caches(k_cache, v_cache, hnd):
     return (p, a, b, d) if hnd else (p, b, a, d)
 
 
+def _coded(k_scale, v_scale):
+    """Whether a call's cache is one of codes."""
+    if k_scale is None and v_scale is None:
+        return False
+    if k_scale is None or v_scale is None:
+        raise ValueError("k_scale and v_scale go together")
+    return True
+
+
+def _check_codes(k_cache, v_cache):
+    if k_cache.dtype not in CODES or v_cache.dtype != k_cache.dtype:
+        raise TypeError("caches with scales must share one of torch.int8 / torch.float8_e4m3fn")
+
+
+def _check_scales(k_scale, v_scale, shape, page_size):
+    """shape: of the scales without their last dimension, the blocks of a page."""
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be a float32 tensor")
+        if t.dim() != len(shape) + 1 or t.shape[:-1] != shape:
+            raise ValueError(f"{name} must be ({', '.join(map(str, shape))}, blocks of a page)")
+    blocks = k_scale.shape[-1]
+    if v_scale.shape[-1] != blocks or blocks == 0 or page_size % blocks != 0:
+        raise ValueError("k_scale and v_scale must have as many blocks of a page, a divisor of the page size")
+
+
+def _scales_desc(k_scale, v_scale, dtype):
+    d = _lib.CacheScales()
+    d.k, d.v, d.blocks, d.codes = k_scale.data_ptr(), v_scale.data_ptr(), k_scale.shape[-1], CODES[dtype]
+    d.k_stride_page, d.k_stride_head, d.k_stride_block = _strides(k_scale)
+    d.v_stride_page, d.v_stride_head, d.v_stride_block = _strides(v_scale)
+    return d
+
+
 def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=False, sm_scale=None, return_log_normalizer=False,
                            *, out=None):
     """The dense forward of ``flash_attention`` over packed sequences of different lengths.
@@ -226,7 +266,7 @@ def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fals
 
 
 def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, tensor_layout="HND", return_log_normalizer=False,
-                    *, out=None):
+                    *, out=None, k_scale=None, v_scale=None):
     """Attention of the newest token of every sequence over a cache of keys and values in pages.
 
     ``q`` ``[S, H, D]``, or ``[S, M, H, D]`` for the M newest tokens of every sequence (fp16 / bf16).  ``k_cache``, ``v_cache``
@@ -239,13 +279,21 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
 
     Returns ``o`` in the shape of ``q``, or ``(o, log_normalizer)`` with the natural log-sum-exp ``[S, H]`` (``[S, H, M]``) in fp32.
     ``out``: where to write instead of a new tensor.  Roundings as in ``flash_attention_varlen``.
+
+    ``k_scale``, ``v_scale`` ``[pages, Hk, blocks]`` fp32 (any strides): the scales of a cache of codes, whose caches are int8 or
+    float8_e4m3fn (see ``append_to_cache``).  Codes are multiplied as they are; scores take K's scales in fp32, and the softmax's weights
+    V's, before they are rounded to fp16 (in a unit that keeps 11 bits of those down to 2^-28 of the largest).  A scale that is not finite
+    reaches the rows that see a token of its block.
     """
+    coded = _coded(k_scale, v_scale)
     call = (q, k_cache, v_cache, block_table, seq_lens, sm_scale, tensor_layout, return_log_normalizer)
+    scales = (k_scale, v_scale) if coded else ()
+    what = "sage_paged8_attn" if coded else "sage_paged_attn"
     if out is None:
-        res = _host().paged(*call)  # a call shape seen before: (o, log normalizer), or a status
+        res = _host().paged8(*call, *scales) if coded else _host().paged(*call)  # a call shape seen before: (o, log normalizer), or a status
         if res is not None:
             if type(res) is int:
-                _lib.check(res, "sage_paged_attn")
+                _lib.check(res, what)
             return res if return_log_normalizer else res[0]
     hnd = _layout(tensor_layout)
     if q.dim() not in (3, 4):
@@ -258,13 +306,19 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
     _check_heads(H, Hk, Hk)
     if D not in (64, 128):
         raise NotImplementedError(f"paged_attention: head_dim {D} is not built (64 or 128)")
-    _check_float16s(q, k_cache, v_cache)
+    if coded:
+        _check_float16s(q, q, q)
+        _check_codes(k_cache, v_cache)
+        _check_scales(k_scale, v_scale, (pages, Hk), page_size)
+    else:
+        _check_float16s(q, k_cache, v_cache)
     _int32(block_table, "block_table", 2)
     _int32(seq_lens, "seq_lens", 1)
     if block_table.shape[0] != S or seq_lens.shape[0] != S:
         raise ValueError("block_table and seq_lens must have a row for every sequence of q")
-    _no_grad("paged_attention", q, k_cache, v_cache, out)
-    _same_device(q.device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, seq_lens=seq_lens)
+    _no_grad("paged_attention", q, k_cache, v_cache, out, *scales)
+    _same_device(q.device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, seq_lens=seq_lens,
+                 **dict(zip(("k_scale", "v_scale"), scales)))
     if out is not None:
         _check_out(out, q)
     sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
@@ -290,46 +344,68 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
         p.seqs, p.new_tokens, p.heads_q, p.heads_kv, p.head_dim = S, M, H, Hk, D
         p.pages, p.page_size, p.dtype, p.sm_scale = pages, page_size, DTYPE_CODE[q.dtype], sm_scale
         lib = _lib.load()
-        ws_bytes = lib.sage_paged_attn_workspace_bytes(p)
+        attend, room, put = lib.sage_paged_attn, lib.sage_paged_attn_workspace_bytes, _host().put_paged
+        if coded:
+            p = _lib.Paged8Params(p, _scales_desc(k_scale, v_scale, k_cache.dtype))
+            attend, room, put = lib.sage_paged8_attn, lib.sage_paged8_attn_workspace_bytes, _host().put_paged8
+        ws_bytes = room(p)
         if ws_bytes < 0:
-            _lib.check(-1, "sage_paged_attn_workspace_bytes")
+            _lib.check(-1, what + "_workspace_bytes")
         if out is None and q is call[0] and block_table is call[3] and seq_lens is call[4]:  # (nothing was copied)
-            _host().put_paged(*call, bytes(p), ws_bytes)
+            put(*call, *scales, bytes(p), ws_bytes)
         ws = split_workspace(q.device, ws_bytes) if ws_bytes else None
-        _lib.check(lib.sage_paged_attn(p, ws.data_ptr() if ws is not None else None, ws_bytes, current_stream_ptr(q.device)),
-                   "sage_paged_attn")
+        _lib.check(attend(p, ws.data_ptr() if ws is not None else None, ws_bytes, current_stream_ptr(q.device)), what)
         if out is not None:
             _written(out)
     return (o, L) if return_log_normalizer else o
 
 
-def append_to_cache(k, v, k_cache, v_cache, slots, tensor_layout="HND"):
+def append_to_cache(k, v, k_cache, v_cache, slots, tensor_layout="HND", *, k_scale=None, v_scale=None):
     """Writes the keys and values of new tokens into the pages of a cache, in place.
 
     ``k``, ``v`` ``[tokens, Hk, D]`` (any strides), caches as for ``paged_attention`` (fp16, bf16 or fp32, one dtype; rows of a multiple of 16
     bytes).  ``slots`` ``[tokens]`` (int32 or int64, on the GPU): token t goes to place ``slots[t] % page_size`` of page
     ``slots[t] // page_size``.  Tokens whose slot the cache does not have are left out: -1 for the rows a batch is padded with.
     The other slots of a call have to differ.
+
+    With ``k_scale``, ``v_scale`` ``[pages, Hk, blocks]`` fp32 (any strides) the caches are int8 or float8_e4m3fn, D a multiple of 16 up to
+    512, and the rows are quantized as they are written: ``page_size / blocks`` (at most 1024) consecutive places of a page
+    and a head share a scale, one place each being the most exact.  A block's scale is the largest absolute value of the call's tokens for it (at
+    least 2^-100), divided by 127 (e4m3: by 448), or what it was where that is more; codes are entry / scale, to the nearest, ties to even.
+    Where a scale grows, the codes that the block holds are converted to it (rounded again); a token for a block's first place begins it anew:
+    what it held is forgotten, and places that the call does not write become zeros.  So blocks are filled from their first place on,
+    and a page that is used again needs no clearing.  (A block that is entered further in has to have a scale: zero, or as copied.)  An infinity or NaN
+    makes the block's scale NaN, until the block begins anew.
     """
+    coded = _coded(k_scale, v_scale)
     call = (k, v, k_cache, v_cache, slots, tensor_layout)
-    status = _host().append(*call)  # a call shape seen before
+    scales = (k_scale, v_scale) if coded else ()
+    what = "sage_cache8_append" if coded else "sage_cache_append"
+    status = _host().append8(*call, *scales) if coded else _host().append(*call)  # a call shape seen before
     if status is not None:
-        return _lib.check(status, "sage_cache_append")
+        return _lib.check(status, what)
     hnd = _layout(tensor_layout)
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError("k and v must be (tokens, heads, head_dim) tensors of the same shape")
     pages, Hk, page_size, D = _check_caches(k_cache, v_cache, hnd)
     if k.shape[1:] != (Hk, D):
         raise ValueError("heads and head_dim of k, v and the caches should be equal")
-    if k.dtype not in DTYPE_CODE or any(t.dtype != k.dtype for t in (v, k_cache, v_cache)):
+    if coded:
+        if k.dtype not in DTYPE_CODE or v.dtype != k.dtype:
+            raise TypeError("k and v must share one of torch.float16 / torch.bfloat16 / torch.float32")
+        _check_codes(k_cache, v_cache)
+        _check_scales(k_scale, v_scale, (pages, Hk), page_size)
+        _no_overlap(k_scale, "k_scale")
+        _no_overlap(v_scale, "v_scale")
+    elif k.dtype not in DTYPE_CODE or any(t.dtype != k.dtype for t in (v, k_cache, v_cache)):
         raise TypeError("k, v and the caches must share one of torch.float16 / torch.bfloat16 / torch.float32")
     _no_overlap(k_cache, "k_cache")
     _no_overlap(v_cache, "v_cache")
     slots = _index_list(slots, "slots")
     if slots.shape[0] != k.shape[0]:
         raise ValueError("slots must have an entry for every token")
-    _no_grad("append_to_cache", k, v, k_cache, v_cache)
-    _same_device(k.device, k=k, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots)
+    _no_grad("append_to_cache", k, v, k_cache, v_cache, *scales)
+    _same_device(k.device, k=k, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots, **dict(zip(("k_scale", "v_scale"), scales)))
     with device_guard(k.device):
         k, v = _rows16(k), _rows16(v)
         p = _lib.AppendParams()
@@ -338,10 +414,98 @@ def append_to_cache(k, v, k_cache, v_cache, slots, tensor_layout="HND"):
         p.slots, p.slots_int64 = slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0
         p.tokens, p.heads_kv, p.head_dim, p.pages, p.page_size = k.shape[0], Hk, D, pages, page_size
         p.dtype = DTYPE_CODE[k.dtype]
-        if k is call[0] and v is call[1] and slots is call[4]:  # (nothing was copied)
-            _host().put_append(*call, bytes(p))
-        _lib.check(_lib.load().sage_cache_append(p, current_stream_ptr(k.device)), "sage_cache_append")
-        _written(k_cache, v_cache)
+        lib, stream = _lib.load(), current_stream_ptr(k.device)
+        as_given = k is call[0] and v is call[1] and slots is call[4]  # (nothing was copied)
+        if coded:
+            p = _lib.Append8Params(p, _scales_desc(k_scale, v_scale, k_cache.dtype))
+            ws_bytes = lib.sage_cache8_append_workspace_bytes(p)
+            if ws_bytes < 0:
+                _lib.check(-1, what + "_workspace_bytes")
+            if as_given:
+                _host().put_append8(*call, *scales, bytes(p), ws_bytes)
+            ws = split_workspace(k.device, ws_bytes) if ws_bytes else None
+            _lib.check(lib.sage_cache8_append(p, ws.data_ptr() if ws is not None else None, ws_bytes, stream), what)
+        else:
+            if as_given:
+                _host().put_append(*call, bytes(p))
+            _lib.check(lib.sage_cache_append(p, stream), what)
+        _written(k_cache, v_cache, *scales)
+
+
+def read_cache(k_cache, v_cache, block_table, cu_seqlens, total, tensor_layout="HND", *, dtype=None, out=None, k_scale=None, v_scale=None):
+    """Reads the tokens of sequences out of the pages of a cache into packed rows, as ``flash_attention_varlen`` takes them: the keys and
+    values so far, before the next chunk of a prompt.
+
+    Caches as for ``paged_attention`` (fp16, bf16 or fp32, or codes with their ``k_scale`` and ``v_scale``; rows of a multiple of 16
+    bytes), ``block_table`` ``[S, width]`` int32.  ``cu_seqlens`` ``[S + 1]`` int32, on the GPU: where each sequence's rows begin, and where the
+    last one's end; sequence s is read from its first token on.  ``total``: rows of the results.
+
+    Returns ``(k, v)``, ``[total, Hk, D]`` each, of ``dtype``: fp16, bf16 or fp32 for a cache of codes (default bf16), whose values are rounded
+    once; the caches' own otherwise.  ``out``: a pair of tensors to write instead of new ones.  Rows behind the last sequence are not
+    written; tokens whose page the cache does not have, or that the table does not hold, are rows of zeros.
+    """
+    coded = _coded(k_scale, v_scale)
+    if dtype is None:
+        dtype = torch.bfloat16 if coded else k_cache.dtype
+    scales = (k_scale, v_scale) if coded else ()
+    call = (k_cache, v_cache, block_table, cu_seqlens, total, tensor_layout, dtype)
+    if out is None:
+        res = _host().read(*call, *scales)  # a call shape seen before: (k, v), or a status
+        if res is not None:
+            if type(res) is int:
+                _lib.check(res, "sage_cache_read")
+            return res
+    hnd = _layout(tensor_layout)
+    pages, Hk, page_size, D = _check_caches(k_cache, v_cache, hnd)
+    if page_size == 0:
+        raise ValueError("page_size must be positive")
+    if dtype not in DTYPE_CODE:
+        raise TypeError("dtype must be one of torch.float16 / torch.bfloat16 / torch.float32")
+    if coded:
+        _check_codes(k_cache, v_cache)
+        _check_scales(k_scale, v_scale, (pages, Hk), page_size)
+    elif k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise TypeError("caches without scales must have the dtype that is asked for")
+    _int32(block_table, "block_table", 2)
+    _int32(cu_seqlens, "cu_seqlens", 1)
+    S = block_table.shape[0]
+    if cu_seqlens.numel() != S + 1:
+        raise ValueError("cu_seqlens must have one entry more than block_table has rows")
+    if isinstance(total, bool) or not isinstance(total, int) or total < 0:
+        raise ValueError("total must be a number of rows")
+    if out is not None and (not isinstance(out, (tuple, list)) or len(out) != 2):
+        raise ValueError("out must be a pair of tensors")
+    _no_grad("read_cache", k_cache, v_cache, *scales, *(out or ()))
+    _same_device(k_cache.device, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cu_seqlens=cu_seqlens,
+                 **dict(zip(("k_scale", "v_scale"), scales)))
+    for t in out or ():
+        if t.shape != (total, Hk, D) or t.dtype != dtype or t.device != k_cache.device:
+            raise ValueError("out must be (total, heads, head_dim) tensors of dtype, on the device of the caches")
+        if not _aligned(t):
+            raise ValueError("out: rows must be 16-byte aligned, with a unit innermost stride")
+        _no_overlap(t, "out")
+    with device_guard(k_cache.device):
+        if block_table.stride(1) != 1 or block_table.stride(0) < 0:
+            block_table = block_table.contiguous()
+        cu_seqlens = cu_seqlens.contiguous()
+        k, v = out if out is not None else (torch.empty((total, Hk, D), dtype=dtype, device=k_cache.device) for _ in range(2))
+        p = _lib.ReadParams()
+        p.k_cache, p.v_cache = _cache_desc(k_cache, hnd), _cache_desc(v_cache, hnd)
+        p.k_out, p.v_out = _token_desc(k), _token_desc(v)
+        p.block_table, p.cu_seqlens = block_table.data_ptr(), cu_seqlens.data_ptr()
+        p.table_stride, p.table_width = block_table.stride(0), block_table.shape[1]
+        p.seqs, p.total, p.heads_kv, p.head_dim, p.pages, p.page_size = S, total, Hk, D, pages, page_size
+        p.out_dtype = DTYPE_CODE[dtype]
+        if coded:
+            p.scales = _scales_desc(k_scale, v_scale, k_cache.dtype)
+        else:
+            p.scales.codes = _lib.SAGE_CODE_NONE
+        if out is None and block_table is call[2] and cu_seqlens is call[3]:  # (nothing was copied)
+            _host().put_read(*call, *scales, bytes(p))
+        _lib.check(_lib.load().sage_cache_read(p, current_stream_ptr(k_cache.device)), "sage_cache_read")
+        if out is not None:
+            _written(k, v)
+    return k, v
 
 
 def _page_bytes(t):
@@ -356,26 +520,40 @@ def _page_bytes(t):
     return size * t.element_size()
 
 
-def copy_pages(k_cache, v_cache, src, dst):
+def copy_pages(k_cache, v_cache, src, dst, *, k_scale=None, v_scale=None):
     """Copies pages of a cache, keys and values, in place: page ``src[i]`` to page ``dst[i]``.
 
     ``k_cache``, ``v_cache`` ``[pages, ...]`` (four dimensions), or ``[layers, pages, ...]`` (five): the pages of all layers in one launch.
     Each page lies in one piece of a multiple of 16 bytes.  ``src``, ``dst`` ``[count]`` (int32 or int64, on the GPU); pairs with a page that the
     cache does not have are left out.  Pages that are written must differ from each other and from every page that is read: that is
     so where sequences split (the last page of each goes to a new one) and where pages in use move to unused ones.
+
+    ``k_scale``, ``v_scale`` ``[pages, Hk, blocks]`` fp32, or ``[layers, pages, Hk, blocks]``: the scales of a cache of codes, which are copied with the
+    pages; those of a page lie in one piece.
     """
+    coded = _coded(k_scale, v_scale)
     call = (k_cache, v_cache, src, dst)
-    status = _host().copy(*call)  # a call shape seen before
+    scales = (k_scale, v_scale) if coded else ()
+    what = "sage_cache8_copy_pages" if coded else "sage_cache_copy_pages"
+    status = _host().copy8(*call, *scales) if coded else _host().copy(*call)  # a call shape seen before
     if status is not None:
-        return _lib.check(status, "sage_cache_copy_pages")
+        return _lib.check(status, what)
     if k_cache.dim() not in (4, 5) or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError("k_cache and v_cache must be (pages, ...) or (layers, pages, ...) tensors of the same shape and dtype")
     src, dst = _index_list(src, "src"), _index_list(dst, "dst")
     if src.shape != dst.shape:
         raise ValueError("src and dst must have the same number of pages")
-    _no_grad("copy_pages", k_cache, v_cache)
-    _same_device(k_cache.device, k_cache=k_cache, v_cache=v_cache, src=src, dst=dst)
     layered = k_cache.dim() == 5
+    if coded:
+        _check_codes(k_cache, v_cache)
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.dtype != torch.float32:
+                raise TypeError(f"{name} must be a float32 tensor")
+            if t.dim() != k_cache.dim() - 1 or t.shape[:2 if layered else 1] != k_cache.shape[:2 if layered else 1] or t.shape != k_scale.shape:
+                raise ValueError(f"{name} must be (pages, heads, blocks) or (layers, pages, heads, blocks), as the caches are")
+            _no_overlap(t, name)
+    _no_grad("copy_pages", k_cache, v_cache, *scales)
+    _same_device(k_cache.device, k_cache=k_cache, v_cache=v_cache, src=src, dst=dst, **dict(zip(("k_scale", "v_scale"), scales)))
     p = _lib.CopyParams()
     p.layers, p.pages, p.count = k_cache.shape[0] if layered else 1, k_cache.shape[1 if layered else 0], src.shape[0]
     if k_cache.numel() == 0 or p.count == 0:
@@ -396,8 +574,22 @@ def copy_pages(k_cache, v_cache, src, dst):
         setattr(p, f"{name}_stride_page", strides[1 if layered else 0] * e)
     p.src, p.src_int64 = src.data_ptr(), 1 if src.dtype == torch.int64 else 0
     p.dst, p.dst_int64 = dst.data_ptr(), 1 if dst.dtype == torch.int64 else 0
+    copy, put = _lib.load().sage_cache_copy_pages, _host().put_copy
+    if coded:
+        p = _lib.Copy8Params(copy=p, k_scale=k_scale.data_ptr(), v_scale=v_scale.data_ptr())
+        copy, put = _lib.load().sage_cache8_copy_pages, _host().put_copy8
+        for name, t in (("k", k_scale), ("v", v_scale)):
+            nbytes = _page_bytes(t[0] if layered else t)
+            if nbytes is None:
+                raise ValueError(f"the scales of a page of {name}_scale do not lie in one piece of memory")
+            p.scale_words = nbytes // 4
+            strides = _strides(t)
+            if p.copy.pages > 1 and strides[1 if layered else 0] < p.scale_words:
+                raise ValueError(f"{name}_scale: pages overlap")
+            setattr(p, f"{name}_scale_stride_layer", strides[0] if layered else 0)
+            setattr(p, f"{name}_scale_stride_page", strides[1 if layered else 0])
     if src is call[2] and dst is call[3]:  # (nothing was copied)
-        _host().put_copy(*call, bytes(p))
+        put(*call, *scales, bytes(p))
     with device_guard(k_cache.device):
-        _lib.check(_lib.load().sage_cache_copy_pages(p, current_stream_ptr(k_cache.device)), "sage_cache_copy_pages")
-        _written(k_cache, v_cache)
+        _lib.check(copy(p, current_stream_ptr(k_cache.device)), what)
+        _written(k_cache, v_cache, *scales)

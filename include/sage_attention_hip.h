@@ -368,6 +368,90 @@ typedef struct sage_copy_params {
 
 int sage_cache_copy_pages(const sage_copy_params* p, void* stream);
 
+/*
+ * Caches of 8-bit codes.  A cache as for sage_paged_attn whose entries are codes of one byte, int8 (-127 .. 127) or e4m3 (OCP, at most
+ * 448), and a scale in fp32 for every block of page_size / blocks consecutive tokens of a page and every K/V head: an entry stands for
+ * code * scale.
+ *
+ *   k, v         scales [pages, Hkv, blocks] through *_stride_page, *_stride_head and *_stride_block (in elements)
+ *   blocks       of a page; divides page_size
+ *   codes        SAGE_CODE_INT8 or SAGE_CODE_E4M3
+ */
+#define SAGE_CODE_INT8 0
+#define SAGE_CODE_E4M3 1
+typedef struct sage_cache_scales {
+    float* k;
+    float* v;
+    int64_t k_stride_page, k_stride_head, k_stride_block, v_stride_page, v_stride_head, v_stride_block, blocks;
+    int32_t codes, reserved;
+} sage_cache_scales;
+
+/*
+ * sage_paged_attn over a cache of codes.  paged.dtype is that of q and out (SAGE_F16 / SAGE_BF16); the strides of the caches count
+ * bytes, and their rows are 16-byte aligned.  Blocks whose scale is not finite reach the rows that see one of their tokens.
+ */
+typedef struct sage_paged8_params {
+    sage_paged_params paged;
+    sage_cache_scales scales;
+} sage_paged8_params;
+
+int64_t sage_paged8_attn_workspace_bytes(const sage_paged8_params* p);
+int sage_paged8_attn(const sage_paged8_params* p, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * sage_cache_append into a cache of codes.  append.dtype is that of k and v (SAGE_F16 / SAGE_BF16 / SAGE_F32), head_dim a multiple of
+ * 16 up to 512, blocks of at most 1024 tokens.  Of the tokens of a call that go to one block, and one head, let a be the largest
+ * absolute value, at least 2^-100.  The block's scale becomes a / 127 (e4m3: a / 448), or stays as it was where that is more; where
+ * one of the tokens goes to the block's first place, the block begins anew, and what it held before is forgotten: the places that are not written get
+ * zero codes.  Codes are x / scale rounded to the nearest, ties to even; where a scale has grown, the codes that stay are
+ * code * old scale / new scale, rounded likewise.  An infinity or NaN makes the block's scale NaN until it begins anew.
+ *
+ * workspace: sage_cache8_append_workspace_bytes(p) bytes, contents irrelevant before and after; rules of sage_attn_fwd_ws, but that
+ * a call that needs one is refused without (SAGE_E_INVALID).
+ */
+typedef struct sage_append8_params {
+    sage_append_params append;
+    sage_cache_scales scales;
+} sage_append8_params;
+
+int64_t sage_cache8_append_workspace_bytes(const sage_append8_params* p);
+int sage_cache8_append(const sage_append8_params* p, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Reads the tokens of sequences out of a cache into packed rows: token t of sequence s goes to row cu_seqlens[s] + t of k_out and v_out, for
+ * cu_seqlens[s + 1] - cu_seqlens[s] tokens.  Rows behind the last sequence are not written; tokens whose page the cache does not have, or that the table
+ * does not hold, are rows of zeros.
+ *
+ *   k_out, v_out  [total, Hkv, D] through stride_n (row) and stride_h, of out_dtype
+ *   scales        of a cache of codes, whose values are rounded once to out_dtype; scales.codes SAGE_CODE_NONE: a cache of
+ *                 entries of out_dtype, which are copied (the rest of scales is not looked at)
+ *   Rows of the caches and outputs are 16-byte aligned and a multiple of 16 bytes long.
+ */
+#define SAGE_CODE_NONE (-1)
+typedef struct sage_read_params {
+    sage_tensor k_cache, v_cache, k_out, v_out;
+    const int32_t* block_table;
+    const int32_t* cu_seqlens;
+    int64_t table_stride, seqs, total, heads_kv, head_dim, pages, page_size, table_width;
+    int32_t out_dtype, reserved;
+    sage_cache_scales scales;
+} sage_read_params;
+
+int sage_cache_read(const sage_read_params* p, void* stream);
+
+/*
+ * sage_cache_copy_pages with the pages' scales, in the same launch.  The scales of a page are scale_words contiguous floats (all heads and
+ * blocks, in any order), pages *_scale_stride_page and layers *_scale_stride_layer floats apart.
+ */
+typedef struct sage_copy8_params {
+    sage_copy_params copy;
+    float* k_scale;
+    float* v_scale;
+    int64_t k_scale_stride_layer, k_scale_stride_page, v_scale_stride_layer, v_scale_stride_page, scale_words;
+} sage_copy8_params;
+
+int sage_cache8_copy_pages(const sage_copy8_params* p, void* stream);
+
 /* Message describing the last non-zero status returned on this thread ("" if none). */
 const char* sage_hip_last_error(void);
 
