@@ -14,11 +14,18 @@ using namespace attn;
 
 constexpr int kOpThreads = 256;
 constexpr int kMostBlock = 1024;     // tokens that share a scale
-constexpr int kScanTokens = 1024;    // calls of up to so many tokens look their slots over instead of mapping them
+constexpr int kScanTokens = 256;    // calls of up to so many tokens look their slots over instead of mapping them
+constexpr int kWriteWorkgroups = 4096;  // that a write of blocks makes where it can
 constexpr float kSmallest = 0x1p-100f;
 
 __device__ __forceinline__ int64_t index_at(const void* list, int wide, int64_t i) {
     return wide ? static_cast<const int64_t*>(list)[i] : (int64_t) static_cast<const int32_t*>(list)[i];
+}
+
+// x / d for x >= 0, in 32 bits where x has no more (a division in 64 costs about 150 instructions); shift: log2 of d, -1: it has none
+__device__ __forceinline__ int64_t quotient(int64_t x, int d, int shift) {
+    if (shift >= 0) return x >> shift;
+    return (x >> 32) == 0 ? (int64_t)((unsigned)x / (unsigned)d) : x / d;
 }
 
 // Sixteen entries of a row.
@@ -94,16 +101,18 @@ template <> struct Rounding<Int8> {
     // Sixteen codes of x, s > 0 (or inv = 0: codes 0).  x inv + 1.5 2^23 is an integer in its low bits.
     template <typename Row>
     static __device__ __forceinline__ v4i codes(const Row& x, float s, float inv) {
-        constexpr float magic = 12582912.0f;
+        constexpr float magic = 12582912.0f, near = 0.5f - 0x1p-15f;
+        auto off = [&](int i, float z) { return __builtin_fabsf(__builtin_fmaf(x.at(i), inv, -(z - magic))); };
         float z[16], far = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             z[i] = __builtin_fmaf(x.at(i), inv, magic);
-            far = fmaxf(far, __builtin_fabsf(__builtin_fmaf(x.at(i), inv, -(z[i] - magic))));
+            far = fmaxf(far, off(i, z[i]));
         }
-        if (__builtin_amdgcn_ballot_w64(far > 0.5f - 0x1p-15f) != 0) {
+        if (__builtin_amdgcn_ballot_w64(far > near) != 0) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) z[i] = settle(x.at(i), s, z[i] - magic) + magic;
+            for (int i = 0; i < 16; i++)
+                if (__builtin_amdgcn_ballot_w64(off(i, z[i]) > near) != 0) z[i] = settle(x.at(i), s, z[i] - magic) + magic;
         }
         v4i w;
 #pragma unroll
@@ -134,22 +143,26 @@ template <> struct Rounding<E4m3> {
     }
     template <typename Row>
     static __device__ __forceinline__ v4i codes(const Row& x, float s, float inv) {
+        // Next to the middle between two numbers: the 20 bits that are rounded away are 2^19, or up to 8 less or more; or among the small
+        // numbers, below 2^-6, whose steps are all the same, and not zero.
+        auto middle = [](float y) { return (__builtin_bit_cast(unsigned, y) << 12) + ((0x80000u + 8) << 12); };
+        auto small = [](float y) { return (__builtin_bit_cast(unsigned, y) << 1) - 1; };
+        auto close = [](unsigned middle, unsigned small) { return middle <= (16u << 12) || small < (0x3c800000u << 1) - 1; };
         float y[16];
-        unsigned close = 0;
+        unsigned least_middle = ~0u, least_small = ~0u;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             y[i] = x.at(i) * inv;
-            // Next to the middle between two numbers (the 20 bits that are rounded away are 2^19, or some less or more), or among the small
-            // numbers, whose steps are all the same, and not zero.
-            const unsigned b = __builtin_bit_cast(unsigned, y[i]) & 0x7fffffffu;
-            close |= ((b - 0x7fff8u) & 0xfffffu) <= 16 || b - 1 < 0x3c7fffffu ? 1 : 0;
+            least_middle = min(least_middle, middle(y[i]));
+            least_small = min(least_small, small(y[i]));
         }
-        if (__builtin_amdgcn_ballot_w64(close != 0) != 0) {
+        if (__builtin_amdgcn_ballot_w64(close(least_middle, least_small)) != 0) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float u = step(y[i]);
-                y[i] = inv != 0.0f ? settle(x.at(i), s * u, __builtin_rintf(y[i] / u)) * u : 0.0f;
-            }
+            for (int i = 0; i < 16; i++)
+                if (__builtin_amdgcn_ballot_w64(close(middle(y[i]), small(y[i]))) != 0) {
+                    const float u = step(y[i]);
+                    y[i] = inv != 0.0f ? settle(x.at(i), s * u, __builtin_rintf(y[i] / u)) * u : 0.0f;
+                }
         }
         v4i w;
 #pragma unroll
@@ -182,7 +195,7 @@ struct WriteArgs {
     const void* slots;
     int32_t* map;  // [slots of the cache]: token that goes there, where that token's slot says so too; null: few tokens
     int64_t slot_limit, rows;  // rows: tokens * heads
-    int32_t wide, tokens, page_size, heads, pieces, group;  // pieces: of 16 entries, of a row; group: tokens a workgroup looks at
+    int32_t wide, tokens, page_size, page_shift, heads, head_shift, pieces, group, span;  // pieces: of 16 entries, of a row; group: tokens a workgroup looks at; span: lanes of a block
 };
 
 __device__ __forceinline__ float& scale_of(const WriteArgs& a, int x, int64_t page, int h, int block) {
@@ -190,27 +203,24 @@ __device__ __forceinline__ float& scale_of(const WriteArgs& a, int x, int64_t pa
              : a.scales.k[page * a.scales.k_p + h * a.scales.k_h + block * a.scales.k_b];
 }
 
-// A scale for every token: LPR lanes take a row of k and the same one of v, 16 entries each.
+// A scale for every token: LPR lanes take a row of k and the same one of v, 16 entries each.  The rows are requested before it is known
+// where they go.
 template <int LPR, typename T, typename Code>
 __global__ __launch_bounds__(kOpThreads) void cache8_write_rows_kernel(WriteArgs a) {
-    const int64_t row = ((int64_t)blockIdx.x * kOpThreads + threadIdx.x) / LPR;
+    const int64_t row = (int64_t)blockIdx.x * (kOpThreads / LPR) + threadIdx.x / LPR;
     const int c = threadIdx.x % LPR;
-    int64_t slot = -1, t = 0;
-    int h = 0;
-    if (row < a.rows) {
-        t = row / a.heads;
-        h = (int)(row - t * a.heads);
-        slot = index_at(a.slots, a.wide, t);
-    }
-    const bool ok = slot >= 0 && slot < a.slot_limit, mine = ok && c < a.pieces;
-    const int64_t page = ok ? slot / a.page_size : 0;
-    const int place = ok ? (int)(slot - page * a.page_size) : 0;
+    const int64_t t = quotient(min(row, a.rows - 1), a.heads, a.head_shift);
+    const int h = (int)(min(row, a.rows - 1) - t * a.heads);
+    const int64_t slot = index_at(a.slots, a.wide, t);
     Row16<T> x[2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        if (mine) x[i].load(a.src[i] + t * a.ss_t[i] + h * a.ss_h[i] + c * (16 * (int)sizeof(T)));
+        if (c < a.pieces) x[i].load(a.src[i] + t * a.ss_t[i] + h * a.ss_h[i] + c * (16 * (int)sizeof(T)));
         else x[i].clear();
     }
+    const bool ok = row < a.rows && slot >= 0 && slot < a.slot_limit, mine = ok && c < a.pieces;
+    const int64_t page = ok ? quotient(slot, a.page_size, a.page_shift) : 0;
+    const int place = ok ? (int)(slot - page * a.page_size) : 0;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         unsigned top = x[i].top(0);
@@ -232,41 +242,185 @@ __global__ __launch_bounds__(kOpThreads) void cache8_map_kernel(WriteArgs a) {
     if (slot >= 0 && slot < a.slot_limit) a.map[slot] = t;
 }
 
-// Blocks of several tokens.  A workgroup looks at `group` tokens; the one with the lowest place of those of the call that go to a block
-// takes care of the block: its tokens are looked for among all of them (SCAN) or through the map, which is not cleared before, since an entry counts
-// only where its token's slot leads back to it.  A wave takes a head of K or of V.
+// Blocks of several tokens.  Of the call's tokens that go to a block, the one with the lowest place takes care of it.  A workgroup looks at
+// `group` tokens, at most 64, and leaves out at once those that follow another one of their block from the place before their own.
+// The tokens of a block are looked for among all of the call's (SCAN) or through the map, which is not cleared before, since an
+// entry counts only where its token's slot leads back to it.
+struct Candidates {
+    int64_t base;   // of the lane's token: slot of its block's first place
+    int place;      // in the block
+    unsigned long long todo;  // tokens left (the same in every lane)
+};
+__device__ __forceinline__ Candidates look(const WriteArgs& a) {
+    Candidates r{0, 0, 0};
+    const int lane = threadIdx.x & 63;
+    bool candidate = false;
+    const int64_t t = (int64_t)blockIdx.x * a.group + lane;
+    if (lane < a.group && t < a.tokens) {
+        const int64_t slot = index_at(a.slots, a.wide, t);
+        const int64_t before = t > 0 ? index_at(a.slots, a.wide, t - 1) : -1;
+        if (slot >= 0 && slot < a.slot_limit) {
+            const int place = (int)(slot - quotient(slot, a.page_size, a.page_shift) * a.page_size);
+            r.place = place - a.scales.of(place) * a.scales.block;
+            r.base = slot - r.place;
+            candidate = r.place == 0 || before != slot - 1;
+        }
+    }
+    r.todo = __builtin_amdgcn_ballot_w64(candidate);
+    return r;
+}
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+    return ((int64_t)__shfl((int)(x >> 32), lane) << 32) | (unsigned)__shfl((int)(unsigned)x, lane);
+}
+__device__ __forceinline__ int mapped(const WriteArgs& a, int64_t slot) {
+    const int who = a.map[slot];
+    return who >= 0 && who < a.tokens && index_at(a.slots, a.wide, who) == slot ? who : -1;
+}
+
+// The scale of a block that had `was` and gets rows whose largest entry has the size `top`.
+template <typename Code>
+__device__ __forceinline__ float next_scale(float was, float top) {
+    const float asked = scale_for<Code>(top);
+    return was >= asked || was != was ? was : asked;
+}
+// Sixteen codes that stay when a scale grows.
+template <typename Code>
+__device__ __forceinline__ void convert(unsigned char* at, float was, float s) {
+    v4i w = *reinterpret_cast<v4i*>(at);
+#pragma unroll 1
+    for (int i = 0; i < 4; i++) {
+        const unsigned now = Rounding<Code>::again((unsigned)w[0], was, s);
+        w = v4i{w[1], w[2], w[3], (int)now};
+    }
+    *reinterpret_cast<v4i*>(at) = w;
+}
+
+constexpr int kKeep = 2;  // steps of 64 / LPR rows that a wave keeps in registers
+constexpr int kScanGroup = 4;
+
+// Blocks whose rows a wave keeps in registers.  A wave takes a block (blocks of 2, 4 or 8 tokens through the map: as many as fit its
+// lanes, `span` of them each) and goes through heads of K and V, the next one's rows on their way.
 template <int LPR, typename T, typename Code, bool SCAN>
-__global__ __launch_bounds__(kOpThreads) void cache8_write_blocks_kernel(WriteArgs a) {
-    constexpr int ROWS = 64 / LPR, KEEP = 4;  // rows of a step; steps whose rows are kept in registers
+__global__ __launch_bounds__(kOpThreads, 4) void cache8_write_blocks_kernel(WriteArgs a) {
+    constexpr int ROWS = 64 / LPR, WAVES = kOpThreads / 64;
+    __shared__ int found[SCAN ? kScanGroup * 64 : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int block = a.scales.block, span = a.span, sub = lane / span, c = lane % LPR;
+    Candidates cand = look(a);
+    if constexpr (SCAN) {
+        constexpr int EACH = kScanTokens / kOpThreads;
+        found[threadIdx.x] = -1;
+        int64_t slot[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int i = e * kOpThreads + threadIdx.x;
+            slot[e] = i < a.tokens ? index_at(a.slots, a.wide, i) : -1;
+        }
+        __syncthreads();
+        int n = 0;
+        for (unsigned long long todo = cand.todo; todo != 0; todo &= todo - 1, n++) {
+            const int64_t begin = lane_value(cand.base, __builtin_ctzll(todo));
+#pragma unroll
+            for (int e = 0; e < EACH; e++) {
+                const int64_t d = slot[e] - begin;
+                if (slot[e] >= 0 && d >= 0 && d < block) atomicMax(&found[n * 64 + d], e * kOpThreads + (int)threadIdx.x);  // (slots that occur twice: the last one)
+            }
+        }
+        __syncthreads();
+    }
+    for (int nth = 0; cand.todo != 0; nth++) {
+        int looker = -1;
+        for (int j = 0; j < 64 / span && cand.todo != 0; j++) {
+            if (sub == j) looker = __builtin_ctzll(cand.todo);
+            cand.todo &= cand.todo - 1;
+        }
+        if (nth % WAVES != wave) continue;
+        const int64_t begin = lane_value(cand.base, looker & 63);
+        const int t = (int)((int64_t)blockIdx.x * a.group + looker), place = __shfl(cand.place, looker & 63);
+        int who[kKeep];  // tokens of the lane's rows, -1: none, -2: no such place
+        bool other = looker < 0, first = false;
+#pragma unroll
+        for (int e = 0; e < kKeep; e++) {
+            const int p = e * ROWS + lane % span / LPR;
+            who[e] = -2;
+            if (p < block && looker >= 0) {
+                who[e] = SCAN ? found[nth * 64 + p] : mapped(a, begin + p);
+                other |= (who[e] >= 0 && p < place) || (p == place && who[e] != t);
+                first |= p == 0 && who[e] >= 0;
+            }
+        }
+        // (bit masks of the lanes of this block)
+        const unsigned long long lanes = span == 64 ? ~0ull : ((1ull << span) - 1) << (sub * span);
+        const bool mine = (__builtin_amdgcn_ballot_w64(other) & lanes) == 0, begun = (__builtin_amdgcn_ballot_w64(first) & lanes) != 0;
+        if (__builtin_amdgcn_ballot_w64(mine) == 0) continue;
+        if (!mine || c >= a.pieces) {
+#pragma unroll
+            for (int e = 0; e < kKeep; e++) who[e] = -2;
+        }
+        const int64_t page = mine ? quotient(begin, a.page_size, a.page_shift) : 0;
+        const int at = mine ? (int)(begin - page * a.page_size) : 0, b = a.scales.of(at);
+        Row16<T> rows[kKeep];
+        auto load = [&](int unit) {
+            const int x = unit & 1, h = unit >> 1;
+            const unsigned char* src = a.src[x] + h * a.ss_h[x] + c * (16 * (int)sizeof(T));
+#pragma unroll
+            for (int e = 0; e < kKeep; e++) {
+                if (who[e] >= 0) rows[e].load(src + who[e] * a.ss_t[x]);
+                else rows[e].clear();
+            }
+        };
+        int unit = blockIdx.y;
+        if (unit < 2 * a.heads) load(unit);
+        for (; unit < 2 * a.heads; unit += gridDim.y) {
+            const int x = unit & 1, h = unit >> 1;
+            unsigned char* dst = a.dst[x] + page * a.ds_p[x] + h * a.ds_h[x] + (at + lane % span / LPR) * a.ds_n[x] + 16 * c;
+            const float was = begun || !mine ? 0.0f : scale_of(a, x, page, h, b);
+            unsigned top = 0;
+#pragma unroll
+            for (int e = 0; e < kKeep; e++) top = rows[e].top(top);
+            for (int d = 1; d < span; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
+            const float s = next_scale<Code>(was, Row16<T>::size(top));
+            const float inv = s < INFINITY ? 1.0f / s : 0.0f;
+#pragma unroll
+            for (int e = 0; e < kKeep; e++) {
+                if (e * ROWS >= block) break;
+                if (!(s < INFINITY)) rows[e].clear();  // (NaN: an entry was not finite)
+                const v4i w = Rounding<Code>::codes(rows[e], s, inv);
+                if (who[e] >= 0 || (who[e] == -1 && begun))  // (zeros where a block begins)
+                    *reinterpret_cast<v4i*>(dst + e * ROWS * a.ds_n[x]) = w;
+            }
+            if (unit + (int)gridDim.y < 2 * a.heads) load(unit + gridDim.y);
+            if (s != was && s == s && !begun) {
+                for (int e = 0; e < kKeep; e++)
+                    if (who[e] == -1) convert<Code>(dst + e * ROWS * a.ds_n[x], was, s);
+            }
+            if (mine && lane % span == 0) scale_of(a, x, page, h, b) = s;
+        }
+    }
+}
+
+// Longer blocks: a workgroup takes a block, its waves a head of K or V each, and goes over the rows twice where they are more than a wave
+// keeps.
+template <int LPR, typename T, typename Code, bool SCAN>
+__global__ __launch_bounds__(kOpThreads, 4) void cache8_write_long_blocks_kernel(WriteArgs a) {
+    constexpr int ROWS = 64 / LPR, KEEP = 4, WAVES = kOpThreads / 64;
     __shared__ int token[kMostBlock];
     __shared__ int lowest;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int block = a.scales.block;
     const int rr = lane / LPR, c = lane % LPR;
-    for (int g = 0; g < a.group; g++) {
-        const int64_t t = (int64_t)blockIdx.x * a.group + g;
-        if (t >= a.tokens) return;
-        const int64_t slot = index_at(a.slots, a.wide, t);
-        if (slot < 0 || slot >= a.slot_limit) continue;
-        const int64_t page = slot / a.page_size;
-        const int place = (int)(slot - page * a.page_size), b = a.scales.of(place);
-        // (the token before it goes to the place before its own: that one, or one before it, takes care)
-        if (place != b * block && t > 0 && index_at(a.slots, a.wide, t - 1) == slot - 1) continue;
-        const int64_t base = page * a.page_size + (int64_t)b * block;
+    Candidates cand = look(a);
+    for (; cand.todo != 0; cand.todo &= cand.todo - 1) {
+        const int looker = __builtin_ctzll(cand.todo);
+        const int t = (int)((int64_t)blockIdx.x * a.group + looker);
+        const int64_t begin = lane_value(cand.base, looker);
         __syncthreads();  // (the tokens of the block before have been read)
-        for (int p = tid; p < block; p += kOpThreads) {
-            int who = -1;
-            if (!SCAN) {
-                who = a.map[base + p];
-                if (who < 0 || who >= a.tokens || index_at(a.slots, a.wide, who) != base + p) who = -1;
-            }
-            token[p] = who;
-        }
         if (tid == 0) lowest = block;
+        for (int p = tid; p < block; p += kOpThreads) token[p] = SCAN ? -1 : mapped(a, begin + p);
         __syncthreads();
         if (SCAN) {
             for (int i = tid; i < a.tokens; i += kOpThreads) {
-                const int64_t d = index_at(a.slots, a.wide, i) - base;
+                const int64_t d = index_at(a.slots, a.wide, i) - begin;
                 if (d >= 0 && d < block) atomicMax(&token[d], i);  // (slots that occur twice: the last one)
             }
             __syncthreads();
@@ -276,10 +430,13 @@ __global__ __launch_bounds__(kOpThreads) void cache8_write_blocks_kernel(WriteAr
         __syncthreads();
         if (token[lowest] != t) continue;
         const bool begun = lowest == 0;
-        for (int unit = blockIdx.y * (kOpThreads / 64) + wave; unit < 2 * a.heads; unit += gridDim.y * (kOpThreads / 64)) {
+        const int64_t page = quotient(begin, a.page_size, a.page_shift);
+        const int at = (int)(begin - page * a.page_size), b = a.scales.of(at);
+        for (int unit = blockIdx.y * WAVES + wave; unit < 2 * a.heads; unit += gridDim.y * WAVES) {
             const int x = unit & 1, h = unit >> 1;
             const unsigned char* src = a.src[x] + h * a.ss_h[x] + c * (16 * (int)sizeof(T));
-            unsigned char* dst = a.dst[x] + page * a.ds_p[x] + h * a.ds_h[x] + (int64_t)b * block * a.ds_n[x] + 16 * c;
+            unsigned char* dst = a.dst[x] + page * a.ds_p[x] + h * a.ds_h[x] + at * a.ds_n[x] + 16 * c;
+            const float was = begun ? 0.0f : scale_of(a, x, page, h, b);
             Row16<T> rows[KEEP];
             int who[KEEP];
             auto load = [&](int p0) {  // rows of places p0 ..; who: their tokens, -1: none, -2: no such place
@@ -299,27 +456,21 @@ __global__ __launch_bounds__(kOpThreads) void cache8_write_blocks_kernel(WriteAr
             }
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
-            const float asked = scale_for<Code>(Row16<T>::size(top));
-            const float was = begun ? 0.0f : scale_of(a, x, page, h, b);
-            const float s = was >= asked || was != was ? was : asked;
+            const float s = next_scale<Code>(was, Row16<T>::size(top));
             const float inv = s < INFINITY ? 1.0f / s : 0.0f;
-            const bool grown = s != was && s == s;
             for (int p0 = 0; p0 < block; p0 += KEEP * ROWS) {
-                if (block > KEEP * ROWS) load(p0);
+                load(p0);
 #pragma unroll
                 for (int e = 0; e < KEEP; e++) {
-                    v4i* to = reinterpret_cast<v4i*>(dst + (p0 + e * ROWS + rr) * a.ds_n[x]);
                     if (!(s < INFINITY)) rows[e].clear();  // (NaN: an entry was not finite)
                     const v4i w = Rounding<Code>::codes(rows[e], s, inv);
-                    if (who[e] >= 0 || (who[e] == -1 && begun)) *to = w;  // (zeros where a block begins)
-                    else if (who[e] == -1 && grown) {
-                        v4i old = *to;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) old[i] = (int)Rounding<Code>::again((unsigned)old[i], was, s);
-                        *to = old;
-                    }
+                    if (who[e] >= 0 || (who[e] == -1 && begun))  // (zeros where a block begins)
+                        *reinterpret_cast<v4i*>(dst + (p0 + e * ROWS + rr) * a.ds_n[x]) = w;
                 }
             }
+            if (s != was && s == s && !begun)
+                for (int p = rr; p < block; p += ROWS)
+                    if (c < a.pieces && token[p] < 0) convert<Code>(dst + p * a.ds_n[x], was, s);
             if (lane == 0) scale_of(a, x, page, h, b) = s;
         }
     }
@@ -437,6 +588,8 @@ __global__ __launch_bounds__(kOpThreads) void cache8_copy_kernel(Copy8Args a) {
     }
 }
 
+int log2_or_none(int64_t n) { return (n & (n - 1)) == 0 ? __builtin_ctzll((unsigned long long)n) : -1; }
+
 bool maps_tokens(const sage_append8_params& p) { return p.scales.blocks != p.append.page_size && p.append.tokens > kScanTokens; }
 
 }  // namespace
@@ -451,16 +604,25 @@ static int launch_write(WriteArgs a, hipStream_t stream) {
         hipLaunchKernelGGL((cache8_write_rows_kernel<LPR, T, Code>), dim3((unsigned)wgs), dim3(kOpThreads), 0, stream, a);
         return check_launch("cache8_write_rows_kernel");
     }
-    const int units = (2 * a.heads + kOpThreads / 64 - 1) / (kOpThreads / 64);
-    a.group = a.map ? 16 : 1;
-    const dim3 grid((unsigned)((a.tokens + a.group - 1) / a.group), (unsigned)(units < 65535 ? units : 65535));
-    if ((int64_t)grid.x > kMaxThreads / kOpThreads) return fail(SAGE_E_UNSUPPORTED, "sage_cache8_append: too many rows for one launch");
+    // A wave goes through heads where the blocks fill the chip, and takes one where there are few.
+    constexpr int ROWS = 64 / LPR;
+    const int block = a.scales.block;
+    const bool longer = block > kKeep * ROWS;
+    a.span = a.map && block <= ROWS && a.scales.shift >= 0 ? LPR * block : 64;
+    a.group = longer ? (a.map ? block < 64 ? block : 64 : 1) : a.map ? 4 * block < 64 ? 4 * block : 64 : kScanGroup;
+    const int64_t groups = (a.tokens + a.group - 1) / a.group;
+    if (groups > kMaxThreads / kOpThreads) return fail(SAGE_E_UNSUPPORTED, "sage_cache8_append: too many rows for one launch");
+    const int units = longer ? (2 * a.heads + 3) / 4 : 2 * a.heads;
+    const int64_t most = kWriteWorkgroups / groups;
+    const dim3 grid((unsigned)groups, (unsigned)(most < 1 ? 1 : most < units ? most : units)), threads(kOpThreads);
     if (a.map) {
-        hipLaunchKernelGGL(cache8_map_kernel, dim3((unsigned)((a.tokens + kOpThreads - 1) / kOpThreads)), dim3(kOpThreads), 0, stream, a);
+        hipLaunchKernelGGL(cache8_map_kernel, dim3((unsigned)((a.tokens + kOpThreads - 1) / kOpThreads)), threads, 0, stream, a);
         if (int rc = check_launch("cache8_map_kernel")) return rc;
-        hipLaunchKernelGGL((cache8_write_blocks_kernel<LPR, T, Code, false>), grid, dim3(kOpThreads), 0, stream, a);
+        if (longer) hipLaunchKernelGGL((cache8_write_long_blocks_kernel<LPR, T, Code, false>), grid, threads, 0, stream, a);
+        else hipLaunchKernelGGL((cache8_write_blocks_kernel<LPR, T, Code, false>), grid, threads, 0, stream, a);
     } else {
-        hipLaunchKernelGGL((cache8_write_blocks_kernel<LPR, T, Code, true>), grid, dim3(kOpThreads), 0, stream, a);
+        if (longer) hipLaunchKernelGGL((cache8_write_long_blocks_kernel<LPR, T, Code, true>), grid, threads, 0, stream, a);
+        else hipLaunchKernelGGL((cache8_write_blocks_kernel<LPR, T, Code, true>), grid, threads, 0, stream, a);
     }
     return check_launch("cache8_write_blocks_kernel");
 }
@@ -493,6 +655,7 @@ int launch_cache8_append(const sage_append8_params& p8, void* workspace, hipStre
     a.slots = p.slots; a.wide = p.slots_int64 ? 1 : 0;
     a.map = maps_tokens(p8) ? (int32_t*)workspace : nullptr;
     a.slot_limit = p.pages * p.page_size; a.rows = p.tokens * p.heads_kv;
+    a.page_shift = log2_or_none(p.page_size); a.head_shift = log2_or_none(p.heads_kv);
     a.tokens = (int)p.tokens; a.page_size = (int)p.page_size; a.heads = (int)p.heads_kv; a.pieces = (int)(p.head_dim / 16);
     return p8.scales.codes == SAGE_CODE_INT8 ? launch_write<Int8>(a, p.dtype, stream) : launch_write<E4m3>(a, p.dtype, stream);
 }
