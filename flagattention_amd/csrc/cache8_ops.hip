@@ -488,13 +488,13 @@ struct ReadArgs {
     const int32_t* table;
     const int32_t* cu;
     int64_t table_stride, capacity;
-    int32_t seqs, total, page_size, pages, heads, pieces;  // pieces: of 8 codes, or 16 bytes, of a row
+    int32_t seqs, total, page_size, page_shift, pages, heads, pieces;  // pieces: of 8 codes, or 16 bytes, of a row
 };
 
 // OutT: codes become numbers of it; Code void: 16 bytes of a row are copied.
 template <typename OutT, typename Code>
 __global__ __launch_bounds__(kOpThreads) void cache_read_kernel(ReadArgs a) {
-    __shared__ int page_of[kReadRows], place_of[kReadRows];  // page -1: a row of zeros, -2: no row
+    __shared__ int page_of[kReadRows], place_of[kReadRows], block_of[kReadRows];  // page -1: a row of zeros, -2: no row
     __shared__ int ends;
     const int tid = threadIdx.x, t0 = blockIdx.x * kReadRows;
     if (tid == 0) ends = 0;
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(kOpThreads) void cache_read_kernel(ReadArgs a) {
             const int64_t pos = (int64_t)t - a.cu[seq];
             page = pos >= 0 ? -1 : -2;
             if (pos >= 0 && pos < a.capacity) {
-                const int64_t e = pos / a.page_size;
+                const int64_t e = quotient(pos, a.page_size, a.page_shift);
                 place = (int)(pos - e * a.page_size);
                 const int p = a.table[seq * a.table_stride + e];
                 if (p >= 0 && p < a.pages) page = p;
@@ -520,33 +520,56 @@ __global__ __launch_bounds__(kOpThreads) void cache_read_kernel(ReadArgs a) {
         }
         page_of[tid] = page;
         place_of[tid] = place;
+        if (!std::is_same<Code, void>::value) block_of[tid] = a.scales.of(place);
     }
     __syncthreads();
-    const int per_row = a.heads * a.pieces;
-    for (int i = tid; i < kReadRows * per_row; i += kOpThreads) {
-        const int r = i / per_row, q = i - r * per_row, h = q / a.pieces, c = q - h * a.pieces;
-        const int64_t page = page_of[r];
-        const int place = place_of[r];
-        if (page == -2) continue;
+    // pieces of the rows, a few of them on their way together
+    const int per_row = a.heads * a.pieces, all = kReadRows * per_row;
+    constexpr int BATCH = 2;
+    constexpr bool CODED = !std::is_same<Code, void>::value;
+    typedef typename std::conditional<CODED, v2i, v4i>::type piece;  // eight codes, or 16 bytes
+    for (int i0 = tid; i0 < all; i0 += BATCH * kOpThreads) {
+        piece w[BATCH][2];
+        float s[BATCH][2];
+        int row[BATCH], head[BATCH], part[BATCH];
+        bool write[BATCH];
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            unsigned char* to = a.dst[x] + (int64_t)(t0 + r) * a.ds_t[x] + h * a.ds_h[x];
-            const unsigned char* from = a.src[x] + page * a.ss_p[x] + h * a.ss_h[x] + place * a.ss_n[x];
-            if constexpr (std::is_same<Code, void>::value) {
-                *reinterpret_cast<v4i*>(to + 16 * c) = page >= 0 ? *reinterpret_cast<const v4i*>(from + 16 * c) : v4i{0, 0, 0, 0};
-            } else {
-                typedef OutT v8 __attribute__((ext_vector_type(8)));
-                v8 out = {};
-                if (page >= 0) {
-                    const BlockScales& b = a.scales;
-                    const float s = x ? b.v[page * b.v_p + h * b.v_h + b.of(place) * b.v_b] : b.k[page * b.k_p + h * b.k_h + b.of(place) * b.k_b];
-                    const f16x8 codes = to_f16<Code>(*reinterpret_cast<const v2i*>(from + 8 * c));
+        for (int e = 0; e < BATCH; e++) {
+            const int i = i0 + e * kOpThreads;
+            const int r = i < all ? i / per_row : 0, q = i - r * per_row;
+            row[e] = r; head[e] = q / a.pieces; part[e] = q - head[e] * a.pieces;
+            const int page = page_of[r], place = place_of[r];
+            write[e] = i < all && page != -2;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) out[j] = (OutT)((float)codes[j] * s);
+            for (int x = 0; x < 2; x++) {
+                w[e][x] = piece{};
+                s[e][x] = 0.0f;
+                if (i < all && page >= 0) {
+                    w[e][x] = *reinterpret_cast<const piece*>(a.src[x] + page * a.ss_p[x] + head[e] * a.ss_h[x] + place * a.ss_n[x] + (int)sizeof(piece) * part[e]);
+                    if constexpr (CODED) {
+                        const BlockScales& b = a.scales;
+                        s[e][x] = x ? b.v[page * b.v_p + head[e] * b.v_h + block_of[r] * b.v_b] : b.k[page * b.k_p + head[e] * b.k_h + block_of[r] * b.k_b];
+                    }
                 }
-                *reinterpret_cast<v8*>(to + 8 * c * (int)sizeof(OutT)) = out;
             }
         }
+#pragma unroll
+        for (int e = 0; e < BATCH; e++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                if (!write[e]) continue;
+                unsigned char* to = a.dst[x] + (int64_t)(t0 + row[e]) * a.ds_t[x] + head[e] * a.ds_h[x];
+                if constexpr (CODED) {
+                    typedef OutT v8 __attribute__((ext_vector_type(8)));
+                    const f16x8 codes = to_f16<Code>(w[e][x]);
+                    v8 out;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) out[j] = (OutT)((float)codes[j] * s[e][x]);
+                    *reinterpret_cast<v8*>(to + 8 * (int)sizeof(OutT) * part[e]) = out;
+                } else {
+                    *reinterpret_cast<v4i*>(to + 16 * part[e]) = w[e][x];
+                }
+            }
     }
 }
 
@@ -680,6 +703,7 @@ int launch_cache_read(const sage_read_params& p, hipStream_t stream) {
     if (coded) a.scales = block_scales(p.scales, p.page_size);
     a.table = p.block_table; a.cu = p.cu_seqlens; a.table_stride = p.table_stride;
     a.capacity = p.pages > 0 ? p.table_width * p.page_size : 0;
+    a.page_shift = log2_or_none(p.page_size);
     a.seqs = (int)p.seqs; a.total = (int)p.total; a.page_size = (int)p.page_size; a.pages = (int)p.pages; a.heads = (int)p.heads_kv;
     a.pieces = (int)(coded ? p.head_dim / 8 : p.head_dim * e / 16);
     const dim3 grid((unsigned)((p.total + kReadRows - 1) / kReadRows));

@@ -20,7 +20,8 @@
 namespace sage {
 namespace {
 
-constexpr int kPaged8Shares = 768;  // three workgroups on each compute unit
+constexpr int kPaged8Shares = 512;  // two workgroups on each compute unit
+constexpr int kPaged8Start = 3;    // chunks that an item's beginning and end cost
 constexpr float kUnit0 = 0x1p100f;   // unit of the weights before a scale is seen
 constexpr float kUnitTop = 16384.0f;
 
@@ -31,7 +32,7 @@ template <int D> __device__ __forceinline__ int paged8_v_swizzle(int row) {
 }
 
 template <int D, typename QT, typename Code, bool SEVERAL, bool PAGE16>
-__global__ __launch_bounds__(kPagedThreads, 3) void paged8_attn_kernel(PagedArgs a, BlockScales bs) {
+__global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 3 : 4) void paged8_attn_kernel(PagedArgs a, BlockScales bs) {
     using F16 = PV<_Float16>;
     constexpr int KLOADS = D / 64;        // 64 codes of a row each
     constexpr int CT = D / 16;            // 16-channel tiles
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(kPagedThreads, 3) void paged8_attn_kernel(PagedArgs
         pos = line.begin(blockIdx.x);
         end = line.begin(blockIdx.x + 1);
         if (pos >= end) return;
-        if (!find_run(a.seqs, pos, [&](int s) { return seq_chunks(a, s) * per_seq; }, seq, seq_begin)) return;
+        if (!find_run(a.seqs, pos, [&](int s) { return seq_units(a, s) * per_seq; }, seq, seq_begin)) return;
     }
     const int share_begin = pos;
 
@@ -77,52 +78,39 @@ __global__ __launch_bounds__(kPagedThreads, 3) void paged8_attn_kernel(PagedArgs
 
     while (pos < end) {
         // ---- the piece: chunks `first` .. of an item
-        const int len = seq_len(a, seq), chunks = seq_chunks(a, seq);
+        const int len = seq_len(a, seq), chunks = seq_chunks(a, seq), units = a.start + chunks;
         // (a workgroup per item: all items at once may be more than 31 bits of chunks)
-        const int item = a.shares == 0 ? blockIdx.x % per_seq : (pos - seq_begin) / chunks;
-        const int first = a.shares == 0 ? 0 : pos - seq_begin - item * chunks;
-        const int hk = item / a.row_tiles, row0 = item % a.row_tiles * (16 * row_waves);
-        const int n = min(chunks - first, end - pos);
-        const bool whole = n == chunks;
-        const int slot = 2 * (int)blockIdx.x + (pos != share_begin);
-        const int kbeg = first * kChunk, kend = min((first + n) * kChunk, len);
+        int item = blockIdx.x % per_seq, first = 0, n = chunks, before = 0;  // before: other pieces of the share
         const int oseq = seq;
-        pos += n;
-        if (a.shares != 0 && pos - seq_begin == chunks * per_seq) {
-            seq_begin = pos;
-            seq++;
+        if (a.shares != 0) {
+            item = (pos - seq_begin) / units;
+            const int begin = seq_begin + item * units, to = min(begin + units, end);
+            before = begin > share_begin ? 1 : 0;
+            first = max(pos - begin - a.start, 0);
+            n = max(to - begin - a.start, 0) - first;
+            pos = to;
+            if (pos - seq_begin == units * per_seq) {
+                seq_begin = pos;
+                seq++;
+            }
+            if (n == 0) continue;  // (nothing but units before its chunks)
+        } else {
+            pos = end;
         }
+        const int hk = item / a.row_tiles, row0 = item % a.row_tiles * (16 * row_waves);
+        const bool whole = n == chunks;
+        const int slot = 2 * (int)blockIdx.x + before;
+        const int kbeg = first * kChunk, kend = min((first + n) * kChunk, len);
 
         // this lane's row; rows past the last one multiply a copy of it
         const int wrow0 = row0 + 16 * row_wave, r = min(wrow0 + l16, rows - 1);
         const int mi = SEVERAL ? r / a.groups : 0, h = hk * a.groups + (SEVERAL ? r % a.groups : r);
         // Q, its channels in the order of K's: steps 2 t and 2 t + 1 take channels 64 t + 16 quad + 0 .. 7 and 8 .. 15
         f16x8 qf[2 * KLOADS];
-        float unit = 1.0f;  // of the row's scores: 2^(e - 15)
         {
             const unsigned char* qp = a.q + (int64_t)oseq * a.qs_s + (int64_t)h * a.qs_h + (int64_t)mi * a.qs_m + 32 * quad;
 #pragma unroll
             for (int t = 0; t < 2 * KLOADS; t++) qf[t] = *reinterpret_cast<const f16x8*>(qp + 128 * (t / 2) + 16 * (t % 2));
-            if constexpr (std::is_same<QT, __bf16>::value) {
-                float top = 0.0f;  // of the finite ones
-#pragma unroll
-                for (int t = 0; t < 2 * KLOADS; t++)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float x = __builtin_fabsf((float)__builtin_bit_cast(bf16x8, qf[t])[i]);
-                        top = fmaxf(top, x < INFINITY ? x : 0.0f);
-                    }
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const int e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 15;
-                unit = __builtin_amdgcn_ldexpf(1.0f, e - 15);
-#pragma unroll
-                for (int t = 0; t < 2 * KLOADS; t++) {
-                    const bf16x8 x = __builtin_bit_cast(bf16x8, qf[t]);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) qf[t][i] = (_Float16)__builtin_amdgcn_ldexpf((float)x[i], 15 - e);
-                }
-            }
         }
         const int my_last = len - a.M + mi;                                      // last key the row sees
         const int all_see = len - a.M + min(wrow0, rows - 1) / a.groups;  // ... the wave's first row
@@ -211,6 +199,29 @@ __global__ __launch_bounds__(kPagedThreads, 3) void paged8_attn_kernel(PagedArgs
             seen = load_tile(key0);
             load_entries(key0 + kstep);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        // (after the first tile has been requested)
+        float unit = 1.0f;  // of the row's scores: 2^(e - 15)
+                    if constexpr (std::is_same<QT, __bf16>::value) {
+                        float top = 0.0f;  // of the finite ones
+        #pragma unroll
+                        for (int t = 0; t < 2 * KLOADS; t++)
+        #pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                const float x = __builtin_fabsf((float)__builtin_bit_cast(bf16x8, qf[t])[i]);
+                                top = fmaxf(top, x < INFINITY ? x : 0.0f);
+                            }
+                        top = fmaxf(top, __shfl_xor(top, 16));
+                        top = fmaxf(top, __shfl_xor(top, 32));
+                        const int e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 15;
+                        unit = __builtin_amdgcn_ldexpf(1.0f, e - 15);
+        #pragma unroll
+                        for (int t = 0; t < 2 * KLOADS; t++) {
+                            const bf16x8 x = __builtin_bit_cast(bf16x8, qf[t]);
+        #pragma unroll
+                            for (int i = 0; i < 8; i++) qf[t][i] = (_Float16)__builtin_amdgcn_ldexpf((float)x[i], 15 - e);
+                        }
+                    }
         for (; key0 < kend; key0 += kstep) {
             // ---- S^T = K.Q^T: register i of score tile u is key key0 + 16 u + 4 quad + i of the lane's row
             v4f s[2];
@@ -385,7 +396,7 @@ __global__ __launch_bounds__(kPagedThreads, 3) void paged8_attn_kernel(PagedArgs
 
 }  // namespace
 
-int64_t paged8_workspace_bytes(const sage_paged8_params& p) { return plan_bytes(plan_paged(p.paged, kPaged8Shares), p.paged.head_dim); }
+int64_t paged8_workspace_bytes(const sage_paged8_params& p) { return plan_bytes(plan_paged(p.paged, kPaged8Shares, kPaged8Start), p.paged.head_dim); }
 
 template <int D, typename QT, typename Code>
 static int launch_paged8(const PagedArgs& a, const BlockScales& bs, const PagedPlan& plan, hipStream_t stream) {
@@ -409,7 +420,7 @@ static int launch_paged8(const sage_paged_params& p, const PagedArgs& a, const B
 }
 
 int launch_paged8_attn(const sage_paged8_params& p, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-    PagedPlan plan = plan_paged(p.paged, kPaged8Shares);
+    PagedPlan plan = plan_paged(p.paged, kPaged8Shares, kPaged8Start);
     if (!workspace || workspace_bytes < plan_bytes(plan, p.paged.head_dim)) plan.shares = 0;  // (nothing is cut then)
     const PagedArgs a = paged_args(p.paged, plan, workspace, 1);
     const BlockScales bs = block_scales(p.scales, p.paged.page_size);

@@ -325,7 +325,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attn_kernel(PagedArgs 
 
 }  // namespace
 
-int64_t paged_workspace_bytes(const sage_paged_params& p) { return plan_bytes(plan_paged(p, kPagedShares), p.head_dim); }
+int64_t paged_workspace_bytes(const sage_paged_params& p) { return plan_bytes(plan_paged(p, kPagedShares, 0), p.head_dim); }
 
 template <int D, typename VT>
 static int launch_paged(const PagedArgs& a, const PagedPlan& plan, hipStream_t stream) {
@@ -342,7 +342,7 @@ static int launch_paged(const PagedArgs& a, const PagedPlan& plan, hipStream_t s
 }
 
 int launch_paged_attn(const sage_paged_params& p, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-    PagedPlan plan = plan_paged(p, kPagedShares);
+    PagedPlan plan = plan_paged(p, kPagedShares, 0);
     if (!workspace || workspace_bytes < plan_bytes(plan, p.head_dim)) plan.shares = 0;  // (nothing is cut then)
     const PagedArgs a = paged_args(p, plan, workspace, 2);
     if (p.head_dim == 128) return p.dtype == SAGE_BF16 ? launch_paged<128, __bf16>(a, plan, stream) : launch_paged<128, _Float16>(a, plan, stream);

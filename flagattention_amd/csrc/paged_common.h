@@ -30,6 +30,7 @@ struct PagedArgs {
     int32_t row_waves;             // waves that share an item's rows, sixteen each: 1, 2 or 4
     int32_t row_tiles, tile_rows;  // items that the rows of a K/V head make; rows of one
     int32_t shares;                // equal shares of the line; 0: a workgroup per item
+    int32_t start;                 // units of the line before an item's chunks
     float qk_scale;                // sm_scale * log2(e)
     float* part_o;                 // [2 * shares][tile_rows][D]
     float* part_lse;               // [2 * shares][tile_rows], base 2
@@ -37,11 +38,13 @@ struct PagedArgs {
 
 __device__ __forceinline__ int seq_len(const PagedArgs& a, int s) { return min(max(a.lens[s], 0), a.capacity); }
 __device__ __forceinline__ int seq_chunks(const PagedArgs& a, int s) { return max((seq_len(a, s) + kChunk - 1) / kChunk, 1); }
+// What an item takes on the line: its chunks, after `start` units for what its beginning and end cost.
+__device__ __forceinline__ int seq_units(const PagedArgs& a, int s) { return a.start + seq_chunks(a, s); }
 
-// Chunks of all sequences.
+// Units of all sequences.
 __device__ __forceinline__ int line_total(const PagedArgs& a) {
     int sum = 0;
-    for (int s = threadIdx.x & 63; s < a.seqs; s += 64) sum += seq_chunks(a, s);
+    for (int s = threadIdx.x & 63; s < a.seqs; s += 64) sum += seq_units(a, s);
     return wave_sum(sum) * a.Hkv * a.row_tiles;
 }
 
@@ -57,9 +60,9 @@ __global__ __launch_bounds__(kCombineThreads) void paged_combine_kernel(PagedArg
     __shared__ v4f sm_acc[kCombineThreads];
     const int per_seq = a.Hkv * a.row_tiles;
     int seq, item, begin;  // begin: of the item on the line
-    int all = 0, before = 0;  // chunks of the sequences; of those before this workgroup's
+    int all = 0, before = 0;  // units of the sequences; of those before this workgroup's
     for (int i = threadIdx.x & 63; i < a.seqs; i += 64) {
-        const int n = seq_chunks(a, i);
+        const int n = seq_units(a, i);
         all += n;
         before += i < (int)blockIdx.x / per_seq ? n : 0;
     }
@@ -67,17 +70,16 @@ __global__ __launch_bounds__(kCombineThreads) void paged_combine_kernel(PagedArg
     if (BY_ITEM) {
         seq = blockIdx.x / per_seq;
         item = blockIdx.x % per_seq;
-        begin = wave_sum(before) * per_seq + item * seq_chunks(a, seq);
+        begin = wave_sum(before) * per_seq + item * seq_units(a, seq);
     } else {
         const int pos = line.begin(blockIdx.x + 1);
         if (pos >= line.begin(blockIdx.x + 2)) return;  // (the shares from here on are empty)
-        if (!find_run(a.seqs, pos, [&](int s) { return seq_chunks(a, s) * per_seq; }, seq, begin)) return;
-        item = (pos - begin) / seq_chunks(a, seq);
-        begin += item * seq_chunks(a, seq);
-        if (begin == pos || line.owner(begin) != (int)blockIdx.x) return;
+        if (!find_run(a.seqs, pos, [&](int s) { return seq_units(a, s) * per_seq; }, seq, begin)) return;
+        item = (pos - begin) / seq_units(a, seq);
+        begin += item * seq_units(a, seq);
+        if (line.owner(begin + a.start) != (int)blockIdx.x) return;
     }
-    const int chunks = seq_chunks(a, seq);
-    const int first = line.owner(begin), last = line.owner(begin + chunks - 1);
+    const int first = line.owner(begin + a.start), last = line.owner(begin + seq_units(a, seq) - 1);
     if (first == last) return;  // (whole)
     const int hk = item / a.row_tiles, row0 = item % a.row_tiles * (16 * a.row_waves), rows = a.groups * a.M;
     const int c = 4 * (threadIdx.x % TPR), sg = (threadIdx.x / TPR) % SG;
@@ -85,7 +87,7 @@ __global__ __launch_bounds__(kCombineThreads) void paged_combine_kernel(PagedArg
     if (row0 + (int)blockIdx.y * ROWS >= rows) return;
     const bool ok = trow < a.tile_rows && row0 + trow < rows;
     const int srow = ok ? trow : 0;
-    auto slot = [&](int w) { return (int64_t)(2 * w + (w == first && begin != line.begin(w))) * a.tile_rows + srow; };
+    auto slot = [&](int w) { return (int64_t)(2 * w + (w == first && begin > line.begin(w))) * a.tile_rows + srow; };
     float m = -INFINITY, den = 0.0f;
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int w0 = first + sg; w0 <= last; w0 += SG * kBatch) {
@@ -146,10 +148,10 @@ __global__ __launch_bounds__(kCombineThreads) void paged_combine_kernel(PagedArg
 }
 
 struct PagedPlan {
-    int64_t row_waves, row_tiles, tile_rows, capacity, items, shares;
+    int64_t row_waves, row_tiles, tile_rows, capacity, items, shares, start;
 };
 
-PagedPlan plan_paged(const sage_paged_params& p, int most_shares) {
+PagedPlan plan_paged(const sage_paged_params& p, int most_shares, int start) {
     PagedPlan plan;
     const int64_t rows = p.heads_q / p.heads_kv * p.new_tokens;
     plan.row_waves = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
@@ -165,7 +167,8 @@ PagedPlan plan_paged(const sage_paged_params& p, int most_shares) {
     // 700 15.7 and 19.5, 128 x 8, up to 500 36.5 and 48, 1000 x 8, up to 1500 378 and 451; D64: 128 x 16, up to 2048 111 and 119.
     const int64_t chunks = (plan.capacity + kChunk - 1) / kChunk;
     plan.shares = plan.items * chunks < most_shares ? plan.items * chunks : most_shares;
-    if (chunks <= 5 + 6 * plan.items / kPagedWhole || plan.items > 0x7fffffffLL / chunks) plan.shares = 0;
+    if (chunks <= 5 + 6 * plan.items / kPagedWhole || plan.items > 0x7fffffffLL / (chunks + start)) plan.shares = 0;
+    plan.start = plan.shares < most_shares ? 0 : start;  // (a share for every chunk: none begins two items)
     return plan;
 }
 
@@ -185,7 +188,7 @@ PagedArgs paged_args(const sage_paged_params& p, const PagedPlan& plan, void* wo
     a.pages = (int)p.pages; a.page_size = (int)p.page_size;
     a.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)p.page_size) : -1;
     a.capacity = (int)plan.capacity; a.row_tiles = (int)plan.row_tiles; a.row_waves = (int)plan.row_waves; a.tile_rows = (int)plan.tile_rows;
-    a.shares = (int)plan.shares;
+    a.shares = (int)plan.shares; a.start = (int)plan.start;
     a.qk_scale = p.sm_scale * 1.44269504089f;
     a.part_o = (float*)workspace;
     a.part_lse = a.part_o + 2 * plan.shares * plan.tile_rows * p.head_dim;
