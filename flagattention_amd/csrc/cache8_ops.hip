@@ -15,7 +15,9 @@ using namespace attn;
 constexpr int kOpThreads = 256;
 constexpr int kMostBlock = 1024;     // tokens that share a scale
 constexpr int kScanTokens = 256;    // calls of up to so many tokens look their slots over instead of mapping them
-constexpr int kWriteWorkgroups = 4096;  // that a write of blocks makes where it can
+// Workgroups that a write of blocks makes where it can (16384 tokens of 8 heads, D128, bf16, blocks of 16 and 32: 512 32 and 34 us, 1024 26.4 and 34,
+// 2048 28.7 and 36, 4096 30.6 and 42: a wave that goes through more heads looks its tokens up less often).
+constexpr int kWriteWorkgroups = 1024;
 constexpr float kSmallest = 0x1p-100f;
 
 __device__ __forceinline__ int64_t index_at(const void* list, int wide, int64_t i) {
@@ -399,16 +401,17 @@ __global__ __launch_bounds__(kOpThreads, 4) void cache8_write_blocks_kernel(Writ
     }
 }
 
-// Longer blocks: a workgroup takes a block, its waves a head of K or V each, and goes over the rows twice where they are more than a wave
-// keeps.
+// Longer blocks: a workgroup takes a block and goes through heads of K and V, its waves sharing the rows; it goes over them twice where they are
+// more than it keeps in registers (128 of them at D128, 256 at D64).
 template <int LPR, typename T, typename Code, bool SCAN>
-__global__ __launch_bounds__(kOpThreads, 4) void cache8_write_long_blocks_kernel(WriteArgs a) {
-    constexpr int ROWS = 64 / LPR, KEEP = 4, WAVES = kOpThreads / 64;
+__global__ __launch_bounds__(kOpThreads, sizeof(T) == 4 ? 3 : 4) void cache8_write_long_blocks_kernel(WriteArgs a) {
+    constexpr int ROWS = 64 / LPR, KEEP = 4, WAVES = kOpThreads / 64, PASS = KEEP * WAVES * ROWS;
     __shared__ int token[kMostBlock];
     __shared__ int lowest;
+    __shared__ unsigned tops[2][WAVES];  // in turn, so that a barrier a unit is enough
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int block = a.scales.block;
-    const int rr = lane / LPR, c = lane % LPR;
+    const int my_row = wave * ROWS + lane / LPR, c = lane % LPR;
     Candidates cand = look(a);
     for (; cand.todo != 0; cand.todo &= cand.todo - 1) {
         const int looker = __builtin_ctzll(cand.todo);
@@ -432,7 +435,7 @@ __global__ __launch_bounds__(kOpThreads, 4) void cache8_write_long_blocks_kernel
         const bool begun = lowest == 0;
         const int64_t page = quotient(begin, a.page_size, a.page_shift);
         const int at = (int)(begin - page * a.page_size), b = a.scales.of(at);
-        for (int unit = blockIdx.y * WAVES + wave; unit < 2 * a.heads; unit += gridDim.y * WAVES) {
+        for (int unit = blockIdx.y, turn = 0; unit < 2 * a.heads; unit += gridDim.y, turn ^= 1) {
             const int x = unit & 1, h = unit >> 1;
             const unsigned char* src = a.src[x] + h * a.ss_h[x] + c * (16 * (int)sizeof(T));
             unsigned char* dst = a.dst[x] + page * a.ds_p[x] + h * a.ds_h[x] + at * a.ds_n[x] + 16 * c;
@@ -442,43 +445,48 @@ __global__ __launch_bounds__(kOpThreads, 4) void cache8_write_long_blocks_kernel
             auto load = [&](int p0) {  // rows of places p0 ..; who: their tokens, -1: none, -2: no such place
 #pragma unroll
                 for (int e = 0; e < KEEP; e++) {
-                    const int p = p0 + e * ROWS + rr;
+                    const int p = p0 + e * (WAVES * ROWS) + my_row;
                     who[e] = p < block && c < a.pieces ? token[p] : -2;
                     if (who[e] >= 0) rows[e].load(src + who[e] * a.ss_t[x]);
                     else rows[e].clear();
                 }
             };
             unsigned top = 0;
-            for (int p0 = 0; p0 < block; p0 += KEEP * ROWS) {
+            for (int p0 = 0; p0 < block; p0 += PASS) {
                 load(p0);
 #pragma unroll
                 for (int e = 0; e < KEEP; e++) top = rows[e].top(top);
             }
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
+            if (lane == 0) tops[turn][wave] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) top = max(top, tops[turn][w]);
             const float s = next_scale<Code>(was, Row16<T>::size(top));
             const float inv = s < INFINITY ? 1.0f / s : 0.0f;
-            for (int p0 = 0; p0 < block; p0 += KEEP * ROWS) {
-                load(p0);
+            for (int p0 = 0; p0 < block; p0 += PASS) {
+                if (block > PASS) load(p0);
 #pragma unroll
                 for (int e = 0; e < KEEP; e++) {
+                    if (p0 + e * (WAVES * ROWS) >= block) break;
                     if (!(s < INFINITY)) rows[e].clear();  // (NaN: an entry was not finite)
                     const v4i w = Rounding<Code>::codes(rows[e], s, inv);
                     if (who[e] >= 0 || (who[e] == -1 && begun))  // (zeros where a block begins)
-                        *reinterpret_cast<v4i*>(dst + (p0 + e * ROWS + rr) * a.ds_n[x]) = w;
+                        *reinterpret_cast<v4i*>(dst + (p0 + e * (WAVES * ROWS) + my_row) * a.ds_n[x]) = w;
                 }
             }
             if (s != was && s == s && !begun)
-                for (int p = rr; p < block; p += ROWS)
+                for (int p = my_row; p < block; p += WAVES * ROWS)
                     if (c < a.pieces && token[p] < 0) convert<Code>(dst + p * a.ds_n[x], was, s);
-            if (lane == 0) scale_of(a, x, page, h, b) = s;
+            if (tid == 0) scale_of(a, x, page, h, b) = s;
         }
     }
 }
 
-// Packed rows of sequences from the pages of a cache.  A workgroup takes kReadRows rows: one search over the sequences for the first,
-// the others go on from there.
-constexpr int kReadRows = 16;
+// Packed rows of sequences from the pages of a cache.  A workgroup takes some rows, about 1024 pieces of K and as many of V: one search over the
+// sequences for the first row, the others go on from there.
+constexpr int kMostReadRows = 32;
 
 struct ReadArgs {
     const unsigned char* src[2];  // caches
@@ -488,22 +496,22 @@ struct ReadArgs {
     const int32_t* table;
     const int32_t* cu;
     int64_t table_stride, capacity;
-    int32_t seqs, total, page_size, page_shift, pages, heads, pieces;  // pieces: of 8 codes, or 16 bytes, of a row
+    int32_t seqs, total, page_size, page_shift, pages, heads, pieces, rows;  // pieces: of 8 codes, or 16 bytes, of a row; rows: of a workgroup
 };
 
 // OutT: codes become numbers of it; Code void: 16 bytes of a row are copied.
 template <typename OutT, typename Code>
 __global__ __launch_bounds__(kOpThreads) void cache_read_kernel(ReadArgs a) {
-    __shared__ int page_of[kReadRows], place_of[kReadRows], block_of[kReadRows];  // page -1: a row of zeros, -2: no row
+    __shared__ int page_of[kMostReadRows], place_of[kMostReadRows], block_of[kMostReadRows];  // page -1: a row of zeros, -2: no row
     __shared__ int ends;
-    const int tid = threadIdx.x, t0 = blockIdx.x * kReadRows;
+    const int tid = threadIdx.x, t0 = blockIdx.x * a.rows;
     if (tid == 0) ends = 0;
     __syncthreads();
     int before = 0;  // sequences that end at or before row t0
     for (int s = tid; s < a.seqs; s += kOpThreads) before += a.cu[s + 1] <= t0 ? 1 : 0;
     if (before) atomicAdd(&ends, before);
     __syncthreads();
-    if (tid < kReadRows) {
+    if (tid < a.rows) {
         const int t = t0 + tid;
         int seq = ends;
         while (seq < a.seqs && a.cu[seq + 1] <= t) seq++;
@@ -524,8 +532,8 @@ __global__ __launch_bounds__(kOpThreads) void cache_read_kernel(ReadArgs a) {
     }
     __syncthreads();
     // pieces of the rows, a few of them on their way together
-    const int per_row = a.heads * a.pieces, all = kReadRows * per_row;
-    constexpr int BATCH = 2;
+    const int per_row = a.heads * a.pieces, all = a.rows * per_row;
+    constexpr int BATCH = 4;
     constexpr bool CODED = !std::is_same<Code, void>::value;
     typedef typename std::conditional<CODED, v2i, v4i>::type piece;  // eight codes, or 16 bytes
     for (int i0 = tid; i0 < all; i0 += BATCH * kOpThreads) {
@@ -632,10 +640,11 @@ static int launch_write(WriteArgs a, hipStream_t stream) {
     const int block = a.scales.block;
     const bool longer = block > kKeep * ROWS;
     a.span = a.map && block <= ROWS && a.scales.shift >= 0 ? LPR * block : 64;
-    a.group = longer ? (a.map ? block < 64 ? block : 64 : 1) : a.map ? 4 * block < 64 ? 4 * block : 64 : kScanGroup;
+    const int per_workgroup = kOpThreads / a.span * block;  // tokens of the blocks that its waves take at a time
+    a.group = longer ? (a.map ? block < 64 ? block : 64 : 1) : a.map ? per_workgroup < 64 ? per_workgroup : 64 : kScanGroup;
     const int64_t groups = (a.tokens + a.group - 1) / a.group;
     if (groups > kMaxThreads / kOpThreads) return fail(SAGE_E_UNSUPPORTED, "sage_cache8_append: too many rows for one launch");
-    const int units = longer ? (2 * a.heads + 3) / 4 : 2 * a.heads;
+    const int units = 2 * a.heads;
     const int64_t most = kWriteWorkgroups / groups;
     const dim3 grid((unsigned)groups, (unsigned)(most < 1 ? 1 : most < units ? most : units)), threads(kOpThreads);
     if (a.map) {
@@ -706,7 +715,9 @@ int launch_cache_read(const sage_read_params& p, hipStream_t stream) {
     a.page_shift = log2_or_none(p.page_size);
     a.seqs = (int)p.seqs; a.total = (int)p.total; a.page_size = (int)p.page_size; a.pages = (int)p.pages; a.heads = (int)p.heads_kv;
     a.pieces = (int)(coded ? p.head_dim / 8 : p.head_dim * e / 16);
-    const dim3 grid((unsigned)((p.total + kReadRows - 1) / kReadRows));
+    // (8 heads, D128: 8 rows 20.3 us for 17700 tokens, 16 rows 22; 1 head: 16 rows 12, 8 rows 16)
+    for (a.rows = 4; a.rows < kMostReadRows && a.rows * a.heads * a.pieces < 1024;) a.rows *= 2;
+    const dim3 grid((unsigned)((p.total + a.rows - 1) / a.rows));
     if ((int64_t)grid.x > kMaxThreads / kOpThreads) return fail(SAGE_E_UNSUPPORTED, "sage_cache_read: too many rows for one launch");
     if (p.scales.codes == SAGE_CODE_INT8) launch_read<Int8>(a, p.out_dtype, grid, stream);
     else if (coded) launch_read<E4m3>(a, p.out_dtype, grid, stream);
