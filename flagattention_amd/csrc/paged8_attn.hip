@@ -244,8 +244,9 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
             }
             const float v_scale = lane >= 32 && ((seen >> (lane & 31)) & 1) ? sc : 0.0f;
             float shrink = 1.0f;  // of the weights' unit
-            if (__builtin_amdgcn_ballot_w64(v_scale * w_unit > kUnitTop && v_scale < INFINITY) != 0) {
-                float top = v_scale < INFINITY ? v_scale : 0.0f;
+            const float v_size = __builtin_fabsf(v_scale);
+            if (__builtin_amdgcn_ballot_w64(v_size * w_unit > kUnitTop && v_size < INFINITY) != 0) {
+                float top = v_size < INFINITY ? v_size : 0.0f;
 #pragma unroll
                 for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
                 const float unit_now = __builtin_amdgcn_ldexpf(kUnitTop, -__builtin_amdgcn_frexp_expf(top));

@@ -635,3 +635,95 @@ def test_another_stream_and_repeated_calls(gpu_device):
             again = flag_attn.paged_attention(q, cache[0], cache[1], wide, n, **scales)
         side.synchronize()
         assert same_bits(first, again)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_offsets_beyond_32_bits(gpu_device, codes):
+    """Caches of more than 2^32 bytes: the last pages and the first ones, in every operator."""
+    import flag_attn
+
+    g = torch.Generator().manual_seed(43)
+    dev, hk, page, d, pages = gpu_device, 8, 16, 128, (1 << 32) // (8 * 16 * 128) + 40
+    kc, vc = (torch.empty(pages, hk, page, d, dtype=torch.int8, device=dev).view(CODES[codes]) for _ in range(2))
+    ks, vs = (torch.zeros(pages, hk, 4, device=dev) for _ in range(2))
+    scales = dict(k_scale=ks, v_scale=vs)
+    places = [pages - 1, 0, pages - 20, 1]
+    small = (torch.zeros(5, hk, page, d, dtype=torch.int8).view(CODES[codes]), torch.zeros(5, hk, page, d, dtype=torch.int8).view(CODES[codes]), torch.zeros(5, hk, 4), torch.zeros(5, hk, 4))
+    k, v = (torch.randn(64, hk, d, generator=g).to(BF16) for _ in range(2))
+    here = torch.arange(64)
+    slots = torch.tensor(places).repeat_interleave(page) * page + here % page
+    flag_attn.append_to_cache(k.to(dev), v.to(dev), kc, vc, slots.to(dev), **scales)
+    small = CO.append(k, v, small[0], small[1], here, small[2], small[3])
+    flag_attn.copy_pages(kc, vc, torch.tensor([pages - 20], device=dev), torch.tensor([pages - 3], device=dev), **scales)
+    places[2] = pages - 3
+    for t, w in zip((kc, vc, ks, vs), small):
+        kind = torch.int8 if t.element_size() == 1 else torch.float32
+        assert same_numbers(t.view(kind)[torch.tensor(places, device=dev)].view(t.dtype), w[:4])
+    table, cu = torch.tensor([places], dtype=torch.int32), torch.tensor([0, 64], dtype=torch.int32)
+    for got, c, s in zip(flag_attn.read_cache(kc, vc, table.to(dev), cu.to(dev), 64, **scales), small[:2], small[2:]):
+        assert same_numbers(got, CO.read(c, s, torch.arange(4)[None], cu, 64, BF16))
+    q = torch.randn(1, 16, d, generator=g).to(BF16)
+    o = flag_attn.paged_attention(q.to(dev), kc, vc, table.to(dev), torch.tensor([64], dtype=torch.int32, device=dev), **scales)
+    want, _, tol, _ = CO.paged(q, *small, torch.arange(4)[None], [64])
+    CO.assert_close(o.cpu(), want, tol)
+
+
+@pytest.mark.parametrize("tokens", [40, 600])
+@pytest.mark.parametrize("blocks", [16, 4, 1])
+def test_a_slot_that_occurs_twice(gpu_device, tokens, blocks):
+    """Not allowed; all the same every other block is right, and the place holds a row of one of the two."""
+    import flag_attn
+
+    g = torch.Generator().manual_seed(44)
+    dev, pages = gpu_device, tokens // 16 + 2
+    slots = torch.arange(tokens)
+    slots[17] = 3
+    x, cache, _ = write_case(pages, 2, 16, blocks, 64, INT8, BF16, slots, g)
+    kc, vc, ks, vs = (t.to(dev) for t in cache)
+    flag_attn.append_to_cache(x[0].to(dev), x[1].to(dev), kc, vc, slots.to(dev), k_scale=ks, v_scale=vs)
+    wants = []
+    for lost in (3, 17):
+        s = slots.clone()
+        s[lost] = -1
+        wants.append(CO.append(x[0], x[1], cache[0], cache[1], s, cache[2], cache[3]))
+    for got, a, b in zip((kc, vc, ks, vs), *wants):
+        assert same_numbers(got[1:], a[1:])
+        if blocks != 16:
+            assert same_numbers(got, a) or same_numbers(got, b)
+
+
+def test_negative_scales(gpu_device):
+    """Scales that a program wrote itself, of either sign and far apart, count as they are."""
+    g = torch.Generator().manual_seed(45)
+    kc, vc, ks, vs = make_cache(10, 2, 16, 4, 64, INT8, g)
+    ks, vs = -ks, vs * torch.where(torch.rand(vs.shape, generator=g) < 0.5, -1.0, 1000.0)
+    table, _ = make_table([90, 33], 16, 10, g)
+    for dtype in (BF16, FP16):
+        check(torch.randn(2, 4, 64, generator=g).to(dtype), (kc, vc, ks, vs), table, [90, 33], gpu_device)
+
+
+def test_caches_and_lists_without_entries(gpu_device):
+    """No pages, no entries of a table, no tokens, no sequences: zero rows, or nothing to do."""
+    import flag_attn
+
+    dev = gpu_device
+
+    def cache(pages):
+        return [torch.zeros(pages, 2, 16, 64, dtype=INT8, device=dev) for _ in range(2)], dict(k_scale=torch.zeros(pages, 2, 4, device=dev), v_scale=torch.zeros(pages, 2, 4, device=dev))
+
+    q = torch.ones(3, 4, 64, dtype=BF16, device=dev)
+    lens = torch.tensor([5, 0, 1], dtype=torch.int32, device=dev)
+    for pages, width in ((0, 2), (4, 0), (0, 0)):
+        c, s = cache(pages)
+        table = torch.zeros(3, width, dtype=torch.int32, device=dev)
+        o, norm = flag_attn.paged_attention(q, *c, table, lens, return_log_normalizer=True, **s)
+        assert not o.any() and (norm == -math.inf).all()
+        k, v = flag_attn.read_cache(*c, table, torch.tensor([0, 5, 5, 6], dtype=torch.int32, device=dev), 6, **s)
+        assert k.shape == (6, 2, 64) and not k.any() and not v.any()
+    c, s = cache(4)
+    row = torch.ones(0, 2, 64, dtype=BF16, device=dev)
+    flag_attn.append_to_cache(row, row, *c, torch.zeros(0, dtype=torch.int64, device=dev), **s)
+    flag_attn.copy_pages(*c, torch.zeros(0, dtype=torch.int64, device=dev), torch.zeros(0, dtype=torch.int64, device=dev), **s)
+    k, v = flag_attn.read_cache(*c, torch.zeros(0, 3, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev), 0, **s)
+    assert k.shape == (0, 2, 64)
+    assert flag_attn.paged_attention(q[:0], *c, torch.zeros(0, 3, dtype=torch.int32, device=dev), lens[:0], **s).shape == (0, 4, 64)
