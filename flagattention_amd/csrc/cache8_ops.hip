@@ -310,16 +310,18 @@ __global__ __launch_bounds__(kOpThreads, 4) void cache8_write_blocks_kernel(Writ
     __shared__ int found[SCAN ? kScanGroup * 64 : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int block = a.scales.block, span = a.span, sub = lane / span, c = lane % LPR;
-    Candidates cand = look(a);
+    constexpr int EACH = SCAN ? kScanTokens / kOpThreads : 1;
+    int64_t slot[EACH];  // (requested beside those that look() asks for)
     if constexpr (SCAN) {
-        constexpr int EACH = kScanTokens / kOpThreads;
-        found[threadIdx.x] = -1;
-        int64_t slot[EACH];
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
             const int i = e * kOpThreads + threadIdx.x;
             slot[e] = i < a.tokens ? index_at(a.slots, a.wide, i) : -1;
         }
+        found[threadIdx.x] = -1;
+    }
+    Candidates cand = look(a);
+    if constexpr (SCAN) {
         __syncthreads();
         int n = 0;
         for (unsigned long long todo = cand.todo; todo != 0; todo &= todo - 1, n++) {

@@ -428,7 +428,10 @@ static int check_scales(const char* who, const sage_cache_scales& s, int64_t pag
 static int check_paged8(const char* who, const sage_paged8_params* p, bool& nothing) {
     if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);
     if (int rc = check_paged(who, &p->paged, nothing, 1)) return rc;
-    return nothing ? SAGE_OK : check_scales(who, p->scales, p->paged.page_size);
+    if (nothing) return SAGE_OK;
+    for (int64_t x : {p->paged.k_cache.stride_b, p->paged.v_cache.stride_b})
+        if (x < 0 || x >= (1LL << 32)) return fail(SAGE_E_UNSUPPORTED, "%s: page strides of the caches must stay between 0 and 2^32", who);
+    return check_scales(who, p->scales, p->paged.page_size);
 }
 
 extern "C" int64_t sage_paged8_attn_workspace_bytes(const sage_paged8_params* p) {

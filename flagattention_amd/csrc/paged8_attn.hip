@@ -31,6 +31,11 @@ template <int D> __device__ __forceinline__ int paged8_v_swizzle(int row) {
     return D == 128 ? ((row >> 1) & 3) | ((row >> 2) & 4) : ((row >> 2) & 1) | ((row >> 3) & 2);
 }
 
+// Of a row in a cache.  (strides below 2^32: a product of 64-bit numbers costs three times as many instructions)
+__device__ __forceinline__ int64_t row_offset(int page, int place, int64_t stride_p, int64_t stride_n) {
+    return (int64_t)((uint64_t)(unsigned)page * (unsigned)stride_p + (uint64_t)(unsigned)place * (unsigned)stride_n);
+}
+
 template <int D, typename QT, typename Code, bool SEVERAL, bool PAGE16>
 __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 3 : 4) void paged8_attn_kernel(PagedArgs a, BlockScales bs) {
     using F16 = PV<_Float16>;
@@ -150,8 +155,8 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
                     const bool ok = (unsigned)entry[u] < (unsigned)a.pages;
                     if (!ok) seen &= u ? 0xffffu : 0xffff0000u;
                     const int page = ok ? entry[u] : 0, at = place_of(key0 + 16 * u);
-                    kp[u] = kg + (int64_t)page * a.ks_p + (int64_t)at * a.ks_n;
-                    vp[u] = vg + (int64_t)page * a.vs_p + (int64_t)at * a.vs_n;
+                    kp[u] = kg + row_offset(page, at, a.ks_p, a.ks_n);
+                    vp[u] = vg + row_offset(page, at, a.vs_p, a.vs_n);
                     pages[u] = page;
                     places[u] = at;
                 }
@@ -170,7 +175,7 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
                 const bool ok = (unsigned)entry[0] < (unsigned)a.pages;
                 seen &= (unsigned)__builtin_amdgcn_ballot_w64(ok);
                 const int page = ok ? entry[0] : 0, at = ok ? place_of(min(key0 + (lane & 31), kend - 1)) : 0;
-                const int64_t ko = (int64_t)page * a.ks_p + (int64_t)at * a.ks_n, vo = (int64_t)page * a.vs_p + (int64_t)at * a.vs_n;
+                const int64_t ko = row_offset(page, at, a.ks_p, a.ks_n), vo = row_offset(page, at, a.vs_p, a.vs_n);
                 auto from = [&](int64_t x, int who) {  // the lane that knows the row
                     return ((int64_t)__shfl((int)(x >> 32), who) << 32) | (unsigned)__shfl((int)(unsigned)x, who);
                 };
