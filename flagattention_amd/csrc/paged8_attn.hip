@@ -14,14 +14,26 @@
 // registers 16 codes a lane, so that a load holds two steps of channels, and Q's channels lie in the same order; V tiles go through
 // the wave's slice of LDS as codes, from where they are read transposed, eight keys of a channel a lane, and become fp16 after that.
 // The 64 scales of a tile are one load, a lane each, and go through LDS to the lanes that hold their keys' scores.
+//
+// A beginning and an end cost about what two or three chunks do, and a share may begin several short items: each takes kPaged8Start units of
+// the line besides its chunks.  Registers are left for as many workgroups as run without spilling: scratch memory costs 3 to
+// 10 us a launch (three workgroups on a compute unit at D128, two registers spilled: 38 us instead of 35).
+//
+// Measured (inputs that change from pass to pass; the slope over the length is 5.95 TB/s): 128 sequences of 512 to 2048 tokens, 16 heads,
+// D64, fp16, int8 64 to 67 us = 4.5 TB/s; 32 of up to 8192, H32/8, D128, bf16, int8 35 us = 3.5 TB/s, 5 of them the second kernel; 2 of 50000 to 65536,
+// H32/4, e4m3, a scale a token 36 us = 3.4 TB/s, 6 of them the second kernel; 24 of up to 5000 with 4 new tokens each 25 us; one of 300
+// tokens 10.8 us.  The launch, the chain of loads before the first product, the last outputs and the second kernel take 12 us of a call in shares.
 #include "cache8_common.h"
 #include "paged_common.h"
 
 namespace sage {
 namespace {
 
-constexpr int kPaged8Shares = 512;  // two workgroups on each compute unit
-constexpr int kPaged8Start = 3;    // chunks that an item's beginning and end cost
+// Two workgroups on each compute unit (32 sequences of 2048 tokens, H32/8, D128: 256 shares 39 us, 512 38, 768 42, 1024 45).
+constexpr int kPaged8Shares = 512;
+// Chunks that an item's beginning and end cost (32 sequences of 200 to 8192 tokens, 24 of 100 to 5000 with 4 new tokens each: 0 44.5 and 38.1 us, 1 38.5
+// and 29.0, 2 36.9 and 27.5, 3 35.9 and 26.5, 4 36.8 and 26.9).
+constexpr int kPaged8Start = 3;
 constexpr float kUnit0 = 0x1p100f;   // unit of the weights before a scale is seen
 constexpr float kUnitTop = 16384.0f;
 

@@ -440,8 +440,8 @@ def read_cache(k_cache, v_cache, block_table, cu_seqlens, total, tensor_layout="
     bytes), ``block_table`` ``[S, width]`` int32.  ``cu_seqlens`` ``[S + 1]`` int32, on the GPU: where each sequence's rows begin, and where the
     last one's end; sequence s is read from its first token on.  ``total``: rows of the results.
 
-    Returns ``(k, v)``, ``[total, Hk, D]`` each, of ``dtype``: fp16, bf16 or fp32 for a cache of codes (default bf16), whose values are rounded
-    once; the caches' own otherwise.  ``out``: a pair of tensors to write instead of new ones.  Rows behind the last sequence are not
+    Returns ``(k, v)``, ``[total, Hk, D]`` each, of ``dtype``: fp16, bf16 or fp32 for a cache of codes (default bf16), which are multiplied
+    by their scale in fp32 and rounded; the caches' own otherwise.  ``out``: a pair of tensors to write instead of new ones.  Rows behind the last sequence are not
     written; tokens whose page the cache does not have, or that the table does not hold, are rows of zeros.
     """
     coded = _coded(k_scale, v_scale)

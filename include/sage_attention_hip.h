@@ -423,7 +423,7 @@ int sage_cache8_append(const sage_append8_params* p, void* workspace, int64_t wo
  * does not hold, are rows of zeros.
  *
  *   k_out, v_out  [total, Hkv, D] through stride_n (row) and stride_h, of out_dtype
- *   scales        of a cache of codes, whose values are rounded once to out_dtype; scales.codes SAGE_CODE_NONE: a cache of
+ *   scales        of a cache of codes, whose products code * scale (fp32) are rounded to out_dtype; scales.codes SAGE_CODE_NONE: a cache of
  *                 entries of out_dtype, which are copied (the rest of scales is not looked at)
  *   Rows of the caches and outputs are 16-byte aligned and a multiple of 16 bytes long.
  */
