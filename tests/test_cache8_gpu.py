@@ -727,3 +727,100 @@ def test_caches_and_lists_without_entries(gpu_device):
     k, v = flag_attn.read_cache(*c, torch.zeros(0, 3, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev), 0, **s)
     assert k.shape == (0, 2, 64)
     assert flag_attn.paged_attention(q[:0], *c, torch.zeros(0, 3, dtype=torch.int32, device=dev), lens[:0], **s).shape == (0, 4, 64)
+
+
+def _prompt_state(codes, g, dev, tokens=700, blocks=2, page=16, hk=2, d=64):
+    """A cache, tokens for it in an order of their own, and what an eager program needs to attend over it."""
+    pages = tokens // page + 3
+    cache = make_cache(pages, hk, page, blocks, d, codes, g)
+    now = [t.to(dev) for t in cache]
+    b = dict(k=torch.zeros(tokens, hk, d, dtype=BF16, device=dev), v=torch.zeros(tokens, hk, d, dtype=BF16, device=dev), slots=torch.full((tokens,), -1, device=dev),
+             q=torch.randn(1, 8, d, generator=g).to(BF16).to(dev), table=torch.zeros(1, 2000, dtype=torch.int32, device=dev), lens=torch.tensor([tokens], dtype=torch.int32, device=dev),
+             cu=torch.tensor([0, tokens], dtype=torch.int32, device=dev))
+    b["table"][0, :pages] = torch.arange(pages, device=dev)
+    return cache, now, b
+
+
+def _prompt_pass(now, b):
+    import flag_attn
+
+    scales = dict(k_scale=now[2], v_scale=now[3])
+    flag_attn.append_to_cache(b["k"], b["v"], now[0], now[1], b["slots"], **scales)
+    o = flag_attn.paged_attention(b["q"], now[0], now[1], b["table"], b["lens"], **scales)
+    return (o, *flag_attn.read_cache(now[0], now[1], b["table"], b["cu"], b["k"].shape[0], **scales))
+
+
+def test_two_captured_prompts_at_once(gpu_device):
+    """Writes through the map, cut attention and reads in two graphs, each with caches of its own, replayed at once on two streams with other
+    tokens and slots each time: no workspace is shared."""
+    g = torch.Generator().manual_seed(46)
+    dev = gpu_device
+    sides = []
+    for codes in (INT8, E4M3):
+        cache, now, b = _prompt_state(codes, g, dev)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            _prompt_pass(now, b)
+        torch.cuda.current_stream().wait_stream(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _prompt_pass(now, b)
+        sides.append([cache, now, b, stream, graph, out])
+    for i in range(4):
+        for side in sides:
+            cache, b = side[0], side[2]
+            slots = torch.randperm(cache[0].shape[0] * 16, generator=g)[:700]
+            slots[::9] = -1
+            k, v = (torch.randn(700, 2, 64, generator=g).to(BF16) * 2.0 ** (i - 1) for _ in range(2))
+            for name, x in (("k", k), ("v", v), ("slots", slots)):
+                b[name].copy_(x)
+            side[0] = CO.append(k, v, cache[0], cache[1], slots, cache[2], cache[3])
+        torch.cuda.synchronize()
+        for side in sides:
+            with torch.cuda.stream(side[3]):
+                for _ in range(3):  # (a write twice is a write once)
+                    side[4].replay()
+        torch.cuda.synchronize()
+        for cache, now, b, _, _, (o, k, v) in sides:
+            assert all(same_numbers(x, y) for x, y in zip(now, cache)), i
+            want, _, tol, _ = CO.paged(b["q"].cpu(), *cache, b["table"].cpu(), [700])
+            CO.assert_close(o.cpu(), want, tol, i)
+            for got, c, s in zip((k, v), cache[:2], cache[2:]):
+                assert same_numbers(got, CO.read(c, s, b["table"].cpu(), torch.tensor([0, 700]), 700, BF16))
+        torch.randn(500, 500, device=dev).sum().item()
+
+
+def test_two_threads_at_once(gpu_device):
+    """Each with a stream and caches of its own; the first calls of a shape and the known ones."""
+    import threading
+
+    dev = gpu_device
+    failed = []
+
+    def work(seed):
+        try:
+            g = torch.Generator().manual_seed(seed)
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                cache, now, b = _prompt_state(INT8, g, dev, tokens=300 + seed)
+                for _ in range(4):
+                    slots = torch.randperm(cache[0].shape[0] * 16, generator=g)[:300 + seed]
+                    k, v = (torch.randn(300 + seed, 2, 64, generator=g).to(BF16) for _ in range(2))
+                    for name, x in (("k", k), ("v", v), ("slots", slots)):
+                        b[name].copy_(x)
+                    cache = CO.append(k, v, cache[0], cache[1], slots, cache[2], cache[3])
+                    o, *_ = _prompt_pass(now, b)
+                    stream.synchronize()
+                    assert all(same_numbers(x, y) for x, y in zip(now, cache))
+                    want, _, tol, _ = CO.paged(b["q"].cpu(), *cache, b["table"].cpu(), [300 + seed])
+                    CO.assert_close(o.cpu(), want, tol)
+        except Exception as e:  # (an assertion of a thread would be lost)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed[0]
