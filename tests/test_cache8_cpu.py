@@ -333,6 +333,76 @@ def test_attention_of_the_oracle():
     assert torch.allclose(half[0], same[0], rtol=1e-12, atol=1e-12)
 
 
+# ---- the line of shares with units before an item's chunks (the arithmetic of paged_common.h, restated)
+
+def _shares_of(chunks, per_seq, shares, start):
+    """Every chunk of every item is in one piece, pieces of cut items have slots of their own, and the joining kernel looks for
+    them where they are; one cut is responsible for each cut item."""
+    units = [start + c for c in chunks]
+    total = sum(units) * per_seq
+    base, rest = divmod(total, shares)
+
+    def begin_of(w):
+        return w * base + min(w, rest)
+
+    def owner(pos):
+        pos = max(min(pos, total - 1), 0)
+        longer = rest * (base + 1)
+        return pos // (base + 1) if pos < longer else rest + (pos - longer) // base
+
+    slots, pieces = {}, {}
+    for w in range(shares):
+        pos, end = begin_of(w), begin_of(w + 1)
+        if pos >= end:
+            continue
+        share_begin, seq, seq_begin = pos, 0, 0
+        while seq_begin + units[seq] * per_seq <= pos:
+            seq_begin += units[seq] * per_seq
+            seq += 1
+        while pos < end:
+            s, u = seq, units[seq]
+            item = (pos - seq_begin) // u
+            begin = seq_begin + item * u
+            to = min(begin + u, end)
+            first = max(pos - begin - start, 0)
+            n = max(to - begin - start, 0) - first
+            pos = to
+            if pos - seq_begin == u * per_seq:
+                seq_begin, seq = pos, seq + 1
+            if n == 0:
+                continue
+            pieces.setdefault((s, item), []).append((first, n))
+            if n != chunks[s]:
+                slot = 2 * w + (begin > share_begin)
+                assert slot not in slots
+                slots[slot] = (s, item)
+    begin, joined = 0, set()
+    for s, u in enumerate(units):
+        for item in range(per_seq):
+            got = pieces[s, item]
+            assert got[0][0] == 0 and sum(n for _, n in got) == chunks[s] and all(a[0] + a[1] == b[0] for a, b in zip(got, got[1:]))
+            first, last = owner(begin + start), owner(begin + u - 1)
+            assert (first == last) == (len(got) == 1)
+            if first != last:
+                for w in range(first, last + 1):
+                    slot = 2 * w + (w == first and begin > begin_of(w))
+                    assert slots[slot] == (s, item)
+                    joined.add(slot)
+                cuts = [w for w in range(shares - 1) if begin_of(w + 1) < begin_of(w + 2) and begin <= begin_of(w + 1) < begin + u and first == w]
+                assert len(cuts) == 1
+            begin += u
+    assert joined == set(slots)
+
+
+def test_shares_with_units_before_chunks():
+    import random
+
+    r = random.Random(0)
+    for _ in range(1500):
+        chunks = [max(1, int(r.choice([0, 1, 2, 5, 20]) * r.random())) for _ in range(r.randint(1, 12))]
+        _shares_of(chunks, r.choice([1, 2, 8]), r.randint(1, 40), r.choice([0, 1, 2, 3, 5]))
+
+
 @pytest.mark.skipif(not os.path.exists("/opt/rocm/bin/hipcc"), reason="needs hipcc")
 def test_kernels_spill_no_vector_registers():
     """A kernel with scratch memory costs several microseconds a launch."""

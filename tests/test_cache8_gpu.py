@@ -116,6 +116,21 @@ def test_cut_launches(gpu_device, codes, h, hk, d, m, lens, page):
     check(q if m > 1 else q[:, 0], cache, wide, lens, gpu_device)
 
 
+@pytest.mark.parametrize("seqs,hk,m,some", [(70, 8, 1, (0, 1, 5, 100, 300, 1500)), (32, 8, 1, (0, 0, 0, 3, 200, 1900)), (40, 4, 3, (0, 0, 129, 2000)), (65, 8, 1, (0,)), (40, 8, 2, (128, 256)),
+                                            (16, 8, 1, (2000,)), (3, 8, 1, (1700, 1))])
+def test_cut_launches_of_many_short_items(gpu_device, seqs, hk, m, some):
+    """Shares that begin several items, empty ones among them, shares that end before an item's first chunk, more items than shares."""
+    g = torch.Generator().manual_seed(12)
+    lens = [some[i] for i in torch.randint(0, len(some), (seqs,), generator=g).tolist()]
+    pages = sum(-(-n // 16) for n in lens) + 2
+    cache = make_cache(pages, hk, 16, 16, 64, E4M3, g)
+    table, _ = make_table(lens, 16, pages, g)
+    wide = torch.zeros(seqs, 250, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table[:, :250]
+    q = torch.randn(seqs, m, hk, 64, generator=g).to(BF16)
+    check(q if m > 1 else q[:, 0], cache, wide, lens, gpu_device)
+
+
 @pytest.mark.parametrize("page", [16, 24])
 @pytest.mark.parametrize("m", [1, 4])
 def test_entries_that_are_no_page(gpu_device, page, m):
