@@ -7,8 +7,10 @@
 //   * Queries in bf16 become fp16 by a power of two of their row's own, 2^(15 - e) with the row's largest entry below 2^e: the entries
 //     above 2^-29 of it keep all their bits, the others are off by at most 2^-40 of it.  Scores stay in that unit, and the
 //     exponent's fma takes them out of it.
-//   * Weights p_j vs_j are rounded to fp16 (off by 2^-11 of themselves at most) in a unit that follows the largest vs of the tiles so far: at most 2^14, so
-//     that weights down to 2^-28 of it keep all 11 bits.
+//   * Weights w_j = p_j vs_j are rounded to fp16 (off by 2^-11 of themselves at most) in a unit of their row's own, a power of two in which the
+//     largest |w| of the keys that the wave has seen lies between kUnitLow and kUnitTop: weights down to 2^-24 of it keep all 11 bits, smaller ones
+//     are off by at most 2^-35 of it.  (The largest |vs| says nothing about it: it may belong to a key of no weight.)  A row's unit changes with
+//     its accumulators, as its reference m does.
 //
 // Bound by the bytes of the codes: half of a 16-bit cache's.  The layout of the work is paged_attn.hip's.  K rows go to the operand
 // registers 16 codes a lane, so that a load holds two steps of channels, and Q's channels lie in the same order; V tiles go through
@@ -34,8 +36,9 @@ constexpr int kPaged8Shares = 512;
 // Chunks that an item's beginning and end cost (32 sequences of 200 to 8192 tokens, 24 of 100 to 5000 with 4 new tokens each: 0 44.5 and 38.1 us, 1 38.5
 // and 29.0, 2 36.9 and 27.5, 3 35.9 and 26.5, 4 36.8 and 26.9).
 constexpr int kPaged8Start = 3;
-constexpr float kUnit0 = 0x1p100f;   // unit of the weights before a scale is seen
-constexpr float kUnitTop = 16384.0f;
+constexpr float kUnitLow = 1024.0f, kUnitTop = 32768.0f;  // (fp16 ends at 65504)
+constexpr int kUnitBits = 14;      // a new unit makes the largest weight so far less than 2^14, and at least half of that
+constexpr int kUnitLeast = -112;   // weights below 2^-112 get the unit of that: 2^126
 
 // V tiles in LDS: 16-byte chunk c of row r lies at chunk c ^ paged8_v_swizzle(r), so that the sixteen rows that half a wave's
 // transposed read touches, 16 bytes each, lie on different banks.
@@ -204,7 +207,9 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
             return seen;
         };
 
-        float m_i = -INFINITY, l_i = 0.0f, w_unit = kUnit0;  // w_unit: weights are multiplied by it (the same in every lane)
+        float m_i = -INFINITY, l_i = 0.0f;
+        // Weights are multiplied by w_unit (the same in a row's four lanes); w_top: the largest that this lane has seen, relative to m_i, in that unit.
+        float w_unit = 1.0f, w_top = 0.0f;
         v4f o[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) o[ct] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -219,26 +224,26 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
         __builtin_amdgcn_sched_barrier(0);
         // (after the first tile has been requested)
         float unit = 1.0f;  // of the row's scores: 2^(e - 15)
-                    if constexpr (std::is_same<QT, __bf16>::value) {
-                        float top = 0.0f;  // of the finite ones
-        #pragma unroll
-                        for (int t = 0; t < 2 * KLOADS; t++)
-        #pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                const float x = __builtin_fabsf((float)__builtin_bit_cast(bf16x8, qf[t])[i]);
-                                top = fmaxf(top, x < INFINITY ? x : 0.0f);
-                            }
-                        top = fmaxf(top, __shfl_xor(top, 16));
-                        top = fmaxf(top, __shfl_xor(top, 32));
-                        const int e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 15;
-                        unit = __builtin_amdgcn_ldexpf(1.0f, e - 15);
-        #pragma unroll
-                        for (int t = 0; t < 2 * KLOADS; t++) {
-                            const bf16x8 x = __builtin_bit_cast(bf16x8, qf[t]);
-        #pragma unroll
-                            for (int i = 0; i < 8; i++) qf[t][i] = (_Float16)__builtin_amdgcn_ldexpf((float)x[i], 15 - e);
-                        }
-                    }
+        if constexpr (std::is_same<QT, __bf16>::value) {
+            float top = 0.0f;  // of the finite ones
+#pragma unroll
+            for (int t = 0; t < 2 * KLOADS; t++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float x = __builtin_fabsf((float)__builtin_bit_cast(bf16x8, qf[t])[i]);
+                    top = fmaxf(top, x < INFINITY ? x : 0.0f);
+                }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const int e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 15;
+            unit = __builtin_amdgcn_ldexpf(1.0f, e - 15);
+#pragma unroll
+            for (int t = 0; t < 2 * KLOADS; t++) {
+                const bf16x8 x = __builtin_bit_cast(bf16x8, qf[t]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) qf[t][i] = (_Float16)__builtin_amdgcn_ldexpf((float)x[i], 15 - e);
+            }
+        }
         for (; key0 < kend; key0 += kstep) {
             // ---- S^T = K.Q^T: register i of score tile u is key key0 + 16 u + 4 quad + i of the lane's row
             v4f s[2];
@@ -259,18 +264,7 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
                 if (seen != ~0u && !((seen >> row) & 1)) vr[e] = v4i{0, 0, 0, 0};
                 *reinterpret_cast<v4i*>(vlds + row * D + 16 * (vchunk ^ paged8_v_swizzle<D>(row))) = vr[e];
             }
-            const float v_scale = lane >= 32 && ((seen >> (lane & 31)) & 1) ? sc : 0.0f;
-            float shrink = 1.0f;  // of the weights' unit
-            const float v_size = __builtin_fabsf(v_scale);
-            if (__builtin_amdgcn_ballot_w64(v_size * w_unit > kUnitTop && v_size < INFINITY) != 0) {
-                float top = v_size < INFINITY ? v_size : 0.0f;
-#pragma unroll
-                for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-                const float unit_now = __builtin_amdgcn_ldexpf(kUnitTop, -__builtin_amdgcn_frexp_expf(top));
-                shrink = unit_now / w_unit;
-                w_unit = unit_now;
-            }
-            slds[lane] = lane < 32 ? sc * a.qk_scale : v_scale * w_unit;
+            slds[lane] = lane < 32 ? sc * a.qk_scale : (seen >> (lane & 31)) & 1 ? sc : 0.0f;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_sched_barrier(0);
             // ---- the registers of K and V are requested anew
@@ -299,18 +293,19 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float m_new = fmaxf(m_i, mx);
             const float m_use = m_new == -INFINITY ? 0.0f : m_new;  // (no key seen yet: every P below is exp2(-inf) = 0)
-            if (__builtin_amdgcn_ballot_w64(m_new > m_i || shrink != 1.0f) != 0) {
+            const bool grown = __builtin_amdgcn_ballot_w64(m_new > m_i) != 0;
+            if (grown) {
                 const float alpha = __builtin_amdgcn_exp2f((m_i - m_use) * unit);  // 0 for a row without a reference point
                 l_i *= alpha;
+                w_top *= alpha;
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) o[ct][i] *= alpha * shrink;
+                    for (int i = 0; i < 4; i++) o[ct][i] *= alpha;
                 m_i = m_new;
             }
-            // Weights, rounded to fp16 for the matrix instructions; the sum of P is taken before that
-            f16x8 pf;
-            float psum = 0.0f;
+            // Weights; the sum of P is taken before they are rounded
+            float psum = 0.0f, top = 0.0f;
             const float m_ref = -m_use * unit;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
@@ -320,10 +315,39 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
                     const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], unit, m_ref));
                     psum += p;
                     float w = p * vs[i];
-                    if (SEVERAL && some_see && s[u][i] == -INFINITY) w = 0.0f;  // (a scale that is not finite, under a hidden key)
-                    pf[4 * u + i] = (_Float16)w;
+                    if (SEVERAL && some_see && key0 + 16 * u + 4 * quad + i > my_last) w = 0.0f;  // (a scale that is not finite, under a hidden key)
+                    s[u][i] = w;
+                    top = fmaxf(top, __builtin_fabsf(w));
                 }
             }
+            // Does the unit hold them?  Weights that are too large for it are seen by one lane; that all of a row's are small, by none of its four.
+            const float before = w_top;
+            w_top = fmaxf(w_top, top * w_unit);
+            bool fits = __builtin_amdgcn_ballot_w64(w_top > kUnitTop) == 0;
+            if (grown) {
+                unsigned long long enough = __builtin_amdgcn_ballot_w64(w_top >= kUnitLow);
+                enough |= enough >> 32;
+                fits &= ((enough | enough >> 16) & 0xffff) == 0xffff;
+            }
+            if (!fits) {
+                // (weights that are not finite spoil their row in any unit; they have the exponent 0 here)
+                const int was = __builtin_amdgcn_frexp_expf(w_unit) - 1;
+                int e = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : kUnitLeast, before > 0.0f ? __builtin_amdgcn_frexp_expf(before) - was : kUnitLeast);
+                e = max(e, __shfl_xor(e, 16));
+                e = max(max(e, __shfl_xor(e, 32)), kUnitLeast);
+                const int change = kUnitBits - e - was;
+                w_unit = __builtin_amdgcn_ldexpf(1.0f, kUnitBits - e);
+                w_top = fminf(fmaxf(__builtin_amdgcn_ldexpf(before, change), top * w_unit), kUnitTop);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[ct][i] = __builtin_amdgcn_ldexpf(o[ct][i], change);
+            }
+            f16x8 pf;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) pf[4 * u + i] = (_Float16)(s[u][i] * w_unit);
             l_i += psum;
             // ---- O^T += V^T.P^T
             auto v_fragment = [&](int ct) {  // channels 16 ct ..
@@ -382,7 +406,8 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
         const float m_use = m == -INFINITY ? 0.0f : m;
         for (int w = row_wave; w < kPagedWaves; w += row_waves) l += row_l[w][l16] * __builtin_amdgcn_exp2f((row_m[w][l16] - m_use) * unit);
         // l = 0: a row that saw no key; its output is 0, its log-sum-exp -inf.  (NaN stays.)
-        const float f = l != 0.0f ? __builtin_amdgcn_exp2f((m_i - m_use) * unit) / l / w_unit : 0.0f;
+        const float f = l != 0.0f ? __builtin_amdgcn_exp2f((m_i - m_use) * unit) / l : 0.0f;
+        const float w_step = 1.0f / w_unit;
         if (wave == row_wave && quad == 0 && wrow0 + l16 < rows) {
             const float lse2 = __builtin_log2f(l) + m_use * unit;
             if (!whole) a.part_lse[(int64_t)slot * a.tile_rows + 16 * row_wave + l16] = lse2;
@@ -391,7 +416,7 @@ __global__ __launch_bounds__(kPagedThreads, D == 128 ? 2 : SEVERAL || !PAGE16 ? 
         float* slice = reinterpret_cast<float*>(smem);  // (the V tiles have been read, since the barrier above)
 #pragma unroll
         for (int ct = 0; ct < CT; ct++)
-            *reinterpret_cast<v4f*>(slice + (wave * 16 + l16) * SL_RS + 16 * ct + 4 * quad) = v4f{o[ct][0] * f, o[ct][1] * f, o[ct][2] * f, o[ct][3] * f};
+            *reinterpret_cast<v4f*>(slice + (wave * 16 + l16) * SL_RS + 16 * ct + 4 * quad) = v4f{o[ct][0] * f * w_step, o[ct][1] * f * w_step, o[ct][2] * f * w_step, o[ct][3] * f * w_step};
         __syncthreads();
         const int tile_end = min(16 * row_waves, rows - row0);  // rows that exist
         for (int piece = tid; piece < tile_end * (D / 4); piece += kPagedThreads) {

@@ -113,6 +113,9 @@ def paged(q, k_cache, v_cache, k_scale, v_scale, table, lens, sm_scale=None, lay
     q4 = q if q.dim() == 4 else q[:, None]
     kv, vv = values(k_cache, k_scale, layout), values(v_cache, v_scale, layout)
     pages, page, hk, d = kv.shape
+    v_size = numbers(v_cache).abs()
+    v_size = v_size.transpose(1, 2) if layout == "HND" else v_size  # [pages, page, Hk, D], of the codes
+    s_size = v_scale.double().abs().repeat_interleave(page // v_scale.shape[-1], dim=-1).transpose(1, 2)  # [pages, page, Hk]
     S, M, H, _ = q4.shape
     half_step = torch.finfo(q.dtype).eps / 2
     least = 2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -134  # half a step of the output below its normal range
@@ -125,9 +128,10 @@ def paged(q, k_cache, v_cache, k_scale, v_scale, table, lens, sm_scale=None, lay
         rows = table[s, :-(-n // page)].long()
         bad = (rows < 0) | (rows >= pages)
         hidden = bad.repeat_interleave(page)[:n]
-        k, v = (c[rows.masked_fill(bad, 0)].reshape(-1, hk, d)[:n] for c in (kv, vv))
+        k, v, vc = (c[rows.masked_fill(bad, 0)].reshape(-1, hk, d)[:n] for c in (kv, vv, v_size))
+        vs = s_size[rows.masked_fill(bad, 0)].reshape(-1, hk)[:n]
         for h in range(H):
-            ki, vi = k[:, h * hk // H], v[:, h * hk // H]
+            ki, vi, ci, si = (x[:, h * hk // H] for x in (k, v, vc, vs))
             for m in range(M):
                 sees = (torch.arange(n) <= n - M + m) & ~hidden
                 if not sees.any():
@@ -146,14 +150,16 @@ def paged(q, k_cache, v_cache, k_scale, v_scale, table, lens, sm_scale=None, lay
                     score += 2.0 ** -40 * float(qi.abs().max()) * float(kk.abs().sum(1).max()) * abs(sm_scale)
                 cnt = int(sees.sum())
                 norm_tol[s, h, m] = score + cnt * 2.0 ** -24 + 2.0 ** -22 * abs(float(norm[s, h, m]))
-                # A weight p vs is rounded to fp16, whose numbers in [1, 2) lie 2^-10 apart: off by half of that, 2^-11 of itself
+                # A weight w = p vs is rounded to fp16, whose numbers in [1, 2) lie 2^-10 apart: off by half of that, 2^-11 of itself
                 # (a bound of 2^-12, as if the step were 2^-11, is below what the rounding itself does); those below 2^-14 lie 2^-24 apart,
-                # and the largest vs is at least 2^13 there: off by 2^-25 / 2^13 = 2^-38 of it.  That reaches the output through
-                # codes of up to 127 or 448; the output is rounded once more.
+                # and the row's largest weight so far is at least 2^10 in their unit: off by 2^-25 / 2^10 = 2^-35 of it, and by no
+                # more than themselves (the nearest number is no further than zero).  In fp32 before that: p below 2^-126 may be zero, products below
+                # it lie 2^-149 apart.  Each reaches the output through its own code; the output is rounded once more.
                 spread = (p @ vw.abs()) * inv
+                w = p * si[sees]
+                small = torch.minimum(w, 2.0 ** -35 * w.max()) + p.clamp(max=2.0 ** -126) * si[sees] + 2.0 ** -150
                 o_tol[s, m, h] = half_step * (o[s, m, h].abs() + 2.0 ** -11 * spread) + 2.0 ** -11 * spread \
-                    + (2 * score + 2 * cnt * 2.0 ** -24 + 2.0 ** -22) * spread \
-                    + cnt * 2.0 ** -38 * LARGEST[v_cache.dtype] * float(v_scale.double().nan_to_num(0, 0, 0).max()) * inv + least
+                    + (2 * score + 2 * cnt * 2.0 ** -24 + 2.0 ** -22) * spread + (small @ ci[sees]) * inv + least
     if q.dim() == 3:
         o, o_tol, norm, norm_tol = o[:, 0], o_tol[:, 0], norm[:, :, 0], norm_tol[:, :, 0]
     return o, norm, o_tol, norm_tol
