@@ -5,7 +5,7 @@
 // 8 layers copied 76 us = 5.0 TB/s, 12 pages 4.3.
 //
 // Quantizing.  A block's scale is s = a / L, a the largest |x| of the call's tokens for it and head (at least 2^-100), L = 127 or 448, or
-// what it was where that is more and the block goes on; codes are x / s to the nearest, ties to even.  x / s is x times the rounded
+// the size of what it was where that is more and the block goes on; codes are x / s to the nearest, ties to even.  x / s is x times the rounded
 // 1 / s first, off by at most 2^-22 of itself; only where that lies next to the middle between two codes (a wave in sixteen) the
 // remainder x - c s, which is exact in an fma, decides.  Codes that stay when a scale grows are c s_old / s, decided by a remainder in 64 bits.
 #include "cache8_common.h"
@@ -130,14 +130,14 @@ template <> struct Rounding<Int8> {
         }
         return w;
     }
-    // A word of codes that stand for numbers in units of `was`, in units of s >= was.
+    // A word of codes that stand for numbers in units of `was`, in units of s >= |was|.  (-128, which no write makes, may change its sign: 127)
     static __device__ __forceinline__ unsigned again(unsigned w, double was, double s) {
         const double ratio = was / s;
         unsigned to = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const double c = (double)(int8_t)(w >> (8 * i));
-            const double n = settle(c * was, s, __builtin_rint(c * ratio));
+            const double n = __builtin_fmin(settle(c * was, s, __builtin_rint(c * ratio)), 127.0);
             to |= ((unsigned)(int)n & 255u) << (8 * i);
         }
         return to;
@@ -284,13 +284,14 @@ __device__ __forceinline__ int mapped(const WriteArgs& a, int64_t slot) {
     return who >= 0 && who < a.tokens && index_at(a.slots, a.wide, who) == slot ? who : -1;
 }
 
-// The scale of a block that had `was` and gets rows whose largest entry has the size `top`.
+// The scale of a block that had `was`, of either sign, and gets rows whose largest entry has the size `top`.  One that is not finite stays.
 template <typename Code>
 __device__ __forceinline__ float next_scale(float was, float top) {
-    const float asked = scale_for<Code>(top);
-    return was >= asked || was != was ? was : asked;
+    const float asked = scale_for<Code>(top), size = __builtin_fabsf(was);
+    if (was != was) return was;
+    return !(size >= asked) ? asked : size < INFINITY ? size : was;
 }
-// Sixteen codes that stay when a scale grows.
+// Sixteen codes that stay when a scale changes.
 template <typename Code>
 __device__ __forceinline__ void convert(unsigned char* at, float was, float s) {
     v4i w = *reinterpret_cast<v4i*>(at);
@@ -389,11 +390,11 @@ __global__ __launch_bounds__(kOpThreads, 4) void cache8_write_blocks_kernel(Writ
             for (int e = 0; e < kKeep; e++) top = rows[e].top(top);
             for (int d = 1; d < span; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
             const float s = next_scale<Code>(was, Row16<T>::size(top));
-            const float inv = s < INFINITY ? 1.0f / s : 0.0f;
+            const float inv = __builtin_fabsf(s) < INFINITY ? 1.0f / s : 0.0f;
 #pragma unroll
             for (int e = 0; e < kKeep; e++) {
                 if (e * ROWS >= block) break;
-                if (!(s < INFINITY)) rows[e].clear();  // (NaN: an entry was not finite)
+                if (!(__builtin_fabsf(s) < INFINITY)) rows[e].clear();  // (NaN: an entry was not finite)
                 const v4i w = Rounding<Code>::codes(rows[e], s, inv);
                 if (who[e] >= 0 || (who[e] == -1 && begun))  // (zeros where a block begins)
                     *reinterpret_cast<v4i*>(dst + e * ROWS * a.ds_n[x]) = w;
@@ -471,13 +472,13 @@ __global__ __launch_bounds__(kOpThreads, sizeof(T) == 4 ? 3 : 4) void cache8_wri
 #pragma unroll
             for (int w = 0; w < WAVES; w++) top = max(top, tops[turn][w]);
             const float s = next_scale<Code>(was, Row16<T>::size(top));
-            const float inv = s < INFINITY ? 1.0f / s : 0.0f;
+            const float inv = __builtin_fabsf(s) < INFINITY ? 1.0f / s : 0.0f;
             for (int p0 = 0; p0 < block; p0 += PASS) {
                 if (block > PASS) load(p0);
 #pragma unroll
                 for (int e = 0; e < KEEP; e++) {
                     if (p0 + e * (WAVES * ROWS) >= block) break;
-                    if (!(s < INFINITY)) rows[e].clear();  // (NaN: an entry was not finite)
+                    if (!(__builtin_fabsf(s) < INFINITY)) rows[e].clear();  // (NaN: an entry was not finite)
                     const v4i w = Rounding<Code>::codes(rows[e], s, inv);
                     if (who[e] >= 0 || (who[e] == -1 && begun))  // (zeros where a block begins)
                         *reinterpret_cast<v4i*>(dst + (p0 + e * (WAVES * ROWS) + my_row) * a.ds_n[x]) = w;

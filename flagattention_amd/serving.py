@@ -371,8 +371,8 @@ def append_to_cache(k, v, k_cache, v_cache, slots, tensor_layout="HND", *, k_sca
     With ``k_scale``, ``v_scale`` ``[pages, Hk, blocks]`` fp32 (any strides) the caches are int8 or float8_e4m3fn, D a multiple of 16 up to
     512, and the rows are quantized as they are written: ``page_size / blocks`` (at most 1024) consecutive places of a page
     and a head share a scale, one place each being the most exact.  A block's scale is the largest absolute value of the call's tokens for it (at
-    least 2^-100), divided by 127 (e4m3: by 448), or what it was where that is more; codes are entry / scale, to the nearest, ties to even.
-    Where a scale grows, the codes that the block holds are converted to it (rounded again); a token for a block's first place begins it anew:
+    least 2^-100), divided by 127 (e4m3: by 448), or the size of what it was where that is more; codes are entry / scale, to the nearest, ties to even.
+    Where a scale grows, or was negative, the codes that the block holds are converted to it (rounded again); a token for a block's first place begins it anew:
     what it held is forgotten, and places that the call does not write become zeros.  So blocks are filled from their first place on,
     and a page that is used again needs no clearing.  (A block that is entered further in has to have a scale: zero, or as copied.)  An infinity or NaN
     makes the block's scale NaN, until the block begins anew.

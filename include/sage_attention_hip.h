@@ -401,10 +401,10 @@ int sage_paged8_attn(const sage_paged8_params* p, void* workspace, int64_t works
 /*
  * sage_cache_append into a cache of codes.  append.dtype is that of k and v (SAGE_F16 / SAGE_BF16 / SAGE_F32), head_dim a multiple of
  * 16 up to 512, blocks of at most 1024 tokens.  Of the tokens of a call that go to one block, and one head, let a be the largest
- * absolute value, at least 2^-100.  The block's scale becomes a / 127 (e4m3: a / 448), or stays as it was where that is more; where
+ * absolute value, at least 2^-100.  The block's scale becomes a / 127 (e4m3: a / 448), or the size of what it was where that is more; where
  * one of the tokens goes to the block's first place, the block begins anew, and what it held before is forgotten: the places that are not written get
- * zero codes.  Codes are x / scale rounded to the nearest, ties to even; where a scale has grown, the codes that stay are
- * code * old scale / new scale, rounded likewise.  An infinity or NaN makes the block's scale NaN until it begins anew.
+ * zero codes.  Codes are x / scale rounded to the nearest, ties to even; where a scale has grown or was negative, the codes that stay are
+ * code * old scale / new scale, rounded likewise.  An infinity or NaN makes the block's scale NaN until it begins anew; a held scale that is infinite stays.
  *
  * workspace: sage_cache8_append_workspace_bytes(p) bytes, contents irrelevant before and after; rules of sage_attn_fwd_ws, but that
  * a call that needs one is refused without (SAGE_E_INVALID).

@@ -37,7 +37,7 @@ def e4m3_numbers():
 def nearest(x, dtype):
     """The nearest codes to numbers in 64 bits, ties to the even one, as numbers."""
     if dtype == torch.int8:
-        return torch.round(x)  # (half to even)
+        return torch.round(x).clamp(max=127)  # (half to even)
     grid = e4m3_numbers()
     size = x.abs().clamp(max=448.0)
     hi = torch.searchsorted(grid, size.contiguous()).clamp(min=1, max=126)
@@ -71,13 +71,14 @@ def append(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout="HND"):
                     asked = float((row.abs().max().clamp(min=SMALLEST) / LARGEST[codes.dtype]).float())
                 else:
                     asked = math.nan
-                now = math.nan if math.isnan(old) or math.isnan(asked) else max(old, asked)
+                # (sizes: a block that the program gave a negative scale keeps its values; one of an infinite scale keeps that)
+                now = math.nan if math.isnan(old) or math.isnan(asked) else old if math.isinf(old) else max(abs(old), asked)
                 scales[p, h, at] = now
                 held = by_place[p, at * size:(at + 1) * size, h]
                 new = numbers(held)
                 if 0 in places:
                     new = torch.zeros_like(new)
-                elif now > old:
+                elif now != old and now == now:
                     new = nearest(new * old / now, codes.dtype)  # (code * old has 31 bits; the quotient next to a middle but not on it differs by 2^-32 of itself)
                 for i, q in enumerate(places):
                     new[q] = 0.0 if math.isnan(now) else nearest(row[i] / now, codes.dtype)
