@@ -283,7 +283,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, sm_scale=None, t
     ``k_scale``, ``v_scale`` ``[pages, Hk, blocks]`` fp32 (any strides): the scales of a cache of codes, whose caches are int8 or
     float8_e4m3fn (see ``append_to_cache``).  Codes are multiplied as they are; scores take K's scales in fp32, and the softmax's weights
     V's, before they are rounded to fp16 (in a unit of each row's own that keeps 11 bits of those down to 2^-24 of the row's largest; smaller ones are
-    off by at most 2^-35 of it).  A scale that is not finite reaches the rows that see a token of its block.
+    off by at most 2^-35 of it).  V scales that are not finite, and K scales that are NaN, spoil the rows that see a token of their block; infinite K
+    scales make its scores infinite: plus infinity spoils the row, minus infinity leaves the key out.
     """
     coded = _coded(k_scale, v_scale)
     call = (q, k_cache, v_cache, block_table, seq_lens, sm_scale, tensor_layout, return_log_normalizer)

@@ -388,7 +388,8 @@ typedef struct sage_cache_scales {
 
 /*
  * sage_paged_attn over a cache of codes.  paged.dtype is that of q and out (SAGE_F16 / SAGE_BF16); the strides of the caches count
- * bytes, below 2^32 between pages, and their rows are 16-byte aligned.  Blocks whose scale is not finite reach the rows that see one of their tokens.
+ * bytes, below 2^32 between pages, and their rows are 16-byte aligned.  V scales that are not finite, and
+ * K scales that are NaN, spoil the rows that see a token of their block; infinite K scales make infinite scores: plus infinity spoils the row, minus infinity leaves the key out.
  */
 typedef struct sage_paged8_params {
     sage_paged_params paged;

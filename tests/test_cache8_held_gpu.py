@@ -69,3 +69,44 @@ def test_a_negative_scale_is_no_reason_to_wrap(gpu_device):
         assert kc.float()[0, 0, 0, :4].tolist() == [-top, top, -1.0, 127.0 if kinds == INT8 else 128.0]
         assert vc.float()[0, 0, 0, :4].tolist() == [top, -top, 1.0, -128.0]
         assert (kc.float()[0, 0, 3] == vc.float()[0, 0, 3]).all() and not kc.float()[0, 0, 1].any()
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("page", [16, 8])
+@pytest.mark.parametrize("m", [1, 4])
+def test_infinite_scales_of_keys(gpu_device, codes, page, m):
+    """A score of minus infinity leaves the key out, one of plus infinity makes the row NaN; rows that do not see the key are as before.  A row
+    whose keys are all left out is a row of zeros."""
+    import flag_attn
+
+    g = torch.Generator().manual_seed(61)
+    dev, n, hk, h, d = gpu_device, 100, 2, 8, 64
+    pages = -(-n // page)
+    kc, vc = (random_codes((pages, hk, page, d), CODES[codes], g) for _ in range(2))
+    ks, vs = (torch.rand(pages, hk, page, generator=g) / 30 + 0.01 for _ in range(2))
+    kc.view(torch.int8)[:, :, :, 0] = 64                               # (channel 0 of every key: 64, or 2 in e4m3)
+    table, lens = torch.arange(pages, dtype=torch.int32)[None].to(dev), torch.tensor([n], dtype=torch.int32, device=dev)
+
+    def attend(q, ks):
+        q, ks = q.to(dev), ks.to(dev)
+        q = q if m > 1 else q[:, 0]
+        o, norm = flag_attn.paged_attention(q, kc.to(dev), vc.to(dev), table, lens, return_log_normalizer=True, k_scale=ks, v_scale=vs.to(dev))
+        return (o.cpu(), norm.transpose(1, 2).cpu()) if m > 1 else (o.cpu()[:, None], norm.cpu()[:, None])
+
+    q = torch.randn(1, m, h, d, generator=g).to(BF16)
+    q[:, :, ::2, 1:] = 0                                               # these rows score by channel 0 alone, and positively before the scale
+    q[:, :, ::2, 0] = 1.5
+    at = n - 3                                                         # new token i of four sees keys up to 96 + i: the last three see it
+    sees = torch.zeros(1, m, h // 2, dtype=torch.bool)
+    sees[:, -3:] = True
+    for kv in range(hk):
+        far, low, high = ks.clone(), ks.clone(), ks.clone()
+        far[at // page, kv, at % page], low[at // page, kv, at % page], high[at // page, kv, at % page] = -2.0 ** 40, -math.inf, math.inf
+        mine = sees & ((torch.arange(0, h, 2) // (h // hk)) == kv)
+        clean, clean_norm = attend(q, ks)
+        (a, an), (b, bn), (c, cn) = (attend(q, x) for x in (far, low, high))
+        assert torch.equal(a[:, :, ::2], b[:, :, ::2]) and torch.equal(an[:, :, ::2], bn[:, :, ::2])
+        assert torch.isnan(c[:, :, ::2][mine]).all() and torch.isnan(cn[:, :, ::2][mine]).all()
+        assert torch.equal(c[:, :, ::2][~mine], clean[:, :, ::2][~mine]) and torch.equal(cn[:, :, ::2][~mine], clean_norm[:, :, ::2][~mine])
+    o, norm = attend(q, torch.full_like(ks, -math.inf))
+    assert not o[:, :, ::2].any() and (norm[:, :, ::2] == -math.inf).all()
