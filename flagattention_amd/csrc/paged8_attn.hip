@@ -5,7 +5,7 @@
 // Codes are exact in fp16, so both products run on the 16-bit matrix instructions without another rounding of K or V; a score is
 // multiplied by its key's scale in fp32, and a weight by its value's before the weights are rounded.
 //   * Queries in bf16 become fp16 by a power of two of their row's own, 2^(15 - e) with the row's largest entry below 2^e: the entries
-//     above 2^-29 of it keep all their bits, the others are off by at most 2^-40 of it.  Scores stay in that unit, and the
+//     above 2^-29 of it keep all their bits, the others are off by at most 2^-39 of it (half of fp16's least step, 2^-25, against 2^14).  Scores stay in that unit, and the
 //     exponent's fma takes them out of it.
 //   * Weights w_j = p_j vs_j are rounded to fp16 (off by 2^-11 of themselves at most) in a unit of their row's own, a power of two in which the
 //     largest |w| of the keys that the wave has seen lies between kUnitLow and kUnitTop: weights down to 2^-24 of it keep all 11 bits, smaller ones

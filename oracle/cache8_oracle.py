@@ -144,11 +144,12 @@ def paged(q, k_cache, v_cache, k_scale, v_scale, table, lens, sm_scale=None, lay
                 inv = 1 / p.sum()
                 o[s, m, h] = (p @ vw) * inv
                 # A score: D products summed in fp32, three factors, the exponent's argument and the exponential, each a few 2^-24 of
-                # the sum of the terms' sizes or of 1; queries in bf16 enter as fp16, off by up to 2^-40 of the row's largest.
+                # the sum of the terms' sizes or of 1; queries in bf16 enter as fp16, off by up to 2^-39 of the row's largest
+                # (which is at least 2^14 there, and half of the least step is 2^-25).
                 size = float(((kk.abs() @ qi.abs()) * abs(sm_scale)).max())
                 score = (d + 16) * 2.0 ** -24 * size + 2.0 ** -21
                 if q.dtype == torch.bfloat16:
-                    score += 2.0 ** -40 * float(qi.abs().max()) * float(kk.abs().sum(1).max()) * abs(sm_scale)
+                    score += 2.0 ** -39 * float(qi.abs().max()) * float(kk.abs().sum(1).max()) * abs(sm_scale)
                 cnt = int(sees.sum())
                 norm_tol[s, h, m] = score + cnt * 2.0 ** -24 + 2.0 ** -22 * abs(float(norm[s, h, m]))
                 # A weight w = p vs is rounded to fp16, whose numbers in [1, 2) lie 2^-10 apart: off by half of that, 2^-11 of itself

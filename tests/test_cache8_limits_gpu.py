@@ -121,3 +121,19 @@ def test_far_scales_in_cut_launches(gpu_device):
     wide = torch.zeros(1, 1300, dtype=torch.int32)
     wide[0, :pages] = torch.arange(pages)
     check((3 + 0.1 * torch.randn(1, 8, d, generator=g)).to(BF16), (kc, vc, ks, vs), wide, [n], gpu_device)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_entries_of_a_query_far_below_its_largest(gpu_device, codes):
+    """Queries in bf16 enter in steps of 2^-38 of a largest entry of 1: one of 1.5 steps beside it is off by half a step, 2^-39."""
+    g = torch.Generator().manual_seed(54)
+    kc, vc, ks, vs = make_cache(2, 1, 16, 1, 64, CODES[codes], g)
+    kc.view(torch.int8).zero_()
+    kc[:, :, :, 1] = torch.arange(32).view(2, 1, 16).to(kc.dtype)
+    ks.fill_(2.0 ** 37)
+    q = torch.zeros(1, 2, 64)
+    q[:, :, 0], q[0, 0, 1], q[0, 1, 1] = 1.0, 1.5 * 2.0 ** -38, 3 * 2.0 ** -38
+    _, norm = attend(q.to(BF16), (kc, vc, ks, vs), torch.arange(2, dtype=torch.int32)[None], [32], gpu_device)
+    _, want, _, tol = CO.paged(q.to(BF16), kc, vc, ks, vs, torch.arange(2, dtype=torch.int32)[None], [32])
+    CO.assert_close(norm, want, tol)
+    assert (norm - want).abs()[0, 0] > 0.6 * tol[0, 0] and (norm - want).abs()[0, 1] < 1e-5
