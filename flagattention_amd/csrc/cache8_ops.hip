@@ -18,7 +18,8 @@ using namespace attn;
 constexpr int kOpThreads = 256;
 constexpr int kMostBlock = 1024;     // tokens that share a scale
 // Calls of up to so many tokens look their slots over instead of mapping them, which is a launch of its own (500 tokens, blocks of 8, 16 heads, D64:
-// 10.4 us by looking, 7.8 through the map).
+// 10.4 us by looking, 7.8 through the map).  Tokens that go to blocks of their own cost more beyond (8 heads, D128, blocks of 16: 256 7.3 us, 257 48.7), since a
+// workgroup then looks at as many as fill its waves' blocks.
 constexpr int kScanTokens = 256;
 // Workgroups that a write of blocks makes where it can (16384 tokens of 8 heads, D128, bf16, blocks of 16 and 32: 512 32 and 34 us, 1024 26.4 and 34,
 // 2048 28.7 and 36, 4096 30.6 and 42: a wave that goes through more heads looks its tokens up less often).

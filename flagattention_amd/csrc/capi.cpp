@@ -393,7 +393,6 @@ extern "C" int sage_cache_append(const sage_append_params* p, void* stream) {
     return nothing ? SAGE_OK : launch_cache_append(*p, (hipStream_t)stream);
 }
 
-
 static int check_copy(const char* who, const sage_copy_params* p, bool& nothing) {
     nothing = false;
     if (!p) return fail(SAGE_E_INVALID, "%s: null params", who);

@@ -22,9 +22,9 @@
 // 10 us a launch (three workgroups on a compute unit at D128, two registers spilled: 38 us instead of 35).
 //
 // Measured (inputs that change from pass to pass; the slope over the length is 5.95 TB/s): 128 sequences of 512 to 2048 tokens, 16 heads,
-// D64, fp16, int8 64 to 67 us = 4.5 TB/s; 32 of up to 8192, H32/8, D128, bf16, int8 35 us = 3.5 TB/s, 5 of them the second kernel; 2 of 50000 to 65536,
-// H32/4, e4m3, a scale a token 36 us = 3.4 TB/s, 6 of them the second kernel; 24 of up to 5000 with 4 new tokens each 25 us; one of 300
-// tokens 10.8 us.  The launch, the chain of loads before the first product, the last outputs and the second kernel take 12 us of a call in shares.
+// D64, fp16, int8 66 us = 4.4 TB/s; 32 of up to 8192, H32/8, D128, bf16, int8 34 us = 3.6 TB/s, 5 of them the second kernel; 2 of 50000 to 65536,
+// H32/4, e4m3, a scale a token 36 us = 3.4 TB/s, 6 of them the second kernel; 24 of up to 5000 with 4 new tokens each 25.6 us; one of 300
+// tokens 10.3 us.  The launch, the chain of loads before the first product, the last outputs and the second kernel take 12 us of a call in shares.
 #include "cache8_common.h"
 #include "paged_common.h"
 
@@ -36,7 +36,9 @@ constexpr int kPaged8Shares = 512;
 // Chunks that an item's beginning and end cost (32 sequences of 200 to 8192 tokens, 24 of 100 to 5000 with 4 new tokens each: 0 44.5 and 38.1 us, 1 38.5
 // and 29.0, 2 36.9 and 27.5, 3 35.9 and 26.5, 4 36.8 and 26.9).
 constexpr int kPaged8Start = 3;
-constexpr float kUnitLow = 1024.0f, kUnitTop = 32768.0f;  // (fp16 ends at 65504)
+// A row's largest weight in its unit.  fp16 ends at 65504; the lower end is 2^3 to 2^4 below a new unit's largest weight, so that units change rarely after a
+// wave's first tiles (the cases take the same time as with one unit for all rows: 34.2 and 34.7 us, 36.0 and 35.5, 66 and 66, 25.6 and 25.1, 10.3 and 10.8).
+constexpr float kUnitLow = 1024.0f, kUnitTop = 32768.0f;
 constexpr int kUnitBits = 14;      // a new unit makes the largest weight so far less than 2^14, and at least half of that
 constexpr int kUnitLeast = -112;   // weights below 2^-112 get the unit of that: 2^126
 
