@@ -137,3 +137,36 @@ def test_entries_of_a_query_far_below_its_largest(gpu_device, codes):
     _, want, _, tol = CO.paged(q.to(BF16), kc, vc, ks, vs, torch.arange(2, dtype=torch.int32)[None], [32])
     CO.assert_close(norm, want, tol)
     assert (norm - want).abs()[0, 0] > 0.6 * tol[0, 0] and (norm - want).abs()[0, 1] < 1e-5
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("m", [1, 3])
+@pytest.mark.parametrize("least,most", [(112, 112), (-105, -105), (-105, 110), (-60, 60), (0, 0)])
+def test_value_scales_near_the_ends_of_fp32(gpu_device, codes, page, m, least, most):
+    """All values very large, or very small (as blocks of the smallest scale are), or of sizes drawn from a wide range, key by key; negative ones among them."""
+    g = torch.Generator().manual_seed(55)
+    lens, hk = [300, 150, m, 64], 2
+    pages = sum(-(-n // page) for n in lens)
+    kc, vc, ks, vs = make_cache(pages, hk, page, page, 64, CODES[codes], g)
+    vs *= torch.exp2(torch.randint(least, most + 1, vs.shape, generator=g).float()) * torch.where(torch.rand(vs.shape, generator=g) < 0.5, -1.0, 1.0)
+    table, at = torch.zeros(len(lens), 300 // page + 1, dtype=torch.int32), 0
+    for s, n in enumerate(lens):
+        table[s, :-(-n // page)] = torch.arange(at, at - (-n // page))
+        at -= -n // page
+    q = torch.randn(len(lens), m, 8, 64, generator=g).to(BF16)
+    check(q if m > 1 else q[:, 0], (kc, vc, ks, vs), table, lens, gpu_device)
+
+
+def test_scales_that_grow_along_a_sequence(gpu_device):
+    """Every tile's values are larger than all before, or every tile's keys count more than all before: units and references move at each step."""
+    g = torch.Generator().manual_seed(56)
+    page, n = 16, 1536
+    pages = n // page
+    for grows in (2, 3):
+        cache = list(make_cache(pages, 1, page, 1, 64, INT8, g, spread=0.2))
+        cache[0].copy_(cache[0].abs())
+        cache[grows] *= torch.exp2(torch.arange(pages).float() * (0.6 if grows == 3 else 0.05))[:, None, None]
+        q = 0.3 + 0.1 * torch.randn(1, 8, 64, generator=g)
+        for dtype in (BF16, FP16) if grows == 2 else (BF16,):
+            check(q.to(dtype), cache, torch.arange(pages, dtype=torch.int32)[None], [n], gpu_device, grows)
